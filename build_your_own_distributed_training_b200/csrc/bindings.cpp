@@ -63,6 +63,20 @@ void ce_peer_combine(std::vector<int64_t> bases, int64_t off, torch::Tensor labe
 void ce_loss_finish(torch::Tensor row_loss, torch::Tensor labels, int64_t vocab_total, int64_t ignore,
                     torch::Tensor loss, torch::Tensor inv_n);
 
+torch::Tensor qk_norm_rope_fwd(torch::Tensor x, torch::Tensor wq, torch::Tensor wk, torch::Tensor cos_t,
+                               torch::Tensor sin_t, c10::optional<torch::Tensor> pos, int64_t nq, int64_t nkv,
+                               int64_t hd, int64_t seqlen, double eps);
+torch::Tensor qk_norm_rope_bwd(torch::Tensor g, torch::Tensor x, torch::Tensor wq, torch::Tensor wk,
+                               torch::Tensor cos_t, torch::Tensor sin_t, c10::optional<torch::Tensor> pos, int64_t nq,
+                               int64_t nkv, int64_t hd, int64_t seqlen, double eps, torch::Tensor dwq,
+                               torch::Tensor dwk, bool accumulate);
+torch::Tensor dropout_add(torch::Tensor x, c10::optional<torch::Tensor> residual, int64_t cut, int64_t seed,
+                          int64_t start);
+std::vector<torch::Tensor> token_logprobs_fwd(torch::Tensor x, torch::Tensor tokens, double temperature, int64_t top_k,
+                                              int64_t ignore);
+void token_logprobs_bwd(torch::Tensor x, torch::Tensor tokens, torch::Tensor state, c10::optional<torch::Tensor> g_lp,
+                        c10::optional<torch::Tensor> g_ent, double temperature, torch::Tensor dx);
+
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.doc() = "sm_100a kernels for B200-native 2-D parallel LLaMA training";
   m.def("gemm", &gemm_entry, "tcgen05 GEMM with fused epilogues");
@@ -112,4 +126,9 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("ce_stats_reduce", &ce_stats_reduce);
   m.def("ce_peer_combine", &ce_peer_combine, "vocabulary-parallel log-sum-exp over the TP group's heaps");
   m.def("ce_loss_finish", &ce_loss_finish);
+  m.def("qk_norm_rope_fwd", &qk_norm_rope_fwd, "per-head RMSNorm of q and k with the rotary rotation, packed qkv");
+  m.def("qk_norm_rope_bwd", &qk_norm_rope_bwd);
+  m.def("dropout_add", &dropout_add, "residual + dropout(x), mask from Philox4x32-10 by element number");
+  m.def("token_logprobs_fwd", &token_logprobs_fwd, "log probabilities of given tokens, entropy, top alternatives");
+  m.def("token_logprobs_bwd", &token_logprobs_bwd);
 }

@@ -1,0 +1,455 @@
+// Per-head RMSNorm of queries and keys with the rotary rotation in the same pass (sm_100a).
+//
+// On the packed projection [q | k | v] of a token, for every query and key head x of hd elements:
+//
+//   r = 1 / sqrt(mean(x^2) + eps),  n = x r,  u = n w          (w: one [hd] weight for q, one for k)
+//   y_j = u_j c_j - u_{j+hd/2} s_j,  y_{j+hd/2} = u_{j+hd/2} c_j + u_j s_j      (j < hd/2)
+//
+// and v is carried over.  Backward, from g = dL/dy:  gu = R^T g,  dw = sum over tokens and heads of
+// gu n,  dx = r (gu w - n mean(gu w n)),  dv = g.  r is recomputed from x, which the backward reads
+// anyway, so nothing but the input is saved.
+//
+// Both directions are bound by memory.  A group of L lanes holds one head, each lane VEC elements of
+// the first half and their partners of the second, so the rotation needs no exchange and the only
+// cross-lane step is the L-lane sum.  A warp stays on one token: its cos/sin row and the weights are
+// read once and live in registers while the token's heads stream through.  Statistics, rotation and
+// weight gradients are fp32; y and dx are rounded once, to the storage type.
+//
+// dw: every warp adds up the heads of its tokens in registers, the block's warps are added in order
+// and written as one partial per block, and qk_dw_reduce_kernel adds the partials in order: the same
+// bits on every run.
+#include <ATen/cuda/CUDAContext.h>
+#include <c10/cuda/CUDAGuard.h>
+#include <torch/extension.h>
+
+#include <algorithm>
+
+#include "common.cuh"
+#include "vecio.cuh"
+
+namespace dtb {
+namespace qk {
+
+constexpr int NT = 256;  // threads per block
+
+struct Args {
+  const void* x;       // [tokens, ld]
+  long ld;
+  const void* g;       // backward: dL/dy [tokens, ldg]
+  long ldg;
+  void* out;           // y or dx, [tokens, ldo]
+  long ldo;
+  const void* wq;
+  const void* wk;
+  int wdt;             // storage type of the weights
+  const float* cos_t;  // [table_rows, hd]; the first hd/2 columns are read
+  const float* sin_t;
+  const void* pos;     // [tokens] int64 / int32, or null: token % seqlen
+  int pos64;
+  long tokens, table_rows, seqlen;
+  int nq, nkv, hd;
+  int lanes;           // lanes per head, a power of two
+  int split;           // warps that share a token's heads
+  float eps;
+  float* part;         // backward: [blocks, 2 hd]
+  int* err;
+};
+
+__device__ __forceinline__ long position(const Args& a, long token) {
+  if (a.pos == nullptr) return token % a.seqlen;
+  return a.pos64 ? (long)reinterpret_cast<const int64_t*>(a.pos)[token]
+                 : (long)reinterpret_cast<const int32_t*>(a.pos)[token];
+}
+
+// The lane's NP chunks of VEC pairs: chunk i starts at element (i * lanes + l) * VEC of either half.
+template <int VEC, int NP>
+struct Lane {
+  int off[NP];
+  bool on[NP];
+  __device__ __forceinline__ Lane(int l, int lanes, int half) {
+#pragma unroll
+    for (int i = 0; i < NP; ++i) {
+      off[i] = (i * lanes + l) * VEC;
+      on[i] = off[i] < half;
+    }
+  }
+};
+
+template <int VEC, int NP>
+__device__ __forceinline__ void load_table(const Args& a, const Lane<VEC, NP>& ln, long token, float (&c)[NP][VEC],
+                                           float (&s)[NP][VEC], int lane) {
+  const long pos = position(a, token);
+  const bool ok = pos >= 0 && pos < a.table_rows;
+  if (!ok && lane == 0) atomicExch(a.err, ERR_BAD_ARG);
+#pragma unroll
+  for (int i = 0; i < NP; ++i) {
+    Pack<float, VEC> pc, ps;
+    if (ok && ln.on[i]) {
+      pc.load(a.cos_t + pos * a.hd + ln.off[i]);
+      ps.load(a.sin_t + pos * a.hd + ln.off[i]);
+    }
+#pragma unroll
+    for (int v = 0; v < VEC; ++v) {
+      // a position outside the table gives NaN heads and sets the device error word
+      c[i][v] = ok ? (ln.on[i] ? pc.at(v) : 0.f) : __int_as_float(0x7fc00000);
+      s[i][v] = ok ? (ln.on[i] ? ps.at(v) : 0.f) : __int_as_float(0x7fc00000);
+    }
+  }
+}
+
+template <int VEC, int NP>
+__device__ __forceinline__ void load_weight(const void* w, int wdt, const Lane<VEC, NP>& ln, int half,
+                                            float (&lo)[NP][VEC], float (&hi)[NP][VEC]) {
+#pragma unroll
+  for (int i = 0; i < NP; ++i)
+#pragma unroll
+    for (int v = 0; v < VEC; ++v) {
+      lo[i][v] = ln.on[i] ? load_as(w, ln.off[i] + v, wdt) : 0.f;
+      hi[i][v] = ln.on[i] ? load_as(w, ln.off[i] + half + v, wdt) : 0.f;
+    }
+}
+
+__device__ __forceinline__ float group_sum(float v, int lanes) {
+  for (int o = lanes >> 1; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+  return v;
+}
+
+// U heads are in flight per lane group.
+template <typename T, int VEC, int NP, int U>
+__global__ void __launch_bounds__(NT) qk_fwd_kernel(const Args a) {
+  const int lane = threadIdx.x & 31;
+  const long item = (long)blockIdx.x * (NT / 32) + (threadIdx.x >> 5);
+  if (item >= a.tokens * a.split) return;
+  const long token = item / a.split;
+  const int part = (int)(item % a.split);
+  const int half = a.hd >> 1, heads = a.nq + 2 * a.nkv, per = 32 / a.lanes;
+  const Lane<VEC, NP> ln(lane & (a.lanes - 1), a.lanes, half);
+  const int grp = lane / a.lanes;
+  const T* x = reinterpret_cast<const T*>(a.x) + token * a.ld;
+  T* y = reinterpret_cast<T*>(a.out) + token * a.ldo;
+  float c[NP][VEC], s[NP][VEC], wl[2][NP][VEC], wh[2][NP][VEC];
+  load_table(a, ln, token, c, s, lane);
+  load_weight(a.wq, a.wdt, ln, half, wl[0], wh[0]);
+  load_weight(a.wk, a.wdt, ln, half, wl[1], wh[1]);
+  const float inv_hd = 1.f / (float)a.hd;
+  const int stride = per * a.split;
+  for (int h0 = part * per; h0 < heads; h0 += U * stride) {
+    Pack<T, VEC> lo[U][NP], hi[U][NP];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int h = h0 + u * stride + grp;
+#pragma unroll
+      for (int i = 0; i < NP; ++i)
+        if (h < heads && ln.on[i]) {
+          lo[u][i].load(x + (long)h * a.hd + ln.off[i]);
+          hi[u][i].load(x + (long)h * a.hd + half + ln.off[i]);
+        } else {
+#pragma unroll
+          for (int v = 0; v < VEC; ++v) lo[u][i].set(v, 0.f), hi[u][i].set(v, 0.f);
+        }
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int h = h0 + u * stride + grp;
+      float ss = 0.f;
+#pragma unroll
+      for (int i = 0; i < NP; ++i)
+#pragma unroll
+        for (int v = 0; v < VEC; ++v) {
+          const float p = lo[u][i].at(v), q = hi[u][i].at(v);
+          ss = fmaf(p, p, fmaf(q, q, ss));
+        }
+      ss = group_sum(ss, a.lanes);
+      if (h >= heads) continue;
+      if (h < a.nq + a.nkv) {
+        const float r = rsqrtf(ss * inv_hd + a.eps);
+        const bool key = h >= a.nq;
+#pragma unroll
+        for (int i = 0; i < NP; ++i)
+#pragma unroll
+          for (int v = 0; v < VEC; ++v) {
+            const float ul = lo[u][i].at(v) * r * (key ? wl[1][i][v] : wl[0][i][v]);
+            const float uh = hi[u][i].at(v) * r * (key ? wh[1][i][v] : wh[0][i][v]);
+            lo[u][i].set(v, ul * c[i][v] - uh * s[i][v]);
+            hi[u][i].set(v, uh * c[i][v] + ul * s[i][v]);
+          }
+      }
+#pragma unroll
+      for (int i = 0; i < NP; ++i)
+        if (ln.on[i]) {
+          lo[u][i].store(y + (long)h * a.hd + ln.off[i]);
+          hi[u][i].store(y + (long)h * a.hd + half + ln.off[i]);
+        }
+    }
+  }
+}
+
+template <typename T, int VEC, int NP>
+__global__ void __launch_bounds__(NT) qk_bwd_kernel(const Args a) {
+  extern __shared__ float sh[];  // [NT / 32][2 hd]
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int half = a.hd >> 1, heads = a.nq + 2 * a.nkv, per = 32 / a.lanes;
+  const Lane<VEC, NP> ln(lane & (a.lanes - 1), a.lanes, half);
+  const int grp = lane / a.lanes;
+  const float inv_hd = 1.f / (float)a.hd;
+  const int stride = per * a.split;
+  float wl[2][NP][VEC], wh[2][NP][VEC], dl[2][NP][VEC], dh[2][NP][VEC];
+  load_weight(a.wq, a.wdt, ln, half, wl[0], wh[0]);
+  load_weight(a.wk, a.wdt, ln, half, wl[1], wh[1]);
+#pragma unroll
+  for (int t = 0; t < 2; ++t)
+#pragma unroll
+    for (int i = 0; i < NP; ++i)
+#pragma unroll
+      for (int v = 0; v < VEC; ++v) dl[t][i][v] = 0.f, dh[t][i][v] = 0.f;
+  for (long item = (long)blockIdx.x * (NT / 32) + warp; item < a.tokens * a.split;
+       item += (long)gridDim.x * (NT / 32)) {
+    const long token = item / a.split;
+    const int part = (int)(item % a.split);
+    const T* x = reinterpret_cast<const T*>(a.x) + token * a.ld;
+    const T* g = reinterpret_cast<const T*>(a.g) + token * a.ldg;
+    T* dx = reinterpret_cast<T*>(a.out) + token * a.ldo;
+    float c[NP][VEC], s[NP][VEC];
+    load_table(a, ln, token, c, s, lane);
+    for (int h0 = part * per; h0 < heads; h0 += stride) {
+      const int h = h0 + grp;
+      const bool norm = h < a.nq + a.nkv;
+      Pack<T, VEC> xl[NP], xh[NP], gl[NP], gh[NP];
+#pragma unroll
+      for (int i = 0; i < NP; ++i) {
+        if (h < heads && ln.on[i]) {
+          gl[i].load(g + (long)h * a.hd + ln.off[i]);
+          gh[i].load(g + (long)h * a.hd + half + ln.off[i]);
+        } else {
+#pragma unroll
+          for (int v = 0; v < VEC; ++v) gl[i].set(v, 0.f), gh[i].set(v, 0.f);
+        }
+        if (norm && ln.on[i]) {
+          xl[i].load(x + (long)h * a.hd + ln.off[i]);
+          xh[i].load(x + (long)h * a.hd + half + ln.off[i]);
+        } else {
+#pragma unroll
+          for (int v = 0; v < VEC; ++v) xl[i].set(v, 0.f), xh[i].set(v, 0.f);
+        }
+      }
+      // one exchange for both sums: sum x^2 and sum gu w x (n = x r, so mean(gu w n) = r mean(gu w x))
+      float ss = 0.f, dot = 0.f;
+      const bool key = h >= a.nq;
+#pragma unroll
+      for (int i = 0; i < NP; ++i)
+#pragma unroll
+        for (int v = 0; v < VEC; ++v) {
+          const float p = xl[i].at(v), q = xh[i].at(v), e = gl[i].at(v), f = gh[i].at(v);
+          const float ul = e * c[i][v] + f * s[i][v], uh = f * c[i][v] - e * s[i][v];
+          ss = fmaf(p, p, fmaf(q, q, ss));
+          dot += ul * (key ? wl[1][i][v] : wl[0][i][v]) * p + uh * (key ? wh[1][i][v] : wh[0][i][v]) * q;
+        }
+      ss = group_sum(ss, a.lanes);
+      dot = group_sum(dot, a.lanes);
+      if (h >= heads) continue;
+      if (norm) {
+        const float r = rsqrtf(ss * inv_hd + a.eps);
+        const float m = r * dot * inv_hd;  // mean(gu w n)
+#pragma unroll
+        for (int i = 0; i < NP; ++i)
+#pragma unroll
+          for (int v = 0; v < VEC; ++v) {
+            const float nl = xl[i].at(v) * r, nh = xh[i].at(v) * r, e = gl[i].at(v), f = gh[i].at(v);
+            const float ul = e * c[i][v] + f * s[i][v], uh = f * c[i][v] - e * s[i][v];
+            gl[i].set(v, r * (ul * (key ? wl[1][i][v] : wl[0][i][v]) - nl * m));
+            gh[i].set(v, r * (uh * (key ? wh[1][i][v] : wh[0][i][v]) - nh * m));
+            if (key) {
+              dl[1][i][v] += ul * nl;
+              dh[1][i][v] += uh * nh;
+            } else {
+              dl[0][i][v] += ul * nl;
+              dh[0][i][v] += uh * nh;
+            }
+          }
+      }
+#pragma unroll
+      for (int i = 0; i < NP; ++i)
+        if (ln.on[i]) {
+          gl[i].store(dx + (long)h * a.hd + ln.off[i]);
+          gh[i].store(dx + (long)h * a.hd + half + ln.off[i]);
+        }
+    }
+  }
+  // the groups of a warp, then the warps of the block, in a fixed order
+#pragma unroll
+  for (int t = 0; t < 2; ++t)
+#pragma unroll
+    for (int i = 0; i < NP; ++i)
+#pragma unroll
+      for (int v = 0; v < VEC; ++v) {
+        float l = dl[t][i][v], h = dh[t][i][v];
+        for (int o = a.lanes; o < 32; o <<= 1) {
+          l += __shfl_xor_sync(0xffffffffu, l, o);
+          h += __shfl_xor_sync(0xffffffffu, h, o);
+        }
+        if (grp == 0 && ln.on[i]) {
+          float* row = sh + (long)warp * 2 * a.hd + t * a.hd;
+          row[ln.off[i] + v] = l;
+          row[ln.off[i] + half + v] = h;
+        }
+      }
+  __syncthreads();
+  for (int j = threadIdx.x; j < 2 * a.hd; j += NT) {
+    float t = 0.f;
+#pragma unroll
+    for (int w = 0; w < NT / 32; ++w) t += sh[w * 2 * a.hd + j];
+    a.part[(long)blockIdx.x * 2 * a.hd + j] = t;
+  }
+}
+
+// Column sums of part[nparts, 2 hd] in a fixed order (32 warps, each every 32nd row, added in warp
+// order): columns [0, hd) to dq, [hd, 2 hd) to dk, stored in their own type or added to fp32.
+__global__ void __launch_bounds__(1024) qk_dw_reduce_kernel(const float* __restrict__ part, int nparts, int hd,
+                                                            void* dq, void* dk, int dt, int accumulate) {
+  __shared__ float red[32][33];
+  const int w = threadIdx.x >> 5, l = threadIdx.x & 31;
+  const int col = blockIdx.x * 32 + l;
+  float s = 0.f;
+  if (col < 2 * hd)
+    for (int b = w; b < nparts; b += 32) s += part[(long)b * 2 * hd + col];
+  red[w][l] = s;
+  __syncthreads();
+  if (w == 0 && col < 2 * hd) {
+    float t = 0.f;
+#pragma unroll
+    for (int i = 0; i < 32; ++i) t += red[i][l];
+    void* d = col < hd ? dq : dk;
+    const int j = col < hd ? col : col - hd;
+    if (accumulate) t += reinterpret_cast<float*>(d)[j];
+    store_as(d, j, dt, t);
+  }
+}
+
+}  // namespace qk
+}  // namespace dtb
+
+using namespace dtb;
+
+namespace {
+
+// Fills what both directions share and chooses the lane layout: 16-byte vectors when the head is a
+// multiple of 16 elements and every row starts on a 16-byte boundary, single elements otherwise.
+bool qk_common(qk::Args& a, const char* op, const torch::Tensor& x, const torch::Tensor& wq, const torch::Tensor& wk,
+               const torch::Tensor& cos_t, const torch::Tensor& sin_t, const c10::optional<torch::Tensor>& pos,
+               int64_t nq, int64_t nkv, int64_t hd, int64_t seqlen, double eps) {
+  DTB_CHECK(x.is_cuda() && x.dim() == 2 && is_float_type(x.scalar_type()), "%s: qkv must be a 2-D CUDA tensor of fp32, bf16 or fp16", op);
+  DTB_CHECK(nq > 0 && nkv > 0 && hd > 0 && hd % 2 == 0 && hd <= 512, "%s: needs heads > 0 and an even head size up to 512 (nq=%ld nkv=%ld hd=%ld)", op, (long)nq, (long)nkv, (long)hd);
+  DTB_CHECK(x.size(1) == (nq + 2 * nkv) * hd, "%s: qkv has %ld columns, (nq + 2 nkv) * head_dim = %ld", op, (long)x.size(1), (long)((nq + 2 * nkv) * hd));
+  DTB_CHECK(x.numel() == 0 || x.stride(1) == 1, "%s: qkv columns must be contiguous", op);
+  for (const torch::Tensor* w : {&wq, &wk})
+    DTB_CHECK(w->is_cuda() && w->is_contiguous() && w->numel() == hd && is_float_type(w->scalar_type()) && w->scalar_type() == wq.scalar_type(), "%s: the norm weights must be contiguous [%ld] tensors of one float type on the GPU", op, (long)hd);
+  for (const torch::Tensor* t : {&cos_t, &sin_t})
+    DTB_CHECK(t->is_cuda() && t->scalar_type() == at::kFloat && t->is_contiguous() && t->dim() == 2 && t->size(1) == hd && t->size(0) == cos_t.size(0), "%s: cos and sin must be contiguous fp32 [positions, %ld]", op, (long)hd);
+  for (const torch::Tensor* t : {&wq, &wk, &cos_t, &sin_t})
+    DTB_CHECK(t->device() == x.device(), "%s: all tensors must be on one device", op);
+  a.x = x.data_ptr();
+  a.ld = x.stride(0);
+  a.wq = wq.data_ptr();
+  a.wk = wk.data_ptr();
+  a.wdt = dt_code(wq.scalar_type());
+  a.cos_t = cos_t.data_ptr<float>();
+  a.sin_t = sin_t.data_ptr<float>();
+  a.tokens = x.size(0);
+  a.table_rows = cos_t.size(0);
+  a.seqlen = seqlen;
+  if (pos.has_value()) {
+    DTB_CHECK(pos->device() == x.device() && pos->is_contiguous() && pos->numel() == x.size(0) && (pos->scalar_type() == at::kLong || pos->scalar_type() == at::kInt), "%s: positions must be a contiguous int64 or int32 tensor with one entry per token, on the tokens' device", op);
+    a.pos = pos->data_ptr();
+    a.pos64 = pos->scalar_type() == at::kLong;
+  } else {
+    DTB_CHECK(seqlen > 0 && (seqlen <= cos_t.size(0) || x.size(0) <= cos_t.size(0)), "%s: seqlen=%ld needs as many table rows (have %ld)", op, (long)seqlen, (long)cos_t.size(0));
+  }
+  a.nq = (int)nq;
+  a.nkv = (int)nkv;
+  a.hd = (int)hd;
+  a.eps = (float)eps;
+  a.err = dtb_error_word();
+  const long es = (long)x.element_size();
+  return hd % 16 == 0 && (reinterpret_cast<uintptr_t>(a.x) & 15) == 0 && (a.ld * es) % 16 == 0 &&
+         (reinterpret_cast<uintptr_t>(a.cos_t) & 15) == 0 && (reinterpret_cast<uintptr_t>(a.sin_t) & 15) == 0;
+}
+
+void qk_lanes(qk::Args& a, bool vec) {
+  int lanes = 32;
+  if (vec) {
+    lanes = 1;
+    while (lanes * 16 < a.hd) lanes *= 2;
+  }
+  a.lanes = lanes;
+  // few tokens: their heads are spread over more warps, down to one round of heads per warp
+  const int per = 32 / lanes, rounds = (a.nq + 2 * a.nkv + per - 1) / per;
+  const long want = (long)device_sm_count() * 32;
+  long split = a.tokens > 0 ? want / a.tokens : 1;
+  a.split = (int)std::max(1L, std::min<long>(split, rounds));
+}
+
+}  // namespace
+
+torch::Tensor qk_norm_rope_fwd(torch::Tensor x, torch::Tensor wq, torch::Tensor wk, torch::Tensor cos_t,
+                               torch::Tensor sin_t, c10::optional<torch::Tensor> pos, int64_t nq, int64_t nkv,
+                               int64_t hd, int64_t seqlen, double eps) {
+  const c10::cuda::CUDAGuard guard(x.device());
+  qk::Args a{};
+  const bool vec = qk_common(a, "qk_norm_rope", x, wq, wk, cos_t, sin_t, pos, nq, nkv, hd, seqlen, eps);
+  auto y = torch::empty({x.size(0), x.size(1)}, x.options());
+  if (x.size(0) == 0) return y;
+  a.out = y.data_ptr();
+  a.ldo = y.stride(0);
+  qk_lanes(a, vec);
+  const long blocks = (a.tokens * a.split + qk::NT / 32 - 1) / (qk::NT / 32);
+  DTB_CHECK(blocks < (1L << 31), "qk_norm_rope: too many tokens");
+  auto st = at::cuda::getCurrentCUDAStream();
+  DTB_FLOAT_TYPES(x.scalar_type(), {
+    if (vec) qk::qk_fwd_kernel<T, 8, 1, sizeof(T) == 4 ? 2 : 4><<<(unsigned)blocks, qk::NT, 0, st>>>(a);
+    else qk::qk_fwd_kernel<T, 1, 8, 1><<<(unsigned)blocks, qk::NT, 0, st>>>(a);
+  });
+  DTB_LAUNCH_CHECK();
+  return y;
+}
+
+// dx; the weight gradients go to dwq / dwk: stored in their type, or added to fp32 when `accumulate`.
+torch::Tensor qk_norm_rope_bwd(torch::Tensor g, torch::Tensor x, torch::Tensor wq, torch::Tensor wk,
+                               torch::Tensor cos_t, torch::Tensor sin_t, c10::optional<torch::Tensor> pos, int64_t nq,
+                               int64_t nkv, int64_t hd, int64_t seqlen, double eps, torch::Tensor dwq,
+                               torch::Tensor dwk, bool accumulate) {
+  const c10::cuda::CUDAGuard guard(x.device());
+  qk::Args a{};
+  bool vec = qk_common(a, "qk_norm_rope backward", x, wq, wk, cos_t, sin_t, pos, nq, nkv, hd, seqlen, eps);
+  DTB_CHECK(g.device() == x.device() && g.sizes() == x.sizes() && g.scalar_type() == x.scalar_type() && (g.numel() == 0 || g.stride(1) == 1), "qk_norm_rope backward: the gradient must have the input's shape and type and contiguous columns");
+  for (const torch::Tensor* d : {&dwq, &dwk})
+    DTB_CHECK(d->device() == x.device() && d->is_contiguous() && d->numel() == hd && is_float_type(d->scalar_type()) && d->scalar_type() == dwq.scalar_type() && (!accumulate || d->scalar_type() == at::kFloat), "qk_norm_rope backward: weight gradients must be contiguous [%ld] tensors of one float type (fp32 to accumulate)", (long)hd);
+  auto dx = torch::empty({x.size(0), x.size(1)}, x.options());
+  if (x.size(0) == 0) {
+    if (!accumulate) {
+      dwq.zero_();
+      dwk.zero_();
+    }
+    return dx;
+  }
+  a.g = g.data_ptr();
+  a.ldg = g.stride(0);
+  a.out = dx.data_ptr();
+  a.ldo = dx.stride(0);
+  vec = vec && (reinterpret_cast<uintptr_t>(a.g) & 15) == 0 && (a.ldg * (long)x.element_size()) % 16 == 0;
+  qk_lanes(a, vec);
+  const int warps = qk::NT / 32;
+  const int blocks = (int)std::min<long>((a.tokens * a.split + warps - 1) / warps, (long)device_sm_count() * 2);
+  auto part = torch::empty({blocks, 2 * hd}, x.options().dtype(at::kFloat));
+  a.part = part.data_ptr<float>();
+  auto st = at::cuda::getCurrentCUDAStream();
+  const size_t smem = sizeof(float) * warps * 2 * hd;
+  DTB_FLOAT_TYPES(x.scalar_type(), {
+    if (vec) qk::qk_bwd_kernel<T, 8, 1><<<blocks, qk::NT, smem, st>>>(a);
+    else qk::qk_bwd_kernel<T, 1, 8><<<blocks, qk::NT, smem, st>>>(a);
+  });
+  DTB_LAUNCH_CHECK();
+  qk::qk_dw_reduce_kernel<<<(unsigned)((2 * hd + 31) / 32), 1024, 0, st>>>(
+      a.part, blocks, (int)hd, dwq.data_ptr(), dwk.data_ptr(), dt_code(dwq.scalar_type()), accumulate ? 1 : 0);
+  DTB_LAUNCH_CHECK();
+  return dx;
+}

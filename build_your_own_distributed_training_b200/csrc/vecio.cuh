@@ -1,0 +1,90 @@
+// Element types and 16-byte vector access shared by the elementwise and row kernels:
+// fp32, bf16 and fp16 storage, arithmetic in fp32.
+#pragma once
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <stdint.h>
+
+namespace dtb {
+
+template <typename T>
+__device__ __forceinline__ float as_float(T v);
+template <>
+__device__ __forceinline__ float as_float<float>(float v) { return v; }
+template <>
+__device__ __forceinline__ float as_float<__nv_bfloat16>(__nv_bfloat16 v) { return __bfloat162float(v); }
+template <>
+__device__ __forceinline__ float as_float<__half>(__half v) { return __half2float(v); }
+
+template <typename T>
+__device__ __forceinline__ T from_float(float v);
+template <>
+__device__ __forceinline__ float from_float<float>(float v) { return v; }
+template <>
+__device__ __forceinline__ __nv_bfloat16 from_float<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
+template <>
+__device__ __forceinline__ __half from_float<__half>(float v) { return __float2half_rn(v); }
+
+// VEC consecutive elements as they lie in memory: 16-byte words where VEC * sizeof(T) is a
+// multiple of 16 (the address must then be 16-byte aligned), single elements otherwise.
+template <typename T, int VEC>
+struct Pack {
+  static constexpr bool WIDE = (VEC * sizeof(T)) % 16 == 0;
+  static constexpr int WORDS = WIDE ? (int)(VEC * sizeof(T) / 16) : 1;
+  union {
+    uint4 w[WORDS];
+    T e[VEC];
+  };
+  __device__ __forceinline__ Pack() {}
+  __device__ __forceinline__ void load(const T* p) {
+    if constexpr (WIDE) {
+#pragma unroll
+      for (int i = 0; i < WORDS; ++i) w[i] = __ldg(reinterpret_cast<const uint4*>(p) + i);
+    } else {
+#pragma unroll
+      for (int i = 0; i < VEC; ++i) e[i] = p[i];
+    }
+  }
+  __device__ __forceinline__ void store(T* p) const {
+    if constexpr (WIDE) {
+#pragma unroll
+      for (int i = 0; i < WORDS; ++i) reinterpret_cast<uint4*>(p)[i] = w[i];
+    } else {
+#pragma unroll
+      for (int i = 0; i < VEC; ++i) p[i] = e[i];
+    }
+  }
+  __device__ __forceinline__ float at(int i) const { return as_float<T>(e[i]); }
+  __device__ __forceinline__ void set(int i, float v) { e[i] = from_float<T>(v); }
+};
+
+// storage type of an operand whose type is chosen at run time
+enum : int { DT_F32 = 0, DT_BF16 = 1, DT_F16 = 2 };
+
+__device__ __forceinline__ float load_as(const void* p, long i, int dt) {
+  if (dt == DT_F32) return reinterpret_cast<const float*>(p)[i];
+  if (dt == DT_BF16) return __bfloat162float(reinterpret_cast<const __nv_bfloat16*>(p)[i]);
+  return __half2float(reinterpret_cast<const __half*>(p)[i]);
+}
+__device__ __forceinline__ void store_as(void* p, long i, int dt, float v) {
+  if (dt == DT_F32) reinterpret_cast<float*>(p)[i] = v;
+  else if (dt == DT_BF16) reinterpret_cast<__nv_bfloat16*>(p)[i] = __float2bfloat16_rn(v);
+  else reinterpret_cast<__half*>(p)[i] = __float2half_rn(v);
+}
+
+}  // namespace dtb
+
+#ifdef TORCH_EXTENSION_NAME
+#include <torch/extension.h>
+namespace dtb {
+inline bool is_float_type(at::ScalarType t) { return t == at::kFloat || t == at::kBFloat16 || t == at::kHalf; }
+inline int dt_code(at::ScalarType t) { return t == at::kFloat ? DT_F32 : t == at::kBFloat16 ? DT_BF16 : DT_F16; }
+}  // namespace dtb
+// runs `...` with T the storage type of scalar type `st`
+#define DTB_FLOAT_TYPES(st, ...)                                   \
+  do {                                                             \
+    if ((st) == at::kFloat) { using T = float; __VA_ARGS__; }      \
+    else if ((st) == at::kBFloat16) { using T = __nv_bfloat16; __VA_ARGS__; } \
+    else { using T = __half; __VA_ARGS__; }                        \
+  } while (0)
+#endif

@@ -14,3 +14,6 @@ from .rope import apply_rotary_emb, precompute_rope_cache  # noqa: F401
 from .attention import causal_attention  # noqa: F401
 from .loss import lm_head_cross_entropy  # noqa: F401
 from .embedding import embedding  # noqa: F401
+from .qk_norm import qk_norm_rope  # noqa: F401
+from .dropout import dropout_add  # noqa: F401
+from .logprobs import TokenLogProbs, lm_head_token_log_probs, token_log_probs  # noqa: F401

@@ -1,0 +1,123 @@
+"""Per-head RMSNorm of queries and keys with the rotary rotation in the same pass.
+
+On the packed ``[q | k | v]`` projection every query and key head ``x`` becomes
+``R(x * rsqrt(mean(x^2) + eps) * w)`` with one ``[head_dim]`` weight for the query heads and one
+for the key heads (shared by all heads) and the rotate-half rotation ``R`` of the token's position;
+the value heads are carried over.  The result is what :func:`..attention.causal_attention` reads.
+
+With normalised queries and keys the rotation cannot ride in the projection's GEMM epilogue (the
+norm comes between them), so this op takes its place.  On CUDA it is one kernel forward and two
+backward (``csrc/qk_norm_rope.cu``): statistics and weight gradients in fp32, sums in a fixed order,
+nothing saved but the input.  No reference counterpart: the reference's attention
+(``src/model/attention.py:109-155``) rotates unnormalised heads.
+"""
+
+from __future__ import annotations
+
+import torch
+
+from . import grad_state
+from ._ext import native
+
+
+def _rotate(u: torch.Tensor, c: torch.Tensor, s: torch.Tensor) -> torch.Tensor:
+    h = u.shape[-1] // 2
+    lo, hi = u[..., :h], u[..., h:]
+    return torch.cat((lo * c - hi * s, hi * c + lo * s), dim=-1)
+
+
+def _tables(cos: torch.Tensor, sin: torch.Tensor, positions: torch.Tensor | None, tokens: int, seqlen: int,
+            hd: int) -> tuple[torch.Tensor, torch.Tensor]:
+    pos = torch.arange(tokens, device=cos.device) % seqlen if positions is None else positions.long()
+    return cos[pos, None, : hd // 2].float(), sin[pos, None, : hd // 2].float()
+
+
+def qk_norm_rope_reference(qkv: torch.Tensor, q_weight: torch.Tensor, k_weight: torch.Tensor, cos: torch.Tensor,
+                           sin: torch.Tensor, nq: int, nkv: int, hd: int, seqlen: int, eps: float,
+                           positions: torch.Tensor | None = None) -> torch.Tensor:
+    """The op in plain differentiable PyTorch: fp32 math, rounded once."""
+    x = qkv.float().view(qkv.shape[0], nq + 2 * nkv, hd)
+    c, s = _tables(cos, sin, positions, qkv.shape[0], seqlen, hd)
+    w = torch.cat((q_weight.float().expand(nq, hd), k_weight.float().expand(nkv, hd)))
+    a = x[:, : nq + nkv]
+    u = a * torch.rsqrt(a.pow(2).mean(-1, keepdim=True) + eps) * w
+    return torch.cat((_rotate(u, c, s), x[:, nq + nkv:]), dim=1).to(qkv.dtype).view(qkv.shape)
+
+
+def _backward_cpu(g, x, wq, wk, cos, sin, pos, nq, nkv, hd, seqlen, eps):
+    x3 = x.float().view(-1, nq + 2 * nkv, hd)
+    g3 = g.float().view(-1, nq + 2 * nkv, hd)
+    c, s = _tables(cos, sin, pos, x.shape[0], seqlen, hd)
+    w = torch.cat((wq.float().expand(nq, hd), wk.float().expand(nkv, hd)))
+    a = x3[:, : nq + nkv]
+    r = torch.rsqrt(a.pow(2).mean(-1, keepdim=True) + eps)
+    n = a * r
+    gu = _rotate(g3[:, : nq + nkv], c, -s)  # the transposed rotation
+    gn = gu * w
+    da = r * (gn - n * (gn * n).mean(-1, keepdim=True))
+    dw = (gu * n).sum(0)
+    dx = torch.cat((da, g3[:, nq + nkv:]), dim=1).to(x.dtype).view(x.shape)
+    return dx, dw[:nq].sum(0), dw[nq:].sum(0)
+
+
+class _QKNormRopeFn(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, qkv, wq, wk, cos, sin, positions, nq, nkv, hd, seqlen, eps, main_grads):  # type: ignore[override]
+        if qkv.is_cuda:
+            y = native().qk_norm_rope_fwd(qkv, wq, wk, cos, sin, positions, nq, nkv, hd, seqlen, eps)
+        else:
+            y = qk_norm_rope_reference(qkv, wq, wk, cos, sin, nq, nkv, hd, seqlen, eps, positions)
+        ctx.save_for_backward(qkv, wq, wk, cos, sin, positions)
+        ctx.cfg = (nq, nkv, hd, seqlen, eps)
+        ctx.main_grads = main_grads
+        return y
+
+    @staticmethod
+    def backward(ctx, g):  # type: ignore[override]
+        qkv, wq, wk, cos, sin, positions = ctx.saved_tensors
+        nq, nkv, hd, seqlen, eps = ctx.cfg
+        mgs = ctx.main_grads
+        if mgs is not None:
+            for mg in mgs:
+                grad_state.zero_if_fresh(mg)  # the weight gradients accumulate
+        if qkv.is_cuda:
+            if g.stride(-1) != 1:
+                g = g.contiguous()
+            dwq, dwk = mgs if mgs is not None else (torch.empty_like(wq), torch.empty_like(wk))
+            dx = native().qk_norm_rope_bwd(g, qkv, wq, wk, cos, sin, positions, nq, nkv, hd, seqlen, eps,
+                                           dwq, dwk, mgs is not None)
+        else:
+            dx, fq, fk = _backward_cpu(g, qkv, wq, wk, cos, sin, positions, nq, nkv, hd, seqlen, eps)
+            dwq, dwk = fq.to(wq.dtype), fk.to(wk.dtype)
+            if mgs is not None:
+                mgs[0].add_(fq)
+                mgs[1].add_(fk)
+        if mgs is not None:
+            dwq = dwk = None
+        return (dx, dwq, dwk) + (None,) * 9
+
+
+def qk_norm_rope(qkv: torch.Tensor, q_weight: torch.Tensor, k_weight: torch.Tensor, cos: torch.Tensor,
+                 sin: torch.Tensor, n_q_heads: int, n_kv_heads: int, head_dim: int, seqlen: int,
+                 eps: float = 1e-5, *, positions: torch.Tensor | None = None,
+                 main_grads: tuple[torch.Tensor, torch.Tensor] | None = None) -> torch.Tensor:
+    """``qkv: [tokens, (nq + 2 nkv) * hd]`` -> the same shape, q and k normalised and rotated.
+
+    Token ``m`` is at position ``m % seqlen``, or at ``positions[m]`` (int64 or int32: packed
+    sequences, decoding) of the fp32 tables ``cos``/``sin`` ``[positions, hd]``; a position outside
+    the tables gives NaN and sets the device error word.  ``qkv`` is fp32, bf16 or fp16 with any row
+    stride; the weights share one float type.  With ``main_grads`` (the engine's fp32 gradient views
+    of the two weights) the weight gradients are added there.
+    """
+    if qkv.dim() != 2 or qkv.shape[1] != (n_q_heads + 2 * n_kv_heads) * head_dim:
+        raise ValueError(f"qkv must be [tokens, {(n_q_heads + 2 * n_kv_heads) * head_dim}], got {tuple(qkv.shape)}")
+    if head_dim % 2:
+        raise ValueError(f"the rotation needs an even head_dim, got {head_dim}")
+    if positions is not None:
+        positions = positions.reshape(-1).contiguous()
+        if positions.numel() != qkv.shape[0]:
+            raise ValueError(f"{positions.numel()} positions for {qkv.shape[0]} tokens")
+    if qkv.stride(1) != 1:
+        qkv = qkv.contiguous()
+    return _QKNormRopeFn.apply(qkv, q_weight, k_weight, cos, sin, positions, n_q_heads, n_kv_heads, head_dim,
+                               seqlen, eps, main_grads)
