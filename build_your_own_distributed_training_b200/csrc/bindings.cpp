@@ -76,6 +76,9 @@ std::vector<torch::Tensor> token_logprobs_fwd(torch::Tensor x, torch::Tensor tok
                                               int64_t ignore);
 void token_logprobs_bwd(torch::Tensor x, torch::Tensor tokens, torch::Tensor state, c10::optional<torch::Tensor> g_lp,
                         c10::optional<torch::Tensor> g_ent, double temperature, torch::Tensor dx);
+std::vector<torch::Tensor> fp8_quantize(torch::Tensor x, bool square, bool plain, bool transposed);
+void fp8_gemm(torch::Tensor A, torch::Tensor sA, int64_t granA, torch::Tensor B, torch::Tensor sB, int64_t granB,
+              torch::Tensor D, c10::optional<torch::Tensor> R, bool accumulate);
 
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.doc() = "sm_100a kernels for B200-native 2-D parallel LLaMA training";
@@ -131,4 +134,6 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("dropout_add", &dropout_add, "residual + dropout(x), mask from Philox4x32-10 by element number");
   m.def("token_logprobs_fwd", &token_logprobs_fwd, "log probabilities of given tokens, entropy, top alternatives");
   m.def("token_logprobs_bwd", &token_logprobs_bwd);
+  m.def("fp8_quantize", &fp8_quantize, "e4m3 codes with a power-of-two scale per block of 128, as they lie and / or transposed");
+  m.def("fp8_gemm", &fp8_gemm, "tcgen05 block-scaled product of e4m3 operands");
 }

@@ -1,0 +1,271 @@
+// Quantisation to 8-bit floating point (e4m3) with one power-of-two scale for each block of 128.
+//
+// A block's scale is the least 2^e with max|x| <= 448 * 2^e (448 = 1.75 * 2^8 is the largest e4m3
+// number), stored as its biased exponent (e8m0); x * 2^-e is exact, so the only rounding is the one to
+// e4m3 (nearest even).  Blocks are 1 x 128 along the axis that a product sums over (activations and
+// gradients) or 128 x 128 (weights, whose codes then serve both products that read them).  A block whose
+// largest magnitude is below 2^-100, zeros included, takes the scale for 2^-100; NaN or infinity in a
+// block makes its scale NaN, so every product it enters is NaN.
+//
+// Training needs each operand along two axes: activations along features (forward) and along tokens
+// (weight gradient).  One kernel reads a 128 x 128 tile once, holds it in registers (8 x 8 elements per
+// thread), and writes the codes as they lie and transposed, so that both products get operands whose
+// summed axis is contiguous.  Bound by memory: 2 bytes in, 1 or 2 bytes out per element.  The transposed
+// codes go through 16 KB of shared memory in 8-byte chunks (8 rows of one column) at chunk
+// rg ^ (column / 8), which is free of bank conflicts on the way in, and leave as 16-byte stores.
+//
+// Scales of 1 x 128 blocks are stored block-major, s[block][row]: the product reads the scales of 128
+// rows of one block together.
+#include <ATen/cuda/CUDAContext.h>
+#include <c10/cuda/CUDAGuard.h>
+#include <cuda_fp8.h>
+#include <torch/extension.h>
+
+#include <algorithm>
+
+#include "common.cuh"
+#include "vecio.cuh"
+
+namespace dtb {
+namespace fp8 {
+
+// |x| as ordered bits: infinity and NaN compare above every finite magnitude
+__device__ __forceinline__ uint32_t mag(float x) { return __float_as_uint(x) & 0x7fffffffu; }
+
+// biased exponent of the block's scale from the bits of its largest magnitude
+__device__ __forceinline__ uint32_t scale_byte(uint32_t amax) {
+  if (amax >= 0x7f800000u) return 255u;             // NaN
+  amax = max(amax, 27u << 23);                      // 2^-100
+  // amax = f * 2^E, 1 <= f < 2: e = E - 8 where f <= 1.75, E - 7 above
+  return (amax >> 23) - 8u + ((amax & 0x7fffffu) > 0x600000u ? 1u : 0u);
+}
+// 2^-e, the factor that brings the block into range (NaN for a NaN scale)
+__device__ __forceinline__ float inv_scale(uint32_t byte) {
+  return byte == 255u ? __int_as_float(0x7fc00000) : __uint_as_float((254u - byte) << 23);
+}
+
+__device__ __forceinline__ uint32_t cvt4(float a, float b, float c, float d) {
+  const uint32_t lo = __nv_cvt_float2_to_fp8x2(make_float2(a, b), __NV_SATFINITE, __NV_E4M3);
+  const uint32_t hi = __nv_cvt_float2_to_fp8x2(make_float2(c, d), __NV_SATFINITE, __NV_E4M3);
+  return lo | (hi << 16);
+}
+
+struct QuantArgs {
+  const void* x;      // [R, C], row stride ld
+  long ld;
+  int R, C;
+  uint8_t* q;         // [R, q_ld] codes as they lie, or null
+  long q_ld;
+  uint8_t* s;         // 1 x 128: [C / 128][R]; 128 x 128: [R / 128][C / 128]
+  uint8_t* qt;        // [C, qt_ld] transposed codes, or null
+  long qt_ld;
+  uint8_t* st;        // 1 x 128 of the transpose: [R / 128][C]
+};
+
+// One 128 x 128 tile per block of 256 threads: thread (rg, cg) holds rows rg * 8 + i, columns cg * 8 + k.
+template <typename T, bool SQUARE, bool WIDE>
+__global__ void __launch_bounds__(256) quant_tile_kernel(const QuantArgs a) {
+  __shared__ __align__(16) uint8_t sh[128 * 128];
+  __shared__ uint32_t colmax[8][128];
+  const int tid = threadIdx.x, cg = tid & 15, rg = tid >> 4, warp = tid >> 5, lane = tid & 31;
+  const int r0 = blockIdx.y * 128 + rg * 8, c0 = blockIdx.x * 128 + cg * 8;
+  const T* x = reinterpret_cast<const T*>(a.x);
+  Pack<T, 8> v[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const long row = r0 + i;
+    if (WIDE && row < a.R && c0 + 8 <= a.C) {
+      v[i].load(x + row * a.ld + c0);
+    } else {
+#pragma unroll
+      for (int k = 0; k < 8; ++k)
+        v[i].e[k] = (row < a.R && c0 + k < a.C) ? x[row * a.ld + c0 + k] : from_float<T>(0.f);
+    }
+  }
+  uint32_t rmax[8], cmax[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) rmax[i] = cmax[i] = 0;
+#pragma unroll
+  for (int i = 0; i < 8; ++i)
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+      const uint32_t m = mag(v[i].at(k));
+      rmax[i] = max(rmax[i], m);
+      cmax[k] = max(cmax[k], m);
+    }
+  if (SQUARE) {
+    uint32_t m = 0;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) m = max(m, rmax[i]);
+    m = __reduce_max_sync(0xffffffffu, m);
+    if (lane == 0) colmax[0][warp] = m;
+    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < 8; ++w) m = max(m, colmax[0][w]);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) rmax[i] = m;
+    if (tid == 0) a.s[(long)blockIdx.y * gridDim.x + blockIdx.x] = (uint8_t)scale_byte(m);
+  } else if (a.q != nullptr) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+#pragma unroll
+      for (int o = 1; o < 16; o <<= 1) rmax[i] = max(rmax[i], __shfl_xor_sync(0xffffffffu, rmax[i], o));
+      if (cg == i && r0 + i < a.R) a.s[(long)blockIdx.x * a.R + r0 + i] = (uint8_t)scale_byte(rmax[i]);
+    }
+  }
+  if (a.q != nullptr) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const float f = inv_scale(scale_byte(rmax[i]));
+      uint2 o;
+      o.x = cvt4(v[i].at(0) * f, v[i].at(1) * f, v[i].at(2) * f, v[i].at(3) * f);
+      o.y = cvt4(v[i].at(4) * f, v[i].at(5) * f, v[i].at(6) * f, v[i].at(7) * f);
+      // q_ld is a multiple of 16: the padding columns get zeros
+      if (r0 + i < a.R && c0 < a.q_ld) *reinterpret_cast<uint2*>(a.q + (long)(r0 + i) * a.q_ld + c0) = o;
+    }
+  }
+  if (a.qt == nullptr) return;
+  float f[8];
+  if (SQUARE) {
+    const float g = inv_scale(scale_byte(rmax[0]));
+#pragma unroll
+    for (int k = 0; k < 8; ++k) f[k] = g;
+  } else {
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+      cmax[k] = max(cmax[k], __shfl_xor_sync(0xffffffffu, cmax[k], 16));
+      if (lane < 16) colmax[warp][cg * 8 + k] = cmax[k];
+    }
+    __syncthreads();
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+      uint32_t m = 0;
+#pragma unroll
+      for (int w = 0; w < 8; ++w) m = max(m, colmax[w][cg * 8 + k]);
+      const uint32_t b = scale_byte(m);
+      f[k] = inv_scale(b);
+      if (rg == k && c0 + k < a.C) a.st[(long)blockIdx.y * a.C + c0 + k] = (uint8_t)b;
+    }
+  }
+#pragma unroll
+  for (int k = 0; k < 8; ++k) {
+    uint2 o;
+    o.x = cvt4(v[0].at(k) * f[k], v[1].at(k) * f[k], v[2].at(k) * f[k], v[3].at(k) * f[k]);
+    o.y = cvt4(v[4].at(k) * f[k], v[5].at(k) * f[k], v[6].at(k) * f[k], v[7].at(k) * f[k]);
+    *reinterpret_cast<uint2*>(sh + (cg * 8 + k) * 128 + ((rg ^ cg) << 3)) = o;
+  }
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int c = (tid >> 3) + i * 32, j = tid & 7;  // column of x, pair of chunks (16 rows)
+    const int col = blockIdx.x * 128 + c;
+    const long row = (long)blockIdx.y * 128 + j * 16;
+    if (col >= a.C || row >= a.qt_ld) continue;
+    const uint8_t* src = sh + c * 128;
+    const uint2 lo = *reinterpret_cast<const uint2*>(src + (((2 * j) ^ (c >> 3)) << 3));
+    const uint2 hi = *reinterpret_cast<const uint2*>(src + (((2 * j + 1) ^ (c >> 3)) << 3));
+    *reinterpret_cast<uint4*>(a.qt + (long)col * a.qt_ld + row) = make_uint4(lo.x, lo.y, hi.x, hi.y);
+  }
+}
+
+// Rows alone (1 x 128, codes as they lie): 16 lanes per block, for any number of rows.
+template <typename T, bool WIDE>
+__global__ void __launch_bounds__(256) quant_rows_kernel(const QuantArgs a) {
+  const int cb = (a.C + 127) / 128;
+  const long item = (long)blockIdx.x * 16 + (threadIdx.x >> 4);  // (row, block)
+  const int cg = threadIdx.x & 15;
+  const bool live = item < (long)a.R * cb;
+  const long row = live ? item / cb : 0;
+  const int blk = live ? (int)(item % cb) : 0;
+  const int c0 = blk * 128 + cg * 8;
+  const T* x = reinterpret_cast<const T*>(a.x) + row * a.ld;
+  Pack<T, 8> v;
+  if (WIDE && live && c0 + 8 <= a.C) {
+    v.load(x + c0);
+  } else {
+#pragma unroll
+    for (int k = 0; k < 8; ++k) v.e[k] = (live && c0 + k < a.C) ? x[c0 + k] : from_float<T>(0.f);
+  }
+  uint32_t m = 0;
+#pragma unroll
+  for (int k = 0; k < 8; ++k) m = max(m, mag(v.at(k)));
+#pragma unroll
+  for (int o = 1; o < 16; o <<= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, o));
+  if (!live) return;
+  const uint32_t b = scale_byte(m);
+  if (cg == 0) a.s[(long)blk * a.R + row] = (uint8_t)b;
+  const float f = inv_scale(b);
+  uint2 o;
+  o.x = cvt4(v.at(0) * f, v.at(1) * f, v.at(2) * f, v.at(3) * f);
+  o.y = cvt4(v.at(4) * f, v.at(5) * f, v.at(6) * f, v.at(7) * f);
+  if (c0 < a.q_ld) *reinterpret_cast<uint2*>(a.q + row * a.q_ld + c0) = o;
+}
+
+}  // namespace fp8
+}  // namespace dtb
+
+using namespace dtb;
+
+// x [R, C] -> {codes [R, C], scales, transposed codes [C, R], their scales}.  square: 128 x 128 blocks, scales
+// [R/128, C/128] and their transpose; else 1 x 128 along the last axis of each output, scales [R, C/128] and
+// [C, R/128] (block-major in memory).  Codes lie in rows padded to 16 bytes.  `plain` / `transposed` select
+// which of the two are made (undefined tensors stand for the other).
+std::vector<torch::Tensor> fp8_quantize(torch::Tensor x, bool square, bool plain, bool transposed) {
+  DTB_CHECK(x.is_cuda() && x.dim() == 2 && is_float_type(x.scalar_type()) && (x.numel() == 0 || x.size(1) == 1 || x.stride(1) == 1), "fp8_quantize: x must be a 2-D CUDA tensor of fp32, bf16 or fp16 with contiguous columns");
+  DTB_CHECK(plain || transposed, "fp8_quantize: nothing asked for");
+  DTB_CHECK(x.size(0) < (1L << 31) - 256 && x.size(1) < (1L << 31) - 256, "fp8_quantize: too large");
+  const c10::cuda::CUDAGuard guard(x.device());
+  const long R = x.size(0), C = x.size(1), RB = (R + 127) / 128, CB = (C + 127) / 128;
+  auto codes = [&](long rows, long cols) {
+    const long pitch = (cols + 15) / 16 * 16;
+    return torch::empty({rows, pitch}, x.options().dtype(at::kFloat8_e4m3fn)).narrow(1, 0, cols);
+  };
+  auto opts = x.options().dtype(at::kFloat8_e8m0fnu);
+  torch::Tensor q, s, qt, st;
+  if (plain) q = codes(R, C);
+  if (transposed) qt = codes(C, R);
+  if (square) {
+    s = torch::empty({RB, CB}, opts);
+    st = s.t();
+  } else {
+    if (plain) s = torch::empty({CB, R}, opts).t();
+    if (transposed) st = torch::empty({RB, C}, opts).t();
+  }
+  if (R == 0 || C == 0) return {q, s, qt, st};
+  fp8::QuantArgs a{};
+  a.x = x.data_ptr();
+  a.ld = x.stride(0);
+  a.R = (int)R;
+  a.C = (int)C;
+  if (plain) {
+    a.q = reinterpret_cast<uint8_t*>(q.data_ptr());
+    a.q_ld = (C + 15) / 16 * 16;
+  }
+  if (square || plain) a.s = reinterpret_cast<uint8_t*>(s.data_ptr());
+  if (transposed) {
+    a.qt = reinterpret_cast<uint8_t*>(qt.data_ptr());
+    a.qt_ld = (R + 15) / 16 * 16;
+    if (!square) a.st = reinterpret_cast<uint8_t*>(st.data_ptr());
+  }
+  const bool wide = (reinterpret_cast<uintptr_t>(a.x) & 15) == 0 && (a.ld * (long)x.element_size()) % 16 == 0;
+  auto stream = at::cuda::getCurrentCUDAStream();
+  const bool tile = square || transposed;
+  DTB_CHECK(!tile || RB <= 65535, "fp8_quantize: more than 8388480 rows");
+  const dim3 grid((unsigned)CB, (unsigned)RB);
+  const long items = (R * CB + 15) / 16;
+  DTB_CHECK(tile || items < (1L << 31), "fp8_quantize: too large");
+  DTB_FLOAT_TYPES(x.scalar_type(), {
+    if (tile && square) {
+      if (wide) fp8::quant_tile_kernel<T, true, true><<<grid, 256, 0, stream>>>(a);
+      else fp8::quant_tile_kernel<T, true, false><<<grid, 256, 0, stream>>>(a);
+    } else if (tile) {
+      if (wide) fp8::quant_tile_kernel<T, false, true><<<grid, 256, 0, stream>>>(a);
+      else fp8::quant_tile_kernel<T, false, false><<<grid, 256, 0, stream>>>(a);
+    } else {
+      if (wide) fp8::quant_rows_kernel<T, true><<<(unsigned)items, 256, 0, stream>>>(a);
+      else fp8::quant_rows_kernel<T, false><<<(unsigned)items, 256, 0, stream>>>(a);
+    }
+  });
+  DTB_LAUNCH_CHECK();
+  return {q, s, qt, st};
+}

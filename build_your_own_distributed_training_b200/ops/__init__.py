@@ -17,3 +17,4 @@ from .embedding import embedding  # noqa: F401
 from .qk_norm import qk_norm_rope  # noqa: F401
 from .dropout import dropout_add  # noqa: F401
 from .logprobs import TokenLogProbs, lm_head_token_log_probs, token_log_probs  # noqa: F401
+from .fp8 import Fp8Blocks, fp8_matmul, linear_fp8, quantize_fp8  # noqa: F401

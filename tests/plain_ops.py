@@ -83,3 +83,19 @@ def top_order(row, k: int) -> list[int]:
 def slope(f, x: torch.Tensor, v: torch.Tensor, h: float) -> float:
     """Central difference of the scalar ``f`` at ``x`` along ``v``."""
     return float((f(x + h * v) - f(x - h * v)) / (2 * h))
+
+
+def fp8_round(x: torch.Tensor, rows: int) -> tuple[torch.Tensor, torch.Tensor]:
+    """(the 64-bit values that the 8-bit codes of ``x`` stand for, scales as floats) in rows x 128
+    blocks, one block at a time."""
+    x = x.double().cpu()
+    out, scales = torch.empty_like(x), torch.empty(-(-x.shape[0] // rows), -(-x.shape[1] // 128), dtype=torch.float64)
+    for i in range(scales.shape[0]):
+        for j in range(scales.shape[1]):
+            b = x[i * rows:(i + 1) * rows, j * 128:(j + 1) * 128]
+            s = 2.0 ** math.ceil(math.log2(max(float(b.abs().max()), 2.0 ** -100) / 448))
+            v = (b / s).numpy()
+            step = np.exp2(np.maximum(np.frexp(v)[1] - 1, -6) - 3.0)  # 4 significant bits, 2^-9 below 2^-6
+            out[i * rows:(i + 1) * rows, j * 128:(j + 1) * 128] = torch.from_numpy(np.rint(v / step) * step) * s
+            scales[i, j] = s
+    return out, scales
