@@ -34,6 +34,12 @@ class ModelConfig:
     ``n_kv_heads`` defaults to ``n_heads`` (plain multi-head attention) and
     ``ffn_hidden_size`` defaults to ``8/3 * d_model`` rounded up to a multiple
     of 256, the LLaMA SwiGLU sizing.
+
+    Without reference counterpart: ``qk_norm`` normalises every query and key
+    head (RMSNorm, one weight for the queries and one for the keys of a block)
+    before the rotation; ``resid_dropout`` drops elements of each sub-layer's
+    output before the residual add (``dropout`` is the attention
+    probabilities', as in the reference).
     """
 
     vocab_size: int = 32000
@@ -49,6 +55,8 @@ class ModelConfig:
     dropout: float = 0.0
     attention_bias: bool = False
     mlp_bias: bool = False
+    qk_norm: bool = False
+    resid_dropout: float = 0.0
 
     def __post_init__(self) -> None:
         if self.n_kv_heads is None:
@@ -165,10 +173,14 @@ class KernelConfig:
     ``fused_comm``: TP/DP collectives run as this package's peer-memory kernels
     (``False`` routes them through ``torch.distributed``/NCCL, the baseline).
     ``deterministic``: fixed-order reductions everywhere (bit-exact reruns).
+    ``fp8_linear``: the blocks' projections in 8 bits with a power-of-two scale
+    for each block of 128 (forward and both gradients; embedding, head and
+    attention stay in ``param_dtype``).
     """
 
     fused_comm: bool = True
     deterministic: bool = True
+    fp8_linear: bool = False
 
 
 @dataclass
@@ -237,6 +249,12 @@ class TrainingConfig:
                 raise ValueError(f"{name}={value} is not divisible by tp_size={tp}.")
         if m.n_heads % m.n_kv_heads:
             raise ValueError(f"n_heads={m.n_heads} is not a multiple of n_kv_heads={m.n_kv_heads}.")
+        if not 0.0 <= m.resid_dropout < 1.0:
+            raise ValueError(f"resid_dropout={m.resid_dropout} is outside [0, 1).")
+        if m.qk_norm and (m.head_dim % 2 or m.head_dim > 512):
+            raise ValueError(f"qk_norm needs an even head size up to 512, got {m.head_dim}.")
+        if self.kernels.fp8_linear and (m.attention_bias or m.mlp_bias):
+            raise ValueError("fp8_linear projections have no bias: set attention_bias and mlp_bias to false.")
         if self.parallel.loss_parallel and m.vocab_size % tp:
             raise ValueError(f"loss_parallel needs vocab_size={m.vocab_size} divisible by tp={tp}.")
         if self.parallel.sequence_parallel and tp > 1:

@@ -76,6 +76,7 @@ std::vector<torch::Tensor> token_logprobs_fwd(torch::Tensor x, torch::Tensor tok
                                               int64_t ignore);
 void token_logprobs_bwd(torch::Tensor x, torch::Tensor tokens, torch::Tensor state, c10::optional<torch::Tensor> g_lp,
                         c10::optional<torch::Tensor> g_ent, double temperature, torch::Tensor dx);
+void swiglu_fwd(torch::Tensor gu, torch::Tensor act);
 std::vector<torch::Tensor> fp8_quantize(torch::Tensor x, bool square, bool plain, bool transposed);
 void fp8_gemm(torch::Tensor A, torch::Tensor sA, int64_t granA, torch::Tensor B, torch::Tensor sB, int64_t granB,
               torch::Tensor D, c10::optional<torch::Tensor> R, bool accumulate);
@@ -136,4 +137,5 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("token_logprobs_bwd", &token_logprobs_bwd);
   m.def("fp8_quantize", &fp8_quantize, "e4m3 codes with a power-of-two scale per block of 128, as they lie and / or transposed");
   m.def("fp8_gemm", &fp8_gemm, "tcgen05 block-scaled product of e4m3 operands");
+  m.def("swiglu_fwd", &swiglu_fwd, "silu(g) * u of packed [g | u]");
 }

@@ -21,6 +21,7 @@ import torch
 import torch.nn as nn
 
 from ..config import ModelConfig
+from ..ops.logprobs import TokenLogProbs, lm_head_token_log_probs
 from ..ops.loss import lm_head_cross_entropy
 from ..ops.norm import rms_norm
 from ..ops.rope import precompute_rope_cache
@@ -110,22 +111,51 @@ class Transformer(nn.Module):
                                              or labels is None)
         return logits, loss
 
-    def forward(self, tokens: torch.Tensor, labels: torch.Tensor | None = None
-                ) -> tuple[torch.Tensor | None, torch.Tensor | None]:
+    def score(self, h: torch.Tensor, targets: torch.Tensor, temperature: float, top_k: int) -> TokenLogProbs:
+        """Log probabilities of ``targets`` from the last block's output (see :meth:`forward`)."""
+        if isinstance(self.tok_embeddings, VocabParallelEmbedding) or tpar.sp_on(self.tp):
+            raise NotImplementedError("token log probabilities need the whole vocabulary and every token on each "
+                                      "rank: turn loss_parallel and sequence_parallel off")
+        h2 = self.norm(h).reshape(-1, h.shape[-1])
+        r = lm_head_token_log_probs(h2, self.lm_head.weight, targets.reshape(-1), temperature=temperature, top_k=top_k,
+                                    main_grad=main_grad_of(self.lm_head.weight))
+        return TokenLogProbs(*(None if t is None else t.view(*targets.shape, *t.shape[1:]) for t in r))
+
+    def forward(self, tokens: torch.Tensor, labels: torch.Tensor | None = None, *,
+                targets: torch.Tensor | None = None, temperature: float = 1.0, top_k: int = 0
+                ) -> tuple[torch.Tensor | None, torch.Tensor | None] | TokenLogProbs:
         """``tokens``/``labels``: ``[batch, seq]``; returns ``(logits, loss)``.
 
         ``logits`` is ``[batch, seq, vocab]`` (``None`` when ``return_logits``
         is off, or under sequence/loss parallelism).
+
+        With ``targets`` ``[batch, seq]`` (the token each position is to be
+        scored on, -100 for none) it returns a :class:`TokenLogProbs` instead,
+        differentiable in its ``logprob`` and ``entropy``: the term of a policy
+        or preference loss.
         """
+        if targets is not None and labels is not None:
+            raise ValueError("give labels (mean cross-entropy) or targets (log probabilities), not both")
         bsz, seqlen = tokens.shape
         cos, sin = self.rope_cos[:seqlen], self.rope_sin[:seqlen]
         h = self.embed(tokens)
         for layer in self.layers:
             h = layer(h, cos, sin)
+        if targets is not None:
+            return self.score(h, targets, temperature, top_k)
         logits, loss = self.head(h, labels)
         if logits is not None and logits.dim() == 2 and logits.shape[0] == bsz * seqlen:
             logits = logits.view(bsz, seqlen, -1)
         return logits, loss
+
+
+def set_fp8_linear(model: Transformer, on: bool = True) -> Transformer:
+    """Run the blocks' projections in 8 bits (``kernels.fp8_linear``)."""
+    if on and (model.config.attention_bias or model.config.mlp_bias):
+        raise ValueError("8-bit projections have no bias")
+    for blk in model.layers:
+        blk.attention.fp8 = blk.mlp.fp8 = on
+    return model
 
 
 def build_model(config: ModelConfig) -> Transformer:

@@ -206,3 +206,26 @@ def linear_swiglu(x: torch.Tensor, weight: torch.Tensor, ffn: int, *,
     input gradient and its TP all-reduce in one kernel (column-parallel use).
     """
     return _SwiGLUFn.apply(x.contiguous(), weight, ffn, main_grad, grad_comm)
+
+
+class _SwiGLUPackedFn(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, gu, ffn):  # type: ignore[override]
+        ctx.save_for_backward(gu)
+        ctx.ffn = ffn
+        if gu.is_cuda:
+            from ._ext import native
+            act = torch.empty(gu.shape[0], ffn, device=gu.device, dtype=gu.dtype)
+            native().swiglu_fwd(gu, act)
+            return act
+        return swiglu_reference(gu.float(), ffn).to(gu.dtype)
+
+    @staticmethod
+    def backward(ctx, dact):  # type: ignore[override]
+        (gu,) = ctx.saved_tensors
+        return swiglu_backward(dact, gu, ctx.ffn), None
+
+
+def swiglu_packed(gu: torch.Tensor, ffn: int) -> torch.Tensor:
+    """``silu(g) * u`` of a packed ``[tokens, g | u]``, for projections without the SwiGLU epilogue."""
+    return _SwiGLUPackedFn.apply(gu.contiguous(), ffn)

@@ -14,6 +14,8 @@ nothing saved but the input.  No reference counterpart: the reference's attentio
 
 from __future__ import annotations
 
+from collections.abc import Callable
+
 import torch
 
 from . import grad_state
@@ -62,14 +64,14 @@ def _backward_cpu(g, x, wq, wk, cos, sin, pos, nq, nkv, hd, seqlen, eps):
 
 class _QKNormRopeFn(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, qkv, wq, wk, cos, sin, positions, nq, nkv, hd, seqlen, eps, main_grads):  # type: ignore[override]
+    def forward(ctx, qkv, wq, wk, cos, sin, positions, nq, nkv, hd, seqlen, eps, main_grads, reduce):  # type: ignore[override]
         if qkv.is_cuda:
             y = native().qk_norm_rope_fwd(qkv, wq, wk, cos, sin, positions, nq, nkv, hd, seqlen, eps)
         else:
             y = qk_norm_rope_reference(qkv, wq, wk, cos, sin, nq, nkv, hd, seqlen, eps, positions)
         ctx.save_for_backward(qkv, wq, wk, cos, sin, positions)
         ctx.cfg = (nq, nkv, hd, seqlen, eps)
-        ctx.main_grads = main_grads
+        ctx.main_grads, ctx.reduce = main_grads, reduce
         return y
 
     @staticmethod
@@ -80,27 +82,39 @@ class _QKNormRopeFn(torch.autograd.Function):
         if mgs is not None:
             for mg in mgs:
                 grad_state.zero_if_fresh(mg)  # the weight gradients accumulate
+        # straight into the weights' own gradients, unless other ranks' parts have to be added first
+        direct = mgs is not None and ctx.reduce is None
         if qkv.is_cuda:
             if g.stride(-1) != 1:
                 g = g.contiguous()
-            dwq, dwk = mgs if mgs is not None else (torch.empty_like(wq), torch.empty_like(wk))
+            if ctx.reduce is not None:
+                dw = torch.empty(2, hd, device=wq.device, dtype=torch.float32)
+                dwq, dwk = dw[0], dw[1]
+            else:
+                dwq, dwk = mgs if direct else (torch.empty_like(wq), torch.empty_like(wk))
             dx = native().qk_norm_rope_bwd(g, qkv, wq, wk, cos, sin, positions, nq, nkv, hd, seqlen, eps,
-                                           dwq, dwk, mgs is not None)
+                                           dwq, dwk, direct)
         else:
-            dx, fq, fk = _backward_cpu(g, qkv, wq, wk, cos, sin, positions, nq, nkv, hd, seqlen, eps)
-            dwq, dwk = fq.to(wq.dtype), fk.to(wk.dtype)
-            if mgs is not None:
-                mgs[0].add_(fq)
-                mgs[1].add_(fk)
+            dx, dwq, dwk = _backward_cpu(g, qkv, wq, wk, cos, sin, positions, nq, nkv, hd, seqlen, eps)
+            dw = torch.stack((dwq, dwk))
+        if ctx.reduce is not None:
+            ctx.reduce(dw)
+            dwq, dwk = dw[0], dw[1]
         if mgs is not None:
+            if not (direct and qkv.is_cuda):
+                mgs[0].add_(dwq)
+                mgs[1].add_(dwk)
             dwq = dwk = None
-        return (dx, dwq, dwk) + (None,) * 9
+        else:
+            dwq, dwk = dwq.to(wq.dtype), dwk.to(wk.dtype)
+        return (dx, dwq, dwk) + (None,) * 10
 
 
 def qk_norm_rope(qkv: torch.Tensor, q_weight: torch.Tensor, k_weight: torch.Tensor, cos: torch.Tensor,
                  sin: torch.Tensor, n_q_heads: int, n_kv_heads: int, head_dim: int, seqlen: int,
                  eps: float = 1e-5, *, positions: torch.Tensor | None = None,
-                 main_grads: tuple[torch.Tensor, torch.Tensor] | None = None) -> torch.Tensor:
+                 main_grads: tuple[torch.Tensor, torch.Tensor] | None = None,
+                 grad_reduce: Callable[[torch.Tensor], None] | None = None) -> torch.Tensor:
     """``qkv: [tokens, (nq + 2 nkv) * hd]`` -> the same shape, q and k normalised and rotated.
 
     Token ``m`` is at position ``m % seqlen``, or at ``positions[m]`` (int64 or int32: packed
@@ -120,4 +134,4 @@ def qk_norm_rope(qkv: torch.Tensor, q_weight: torch.Tensor, k_weight: torch.Tens
     if qkv.stride(1) != 1:
         qkv = qkv.contiguous()
     return _QKNormRopeFn.apply(qkv, q_weight, k_weight, cos, sin, positions, n_q_heads, n_kv_heads, head_dim,
-                               seqlen, eps, main_grads)
+                               seqlen, eps, main_grads, grad_reduce)

@@ -67,3 +67,27 @@ def rope_backward_(d: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor, rope_c
     vs = v * s
     back = v * c + torch.cat((vs[..., h:], -vs[..., :h]), dim=-1)
     d[:, :rope_cols] = back.to(d.dtype).reshape(d.shape[0], rope_cols)
+
+
+class _RopePackedFn(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, y, cos, sin, rope_cols, head_dim, seqlen):  # type: ignore[override]
+        ctx.save_for_backward(cos, sin)
+        ctx.cfg = (rope_cols, head_dim, seqlen)
+        out = y.contiguous().clone()
+        rope_forward(out, cos, sin, rope_cols, head_dim, seqlen)
+        return out
+
+    @staticmethod
+    def backward(ctx, d):  # type: ignore[override]
+        cos, sin = ctx.saved_tensors
+        back = d.contiguous().clone()
+        rope_backward_(back, cos, sin, *ctx.cfg)
+        return back, None, None, None, None, None
+
+
+def rope_packed(y: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor, rope_cols: int, head_dim: int,
+                seqlen: int) -> torch.Tensor:
+    """Differentiable :func:`rope_forward` into a new tensor, for projections without the rotation in
+    their epilogue."""
+    return _RopePackedFn.apply(y, cos, sin, rope_cols, head_dim, seqlen)

@@ -43,6 +43,8 @@ import torch.distributed as dist
 import torch.nn as nn
 import torch.nn.functional as F
 
+from ..ops.dropout import dropout_add
+from ..ops.fp8 import linear_fp8
 from ..ops.linear import linear
 
 
@@ -308,17 +310,34 @@ def column_input(x2: torch.Tensor, tp: TPInfo | None) -> torch.Tensor:
 
 def row_output_linear(x2: torch.Tensor, weight: torch.Tensor, residual: torch.Tensor | None,
                       tp: TPInfo | None, *, main_grad: torch.Tensor | None = None,
-                      bias: torch.Tensor | None = None) -> torch.Tensor:
-    """``reduce(x2 @ W^T) (+ bias) (+ residual)`` for a row-parallel weight."""
+                      bias: torch.Tensor | None = None, fp8: bool = False) -> torch.Tensor:
+    """``reduce(x2 @ W^T) (+ bias) (+ residual)`` for a row-parallel weight; ``fp8``: the product in 8 bits."""
     if tp is None or tp.size == 1:
+        if fp8:
+            return linear_fp8(x2, weight, residual=residual, main_grad=main_grad)
         return linear(x2, weight, bias=bias, residual=residual, main_grad=main_grad)
-    if tp.fused and x2.is_cuda and tp.comm is not None and bias is None and (tp.sequence_parallel or _fused_ar(tp)):
+    if not fp8 and tp.fused and x2.is_cuda and tp.comm is not None and bias is None and (tp.sequence_parallel or _fused_ar(tp)):
         return tp.comm.row_parallel_linear(x2, weight, residual, main_grad)
-    y = linear(x2, weight, main_grad=main_grad)
+    y = (linear_fp8 if fp8 else linear)(x2, weight, main_grad=main_grad)
     y = _SeqReduceScatter.apply(y, tp) if tp.sequence_parallel else _AllReduceFwd.apply(y, tp)
     if bias is not None:
         y = y + bias.to(y.dtype)
     return y + residual if residual is not None else y
+
+
+def row_output_dropout(x2: torch.Tensor, weight: torch.Tensor, residual: torch.Tensor, tp: TPInfo | None, p: float, *,
+                       main_grad: torch.Tensor | None = None, bias: torch.Tensor | None = None,
+                       fp8: bool = False) -> torch.Tensor:
+    """``residual + dropout(reduce(x2 @ W^T) (+ bias))``.
+
+    The mask is a function of a seed and the element's number in the whole activation.  The seed comes
+    from torch's CPU generator, which TP peers share and activation checkpointing restores for its
+    recompute; under sequence parallelism each rank numbers its rows from where they stand, so every
+    layout of the same activation drops the same elements.
+    """
+    y = row_output_linear(x2, weight, None, tp, main_grad=main_grad, bias=bias, fp8=fp8)
+    seed = int(torch.randint(0, 1 << 62, ()))
+    return dropout_add(y, residual.to(y.dtype), p, seed, start=tp.rank * y.numel() if sp_on(tp) else 0)
 
 
 # ----------------------------------------------------------------------------

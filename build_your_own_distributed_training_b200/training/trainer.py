@@ -30,7 +30,7 @@ from ..checkpointing.recovery import find_latest_valid_checkpoint, require_valid
 from ..config import TrainingConfig
 from ..data.dataloader import build_dataloader
 from ..data.dataset import PackedTokenDataset, SyntheticTokenDataset, UniformTokenDataset
-from ..models.transformer import TransformerBlock, build_model
+from ..models.transformer import TransformerBlock, build_model, set_fp8_linear
 from ..observability.logging import build_logger
 from ..observability.metrics import reset_peak_memory
 from ..observability.profiler import build_profiler
@@ -48,6 +48,8 @@ def build_engine(config: TrainingConfig, ctx: ProcessContext) -> torch.nn.Module
     # TP ranks must start from identical full weights: seed by the base seed here
     torch.manual_seed(config.seed)
     model = build_model(config.model)
+    if config.kernels.fp8_linear:
+        set_fp8_linear(model)
     use_peer = (ctx.device.type == "cuda" and config.kernels.fused_comm and ctx.world_size > 1)
     tp_comm = dp_comm = None
     if use_peer:
