@@ -70,8 +70,6 @@ torch::Tensor qk_norm_rope_bwd(torch::Tensor g, torch::Tensor x, torch::Tensor w
                                torch::Tensor cos_t, torch::Tensor sin_t, c10::optional<torch::Tensor> pos, int64_t nq,
                                int64_t nkv, int64_t hd, int64_t seqlen, double eps, torch::Tensor dwq,
                                torch::Tensor dwk, bool accumulate);
-torch::Tensor dropout_add(torch::Tensor x, c10::optional<torch::Tensor> residual, int64_t cut, int64_t seed,
-                          int64_t start);
 std::vector<torch::Tensor> token_logprobs_fwd(torch::Tensor x, torch::Tensor tokens, double temperature, int64_t top_k,
                                               int64_t ignore);
 void token_logprobs_bwd(torch::Tensor x, torch::Tensor tokens, torch::Tensor state, c10::optional<torch::Tensor> g_lp,
@@ -80,6 +78,14 @@ void swiglu_fwd(torch::Tensor gu, torch::Tensor act);
 std::vector<torch::Tensor> fp8_quantize(torch::Tensor x, bool square, bool plain, bool transposed);
 void fp8_gemm(torch::Tensor A, torch::Tensor sA, int64_t granA, torch::Tensor B, torch::Tensor sB, int64_t granB,
               torch::Tensor D, c10::optional<torch::Tensor> R, bool accumulate);
+torch::Tensor qk_norm_rope_autograd(torch::Tensor x, torch::Tensor wq, torch::Tensor wk, torch::Tensor cos_t,
+                                    torch::Tensor sin_t, c10::optional<torch::Tensor> pos, int64_t nq, int64_t nkv,
+                                    int64_t hd, int64_t seqlen, double eps);
+torch::Tensor dropout_add_autograd(torch::Tensor x, c10::optional<torch::Tensor> residual, int64_t cut, int64_t seed,
+                                   int64_t start);
+std::vector<torch::Tensor> token_logprobs_autograd(torch::Tensor x, torch::Tensor tokens, double temperature,
+                                                   int64_t top_k, int64_t ignore);
+torch::Tensor linear_fp8_autograd(torch::Tensor x, torch::Tensor w, c10::optional<torch::Tensor> residual);
 
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.doc() = "sm_100a kernels for B200-native 2-D parallel LLaMA training";
@@ -132,10 +138,13 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("ce_loss_finish", &ce_loss_finish);
   m.def("qk_norm_rope_fwd", &qk_norm_rope_fwd, "per-head RMSNorm of q and k with the rotary rotation, packed qkv");
   m.def("qk_norm_rope_bwd", &qk_norm_rope_bwd);
-  m.def("dropout_add", &dropout_add, "residual + dropout(x), mask from Philox4x32-10 by element number");
   m.def("token_logprobs_fwd", &token_logprobs_fwd, "log probabilities of given tokens, entropy, top alternatives");
   m.def("token_logprobs_bwd", &token_logprobs_bwd);
   m.def("fp8_quantize", &fp8_quantize, "e4m3 codes with a power-of-two scale per block of 128, as they lie and / or transposed");
   m.def("fp8_gemm", &fp8_gemm, "tcgen05 block-scaled product of e4m3 operands");
   m.def("swiglu_fwd", &swiglu_fwd, "silu(g) * u of packed [g | u]");
+  m.def("qk_norm_rope", &qk_norm_rope_autograd, "qk_norm_rope_fwd as an autograd node");
+  m.def("dropout_add", &dropout_add_autograd, "residual + dropout(x), mask from Philox4x32-10 by element number; an autograd node");
+  m.def("token_logprobs", &token_logprobs_autograd, "token_logprobs_fwd as an autograd node");
+  m.def("linear_fp8", &linear_fp8_autograd, "8-bit linear layer with its backward as an autograd node");
 }

@@ -1,0 +1,141 @@
+// Autograd nodes of the block operators, so that a call and its backward stay out of the interpreter:
+// at a few thousand elements an operator costs what its launch costs, and a Python node adds some 30 us
+// to a forward and backward.  The Python layer keeps its own nodes for what belongs to the sharding engine
+// (gradients that go into its fp32 buffers) and for the CPU path; both call the same kernels.
+#include <torch/extension.h>
+
+using torch::Tensor;
+using torch::autograd::AutogradContext;
+using torch::autograd::Function;
+using torch::autograd::variable_list;
+
+Tensor qk_norm_rope_fwd(Tensor x, Tensor wq, Tensor wk, Tensor cos_t, Tensor sin_t, c10::optional<Tensor> pos,
+                        int64_t nq, int64_t nkv, int64_t hd, int64_t seqlen, double eps);
+Tensor qk_norm_rope_bwd(Tensor g, Tensor x, Tensor wq, Tensor wk, Tensor cos_t, Tensor sin_t,
+                        c10::optional<Tensor> pos, int64_t nq, int64_t nkv, int64_t hd, int64_t seqlen, double eps,
+                        Tensor dwq, Tensor dwk, bool accumulate);
+Tensor dropout_add(Tensor x, c10::optional<Tensor> residual, int64_t cut, int64_t seed, int64_t start);
+std::vector<Tensor> token_logprobs_fwd(Tensor x, Tensor tokens, double temperature, int64_t top_k, int64_t ignore);
+void token_logprobs_bwd(Tensor x, Tensor tokens, Tensor state, c10::optional<Tensor> g_lp, c10::optional<Tensor> g_ent,
+                        double temperature, Tensor dx);
+std::vector<Tensor> fp8_quantize(Tensor x, bool square, bool plain, bool transposed);
+void fp8_gemm(Tensor A, Tensor sA, int64_t granA, Tensor B, Tensor sB, int64_t granB, Tensor D,
+              c10::optional<Tensor> R, bool accumulate);
+
+namespace {
+
+struct QkNormRope : public Function<QkNormRope> {
+  static Tensor forward(AutogradContext* ctx, const Tensor& x, const Tensor& wq, const Tensor& wk, const Tensor& cos_t,
+                        const Tensor& sin_t, const c10::optional<Tensor>& pos, int64_t nq, int64_t nkv, int64_t hd,
+                        int64_t seqlen, double eps) {
+    ctx->save_for_backward({x, wq, wk, cos_t, sin_t, pos.value_or(Tensor())});
+    ctx->saved_data["c"] = std::vector<int64_t>{nq, nkv, hd, seqlen};
+    ctx->saved_data["eps"] = eps;
+    return qk_norm_rope_fwd(x, wq, wk, cos_t, sin_t, pos, nq, nkv, hd, seqlen, eps);
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    const auto s = ctx->get_saved_variables();
+    const auto c = ctx->saved_data["c"].toIntVector();
+    Tensor g = grads[0];
+    if (g.stride(1) != 1) g = g.contiguous();
+    Tensor dwq = torch::empty_like(s[1]), dwk = torch::empty_like(s[2]);
+    Tensor dx = qk_norm_rope_bwd(g, s[0], s[1], s[2], s[3], s[4],
+                                 s[5].defined() ? c10::optional<Tensor>(s[5]) : c10::nullopt, c[0], c[1], c[2], c[3],
+                                 ctx->saved_data["eps"].toDouble(), dwq, dwk, false);
+    return {dx, dwq, dwk, {}, {}, {}, {}, {}, {}, {}, {}};
+  }
+};
+
+struct DropoutAdd : public Function<DropoutAdd> {
+  static Tensor forward(AutogradContext* ctx, const Tensor& x, const c10::optional<Tensor>& residual, int64_t cut,
+                        int64_t seed, int64_t start) {
+    ctx->saved_data["c"] = std::vector<int64_t>{cut, seed, start, residual.has_value()};
+    return dropout_add(x, residual, cut, seed, start);
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    const auto c = ctx->saved_data["c"].toIntVector();
+    Tensor dx;
+    if (ctx->needs_input_grad(0)) dx = dropout_add(grads[0].contiguous(), c10::nullopt, c[0], c[1], c[2]);
+    // an input that was not given takes no gradient
+    return {dx, c[3] ? grads[0] : Tensor(), {}, {}, {}};
+  }
+};
+
+Tensor row_grad(const Tensor& g) { return g.defined() ? g.to(at::kFloat).contiguous() : g; }
+
+struct TokenLogProbs : public Function<TokenLogProbs> {
+  static variable_list forward(AutogradContext* ctx, const Tensor& x, const Tensor& tokens, double temperature,
+                               int64_t top_k, int64_t ignore) {
+    auto r = token_logprobs_fwd(x, tokens, temperature, top_k, ignore);  // logprob, entropy, state, top
+    ctx->save_for_backward({x, tokens, r[2]});
+    ctx->saved_data["t"] = temperature;
+    ctx->mark_non_differentiable({r[3], r[4]});
+    ctx->set_materialize_grads(false);
+    return {r[0], r[1], r[3], r[4]};
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    const auto s = ctx->get_saved_variables();
+    const Tensor& x = s[0];
+    // the gradient's rows lie as the logits' rows do (padded vocabulary buffers included)
+    const int64_t M = x.size(0), V = x.size(1);
+    int64_t pitch = M > 1 ? std::max(x.stride(0), V) : V;
+    if (pitch > 2 * V + 1024) pitch = V;
+    Tensor dx = torch::empty({M, pitch}, x.options());
+    if (pitch != V) dx = dx.narrow(1, 0, V);
+    const Tensor gl = row_grad(grads[0]), ge = row_grad(grads[1]);
+    token_logprobs_bwd(x, s[1], s[2], gl.defined() ? c10::optional<Tensor>(gl) : c10::nullopt,
+                       ge.defined() ? c10::optional<Tensor>(ge) : c10::nullopt, ctx->saved_data["t"].toDouble(), dx);
+    return {dx, {}, {}, {}, {}};
+  }
+};
+
+struct LinearFp8 : public Function<LinearFp8> {
+  static Tensor forward(AutogradContext* ctx, const Tensor& x, const Tensor& w, const c10::optional<Tensor>& residual) {
+    const bool need_x = x.requires_grad(), need_w = w.requires_grad();
+    auto xq = fp8_quantize(x, false, true, need_w);  // codes, scales, transposed codes, their scales
+    auto wq = fp8_quantize(w, true, true, need_x);
+    Tensor y = torch::empty({x.size(0), w.size(0)}, x.options());
+    fp8_gemm(xq[0], xq[1], 1, wq[0], wq[1], 128, y, residual, false);
+    ctx->save_for_backward({xq[2], xq[3], wq[2], wq[3]});
+    ctx->saved_data["t"] = w.scalar_type();
+    ctx->saved_data["r"] = residual.has_value();
+    return y;
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    const auto s = ctx->get_saved_variables();
+    const bool need_x = ctx->needs_input_grad(0), need_w = ctx->needs_input_grad(1);
+    Tensor dx, dw;
+    if (need_x || need_w) {
+      Tensor g = grads[0].contiguous();
+      auto gq = fp8_quantize(g, false, need_x, need_w);
+      if (need_x) {
+        dx = torch::empty({g.size(0), s[2].size(0)}, g.options());
+        fp8_gemm(gq[0], gq[1], 1, s[2], s[3], 128, dx, c10::nullopt, false);
+      }
+      if (need_w) {
+        const auto t = ctx->saved_data["t"].toScalarType();
+        dw = torch::empty({g.size(1), s[0].size(0)}, g.options().dtype(t == at::kHalf ? at::kFloat : t));
+        fp8_gemm(gq[2], gq[3], 1, s[0], s[1], 1, dw, c10::nullopt, false);
+        dw = dw.to(t);
+      }
+    }
+    return {dx, dw, ctx->saved_data["r"].toBool() ? grads[0] : Tensor()};
+  }
+};
+
+}  // namespace
+
+Tensor qk_norm_rope_autograd(Tensor x, Tensor wq, Tensor wk, Tensor cos_t, Tensor sin_t, c10::optional<Tensor> pos,
+                             int64_t nq, int64_t nkv, int64_t hd, int64_t seqlen, double eps) {
+  return QkNormRope::apply(x, wq, wk, cos_t, sin_t, pos, nq, nkv, hd, seqlen, eps);
+}
+Tensor dropout_add_autograd(Tensor x, c10::optional<Tensor> residual, int64_t cut, int64_t seed, int64_t start) {
+  return DropoutAdd::apply(x, residual, cut, seed, start);
+}
+std::vector<Tensor> token_logprobs_autograd(Tensor x, Tensor tokens, double temperature, int64_t top_k, int64_t ignore) {
+  return TokenLogProbs::apply(x, tokens, temperature, top_k, ignore);
+}
+// x [T, K] bf16, w [N, K], residual [T, N] bf16 or none
+Tensor linear_fp8_autograd(Tensor x, Tensor w, c10::optional<Tensor> residual) {
+  return LinearFp8::apply(x, w, residual);
+}

@@ -38,10 +38,7 @@ def keep_mask(n: int, p: float, seed: int, start: int = 0) -> torch.Tensor:
     return bits[start - first * 8:start - first * 8 + n] >= _cut(p)
 
 
-def _apply(x: torch.Tensor, residual: torch.Tensor | None, p: float, seed: int, start: int) -> torch.Tensor:
-    if x.is_cuda:
-        key = seed - (1 << 64) if seed >= 1 << 63 else seed  # the same 64 bits, signed
-        return native().dropout_add(x, residual, _cut(p), key, start)
+def _apply_cpu(x: torch.Tensor, residual: torch.Tensor | None, p: float, seed: int, start: int) -> torch.Tensor:
     keep = keep_mask(x.numel(), p, seed, start).view(x.shape)
     cut = _cut(p)
     scale = 65536.0 / (65536 - cut) if cut < 65536 else 0.0
@@ -53,12 +50,12 @@ class _DropoutAddFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, residual, p, seed, start):  # type: ignore[override]
         ctx.cfg = (p, seed, start)
-        return _apply(x, residual, p, seed, start)
+        return _apply_cpu(x, residual, p, seed, start)
 
     @staticmethod
     def backward(ctx, g):  # type: ignore[override]
         p, seed, start = ctx.cfg
-        dx = _apply(g.contiguous(), None, p, seed, start) if ctx.needs_input_grad[0] else None
+        dx = _apply_cpu(g.contiguous(), None, p, seed, start) if ctx.needs_input_grad[0] else None
         return dx, (g if ctx.needs_input_grad[1] else None), None, None, None
 
 
@@ -79,4 +76,8 @@ def dropout_add(x: torch.Tensor, residual: torch.Tensor | None, p: float, seed: 
         raise ValueError(f"negative start {start}")
     if residual is not None and (residual.shape != x.shape or residual.dtype != x.dtype):
         raise ValueError(f"residual {tuple(residual.shape)} {residual.dtype} does not match x {tuple(x.shape)} {x.dtype}")
-    return _DropoutAddFn.apply(x.contiguous(), None if residual is None else residual.contiguous(), p, seed, start)
+    x, residual = x.contiguous(), None if residual is None else residual.contiguous()
+    if x.is_cuda:
+        key = seed - (1 << 64) if seed >= 1 << 63 else seed  # the same 64 bits, signed
+        return native().dropout_add(x, residual, _cut(p), key, start)
+    return _DropoutAddFn.apply(x, residual, p, seed, start)

@@ -190,5 +190,6 @@ def linear_fp8(x: torch.Tensor, weight: torch.Tensor | Fp8Blocks, *, residual: t
             raise ValueError("weights kept in 8 bits have no backward: call linear_fp8 with the weight tensor")
         y = fp8_matmul(_quantize(x2, False, True, False)[0], weight, residual=r2, out_dtype=x.dtype)
     else:
-        y = _LinearFp8Fn.apply(x2, weight if weight.is_contiguous() else weight.contiguous(), r2, main_grad)
+        w = weight if weight.is_contiguous() else weight.contiguous()
+        y = native().linear_fp8(x2, w, r2) if x.is_cuda and main_grad is None else _LinearFp8Fn.apply(x2, w, r2, main_grad)
     return y.view(*x.shape[:-1], N)

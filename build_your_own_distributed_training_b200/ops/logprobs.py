@@ -83,12 +83,8 @@ def _reference_grad(x, tokens, state, g_lp, g_ent, temperature):
 class _TokenLogProbsFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, tokens, temperature, top_k, ignore):  # type: ignore[override]
-        if x.is_cuda:
-            lp, ent, state, top_v, top_i = native().token_logprobs_fwd(x, tokens, temperature, top_k, ignore)
-            ctx.save_for_backward(x, tokens, state)
-        else:
-            lp, ent, top_v, top_i, state = _reference(x, tokens, temperature, top_k, ignore)
-            ctx.save_for_backward(x, tokens, *state)
+        lp, ent, top_v, top_i, state = _reference(x, tokens, temperature, top_k, ignore)
+        ctx.save_for_backward(x, tokens, *state)
         ctx.temperature = temperature
         ctx.mark_non_differentiable(top_v, top_i)
         ctx.set_materialize_grads(False)
@@ -97,15 +93,7 @@ class _TokenLogProbsFn(torch.autograd.Function):
     @staticmethod
     def backward(ctx, g_lp, g_ent, _v, _i):  # type: ignore[override]
         x, tokens, *state = ctx.saved_tensors
-        if not x.is_cuda:
-            return _reference_grad(x, tokens, state, g_lp, g_ent, ctx.temperature).to(x.dtype), None, None, None, None
-        # the gradient's rows lie as the logits' rows do (padded vocabulary buffers included)
-        pitch = max(x.stride(0), x.shape[1]) if x.shape[0] > 1 else x.shape[1]
-        if pitch > 2 * x.shape[1] + 1024:
-            pitch = x.shape[1]
-        dx = torch.empty(x.shape[0], pitch, device=x.device, dtype=x.dtype)[:, :x.shape[1]]
-        native().token_logprobs_bwd(x, tokens, state[0], _row_grad(g_lp), _row_grad(g_ent), ctx.temperature, dx)
-        return dx, None, None, None, None
+        return _reference_grad(x, tokens, state, g_lp, g_ent, ctx.temperature).to(x.dtype), None, None, None, None
 
 
 def _row_grad(g: torch.Tensor | None) -> torch.Tensor | None:
@@ -137,8 +125,9 @@ def token_log_probs(logits: torch.Tensor, tokens: torch.Tensor, *, temperature: 
     x = logits if logits.dim() == 2 else logits.reshape(-1, V)
     if x.stride(1) != 1:
         x = x.contiguous()
-    lp, ent, top_v, top_i = _TokenLogProbsFn.apply(x, tokens.reshape(-1).contiguous(), float(temperature),
-                                                   int(top_k), int(ignore_index))
+    apply = native().token_logprobs if x.is_cuda else _TokenLogProbsFn.apply
+    lp, ent, top_v, top_i = apply(x, tokens.reshape(-1).contiguous(), float(temperature), int(top_k),
+                                  int(ignore_index))
     return _shaped(lp, ent, top_v, top_i, tokens.shape, top_k)
 
 

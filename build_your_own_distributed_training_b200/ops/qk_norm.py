@@ -133,5 +133,8 @@ def qk_norm_rope(qkv: torch.Tensor, q_weight: torch.Tensor, k_weight: torch.Tens
             raise ValueError(f"{positions.numel()} positions for {qkv.shape[0]} tokens")
     if qkv.stride(1) != 1:
         qkv = qkv.contiguous()
+    if qkv.is_cuda and main_grads is None and grad_reduce is None:
+        return native().qk_norm_rope(qkv, q_weight, k_weight, cos, sin, positions, n_q_heads, n_kv_heads, head_dim,
+                                     seqlen, eps)
     return _QKNormRopeFn.apply(qkv, q_weight, k_weight, cos, sin, positions, n_q_heads, n_kv_heads, head_dim,
                                seqlen, eps, main_grads, grad_reduce)
