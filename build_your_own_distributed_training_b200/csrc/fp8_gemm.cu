@@ -4,21 +4,32 @@
 //
 // A [M, K] and B [N, K] are e4m3 codes with the summed axis contiguous; the scales are e8m0.
 //
-// Persistent tcgen05 kernel, one CTA per SM, 12 warps:
-//   warp 0       TMA: 128 x 128-byte tiles of A and B (128-byte swizzle) into a 4-stage ring;
-//   warp 1       one thread issues, per stage, three tcgen05.cp (the stage's scales, shared memory ->
-//                tensor memory) and four block-scaled MMAs (kind::mxf8f6f4, 128 x BN x 32);
-//   warps 2, 3   gather the scale bytes of A's and B's rows of the stage from global memory, four stages
-//                ahead in registers, and lay them out for tcgen05.cp;
-//   warps 4-11   epilogue: two warpgroups, each half of the tile's columns.
+// Persistent tcgen05 kernel, 10 warps per CTA, one CTA per SM.  Large products run on CTA pairs: a (2,1,1)
+// cluster computes a 256 x 256 tile with cta_group::2 MMAs that the even CTA issues; each CTA holds its 128
+// rows of A and 128 columns of B.  Small ones run on single CTAs with 128 x 128 tiles.
+//   warp 0       TMA: 128 x 128-byte tiles of A and B (128-byte swizzle) and their scale tiles into a 6-stage
+//                ring;
+//   warp 1       one thread issues, per stage, the tcgen05.cp of the stage's scales (shared memory -> tensor
+//                memory) and four block-scaled MMAs (kind::mxf8f6f4, 32 deep);
+//   warps 2-9    epilogue: two warpgroups, each half of the tile's columns.
 // The hardware applies a scale to 32 elements; a block of 128 is four of them, so a 128-deep stage has one
 // scale byte per row, repeated in the four byte places of its 32-bit word, and every MMA of the stage reads
 // the word's byte 0.  Powers of two make the scaling exact: the sum is the fp32 accumulation of the codes'
 // products in tensor memory, over all of K, with no promotion pass through registers.
 //
-// Tensor memory: the accumulator takes 256 columns (one 128 x 256 tile, or two 128 x 128 tiles in turn), the
-// scales 16 columns per stage.  With 256-column tiles the accumulator is read into registers as bf16 before
-// the tile is stored, so the MMAs of the next tile wait only for that read.
+// Scale tiles: for each 128 rows and each 128-block of K the 512 bytes that tcgen05.cp takes (row r: the
+// 32-bit word at (r % 32) * 16 + (r / 32) * 4), written by the quantisation kernels, 3% of the codes' bytes.
+// Gathering scale bytes from a plain [rows, blocks] tensor inside this kernel was measured and left: two
+// warps per CTA could not keep up (their loads' latency came back once per stage), 1230 against
+// 2700 TFLOP/s at 8192 x 11008 x 4096.
+//
+// What bounds it: a 128 x 256 x 128 step takes the tensor cores 512 cycles, in which one CTA alone would
+// move 48 KB into shared memory and read 48 KB from it, 192 bytes a cycle against the 128 there are.  A pair
+// halves B's share: 64 KB per CTA and step, 128 bytes a cycle.
+//
+// Tensor memory: the accumulator takes 256 columns (one 256-column tile, or two 128-column tiles in turn),
+// the scales 16 columns per stage.  With 256-column tiles the accumulator is read into registers as bf16
+// before the tile is stored, so the MMAs of the next tile wait only for that read.
 #include <ATen/cuda/CUDAContext.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <cudaTypedefs.h>
@@ -34,15 +45,8 @@ namespace fp8 {
 
 enum Out : int { OUT_BF16 = 0, OUT_F32 = 1, OUT_ACC_F32 = 2 };
 
-struct Scale {
-  const uint8_t* s;
-  long row, blk;  // strides of the row group and of the 128-block of K, in bytes
-  int gran;       // rows per group: 1 or 128
-};
-
 struct GemmArgs {
   int M, N, K;
-  Scale sa, sb;
   void* D;
   long ldd;
   const __nv_bfloat16* R;  // OUT_BF16: residual, or null
@@ -52,12 +56,13 @@ struct GemmArgs {
   int* err;
 };
 
-constexpr int BM = 128, BK = 128, STAGES = 4, GROUP_M = 16;
+constexpr int BM = 128, BK = 128, STAGES = 6, GROUP_M = 16;
 constexpr uint32_t TMEM_COLS = 512, SF_COL = 256;
 
-template <int BN>
+// PAIR: each CTA of a pair holds half of B's columns
+template <int BN, bool PAIR>
 struct Smem {
-  static constexpr int A_BYTES = BM * BK, B_BYTES = BN * BK;
+  static constexpr int A_BYTES = BM * BK, B_BYTES = (PAIR ? BN / 2 : BN) * BK;
   static constexpr int STAGE = A_BYTES + B_BYTES;
   static constexpr int SF_OFF = STAGES * STAGE;
   static constexpr int SF_STAGE = 512 * (1 + BN / 128);  // 512 bytes for each 128 rows of A and of B
@@ -65,6 +70,7 @@ struct Smem {
   static constexpr int STG_BYTES = 8 * 2048;             // per epilogue warp: 32 rows x 64 bytes
   static constexpr int BAR_OFF = STG_OFF + STG_BYTES;
   static constexpr int TOTAL = BAR_OFF + 256 + 1024;     // + alignment slack
+  static constexpr int TX = STAGE + SF_STAGE;            // bytes that land per stage and CTA
   static_assert(TOTAL <= 232448, "shared memory per CTA");
 };
 
@@ -81,12 +87,26 @@ __device__ __forceinline__ void umma_mxf8(uint32_t d, uint64_t ad, uint64_t bd, 
       "l"(ad), "l"(bd), "r"(idesc), "r"(sfa), "r"(sfb), "r"(accumulate)
       : "memory");
 }
+__device__ __forceinline__ void umma_mxf8_pair(uint32_t d, uint64_t ad, uint64_t bd, uint32_t idesc, uint32_t sfa,
+                                               uint32_t sfb, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %6, 0;\n\t"
+      "tcgen05.mma.cta_group::2.kind::mxf8f6f4.block_scale [%0], %1, %2, %3, [%4], [%5], p;\n\t}" ::"r"(d),
+      "l"(ad), "l"(bd), "r"(idesc), "r"(sfa), "r"(sfb), "r"(accumulate)
+      : "memory");
+}
 // 512 bytes (32 lanes x 16 bytes) of shared memory to 4 columns of every 32-lane quarter
+// (of each CTA of a pair, from its own shared memory)
+template <bool PAIR>
 __device__ __forceinline__ void tmem_copy_scales(uint32_t taddr, uint32_t saddr) {
   // no swizzle, 8 x 16-byte core matrices one after the other
   const uint64_t desc = (uint64_t)((saddr >> 4) & 0x3FFF) | ((uint64_t)(128 >> 4) << 16) |
                         ((uint64_t)(128 >> 4) << 32) | ((uint64_t)1 << 46);
-  asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(desc) : "memory");
+  if constexpr (PAIR)
+    asm volatile("tcgen05.cp.cta_group::2.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(desc) : "memory");
+  else
+    asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(desc) : "memory");
 }
 
 __device__ __forceinline__ void tile_coords(int tile, int mblocks, int nblocks, int& mb, int& nb) {
@@ -96,12 +116,6 @@ __device__ __forceinline__ void tile_coords(int tile, int mblocks, int nblocks, 
   const int r = tile - g * per_group;
   mb = first + r % gm;
   nb = r / gm;
-}
-
-// the scale byte of a row, 1.0 outside the matrix
-__device__ __forceinline__ uint32_t scale_of(const Scale& s, int row, int rows, int kb) {
-  if (row >= rows) return 127u;
-  return __ldg(s.s + (long)(s.gran == 1 ? row : row >> 7) * s.row + (long)kb * s.blk);
 }
 
 // 32 rows x 64 bytes staged by the warp (16-byte chunks swizzled by the row) -> global rows
@@ -133,10 +147,14 @@ __device__ __forceinline__ void store_segment(const GemmArgs& a, uint8_t* stg, i
       float e[4] = {__uint_as_float(v.x), __uint_as_float(v.y), __uint_as_float(v.z), __uint_as_float(v.w)};
       if (vec) {
         if constexpr (OUT == OUT_ACC_F32) {
-          const float4 o = *reinterpret_cast<const float4*>(d);
-          e[0] += o.x, e[1] += o.y, e[2] += o.z, e[3] += o.w;
+          // each element is added to once, by one thread: the reduction happens in L2, nothing waits for
+          // the old value (accumulating 8192 x 11008 with loads held the accumulator 280 us longer)
+          asm volatile("red.global.add.v4.f32 [%0], {%1, %2, %3, %4};" ::"l"(d), "f"(e[0]), "f"(e[1]), "f"(e[2]),
+                       "f"(e[3])
+                       : "memory");
+        } else {
+          *reinterpret_cast<float4*>(d) = make_float4(e[0], e[1], e[2], e[3]);
         }
-        *reinterpret_cast<float4*>(d) = make_float4(e[0], e[1], e[2], e[3]);
       } else {
 #pragma unroll
         for (int k = 0; k < PER; ++k)
@@ -170,12 +188,15 @@ __device__ __forceinline__ void add_residual(const GemmArgs& a, int row, int col
   }
 }
 
-template <int BN, int OUT>
-__global__ void __launch_bounds__(384, 1)
+template <int BN, bool PAIR, int OUT>
+__global__ void __launch_bounds__(320, 1)
     fp8_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB,
+                    const __grid_constant__ CUtensorMap tmSA, const __grid_constant__ CUtensorMap tmSB,
                     const GemmArgs args) {
-  using L = Smem<BN>;
+  static_assert(PAIR == (BN == 256), "CTA pairs compute 256-column tiles");
+  using L = Smem<BN, PAIR>;
   constexpr int ACCS = BN == 256 ? 1 : 2;  // accumulators of BN columns in 256
+  constexpr int TILE_M = PAIR ? 2 * BM : BM, CTAS = PAIR ? 2 : 1;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint64_t* full = reinterpret_cast<uint64_t*>(smem + L::BAR_OFF);
@@ -185,27 +206,39 @@ __global__ void __launch_bounds__(384, 1)
   uint32_t* tmem_holder = reinterpret_cast<uint32_t*>(acc_empty + 2);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_holder + 1);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int cta = PAIR ? (int)cluster_ctarank() : 0;
+  const bool leader = cta == 0;
+  const int unit = (int)blockIdx.x / CTAS, units = (int)gridDim.x / CTAS;
 
   if (threadIdx.x == 0) {
     for (int s = 0; s < STAGES; ++s) {
-      mbar_init(&full[s], 3);  // the TMA thread and the two scale warps
+      mbar_init(&full[s], 1);
       mbar_init(&empty[s], 1);
     }
     for (int i = 0; i < 2; ++i) {
       mbar_init(&acc_full[i], 1);
-      mbar_init(&acc_empty[i], 8);
+      mbar_init(&acc_empty[i], 8 * CTAS);
     }
     *abort_flag = 0;
-    fence_mbar_init();
+    if constexpr (PAIR) fence_mbar_init_cluster();
+    else fence_mbar_init();
     tma_prefetch_desc(&tmA);
     tma_prefetch_desc(&tmB);
+    tma_prefetch_desc(&tmSA);
+    tma_prefetch_desc(&tmSB);
   }
   if (warp == 1) {
-    tmem_alloc(tmem_holder, TMEM_COLS);
-    tmem_relinquish();
+    if constexpr (PAIR) {
+      tmem_alloc_pair(tmem_holder, TMEM_COLS);
+      tmem_relinquish_pair();
+    } else {
+      tmem_alloc(tmem_holder, TMEM_COLS);
+      tmem_relinquish();
+    }
   }
   tc_fence_before();
   __syncthreads();
+  if constexpr (PAIR) cluster_sync();  // the peer's barriers exist before any remote arrive
   tc_fence_after();
   const uint32_t tmem = *tmem_holder;
 
@@ -215,7 +248,7 @@ __global__ void __launch_bounds__(384, 1)
       uint32_t phase = 0;
       uint32_t issued = 0, issued_phase = 0;  // bit per stage
       bool ok = true;
-      for (int tile = blockIdx.x; tile < args.num_tiles && ok; tile += gridDim.x) {
+      for (int tile = unit; tile < args.num_tiles && ok; tile += units) {
         int mb, nb;
         tile_coords(tile, args.m_blocks, args.n_blocks, mb, nb);
         for (int k = 0; k < args.k_iters; ++k) {
@@ -225,27 +258,43 @@ __global__ void __launch_bounds__(384, 1)
             break;
           }
           uint8_t* sa = smem + stage * L::STAGE;
-          mbar_arrive_expect_tx(&full[stage], L::STAGE);
-          tma_load_2d(sa, &tmA, &full[stage], k * BK, mb * BM);
+          uint8_t* sf = smem + L::SF_OFF + stage * L::SF_STAGE;
+          // row blocks of this CTA; a pair's CTAs both take all of B's scales, for their own tensor memory
+          const int arow = mb * CTAS + cta, brow = nb * (BN / 128);
+          // a pair's bytes complete on the leader's barrier
+          if (leader) mbar_arrive_expect_tx(&full[stage], CTAS * L::TX);
+          if constexpr (PAIR) {
+            const uint32_t fb = mapa_shared(smem_u32(&full[stage]), 0);
+            tma_load_2d_pair(sa, &tmA, fb, k * BK, arow * BM);
+            tma_load_2d_pair(sa + L::A_BYTES, &tmB, fb, k * BK, (brow + cta) * 128);
+            tma_load_2d_pair(sf, &tmSA, fb, 0, arow * args.k_iters + k);
 #pragma unroll
-          for (int j = 0; j < BN / 128; ++j)
-            tma_load_2d(sa + L::A_BYTES + j * 16384, &tmB, &full[stage], k * BK, nb * BN + j * 128);
+            for (int j = 0; j < BN / 128; ++j)
+              tma_load_2d_pair(sf + 512 * (1 + j), &tmSB, fb, 0, (brow + j) * args.k_iters + k);
+          } else {
+            tma_load_2d(sa, &tmA, &full[stage], k * BK, arow * BM);
+            tma_load_2d(sa + L::A_BYTES, &tmB, &full[stage], k * BK, brow * 128);
+            tma_load_2d(sf, &tmSA, &full[stage], 0, arow * args.k_iters + k);
+            tma_load_2d(sf + 512, &tmSB, &full[stage], 0, brow * args.k_iters + k);
+          }
           issued |= 1u << stage;
           issued_phase = (issued_phase & ~(1u << stage)) | (phase << stage);
           if (++stage == STAGES) stage = 0, phase ^= 1;
         }
       }
-      if (!ok)  // copies in flight land before the shared memory goes away
+      // copies in flight land before the shared memory goes away (a pair's follower has no barrier of its
+      // own for them: its bounded waits outlast its last copy by far)
+      if (!ok && leader)
         for (int s = 0; s < STAGES; ++s)
           if (issued >> s & 1) mbar_wait(&full[s], issued_phase >> s & 1, args.err);
     }
   } else if (warp == 1) {
-    if (lane == 0) {
+    if (lane == 0 && leader) {
       int stage = 0, t = 0;
       uint32_t phase = 0;
       bool ok = true;
-      constexpr uint32_t IDESC = idesc_mxf8(BM, BN);
-      for (int tile = blockIdx.x; tile < args.num_tiles && ok; tile += gridDim.x, ++t) {
+      constexpr uint32_t IDESC = idesc_mxf8(TILE_M, BN);
+      for (int tile = unit; tile < args.num_tiles && ok; tile += units, ++t) {
         const int acc = t % ACCS;
         const uint32_t acc_phase = (t / ACCS) & 1;
         if (*abort_flag || !mbar_wait(&acc_empty[acc], acc_phase ^ 1, args.err)) {
@@ -263,77 +312,29 @@ __global__ void __launch_bounds__(384, 1)
           const uint32_t a0 = smem_u32(smem + stage * L::STAGE), b0 = a0 + L::A_BYTES;
           const uint32_t sf = smem_u32(smem + L::SF_OFF + stage * L::SF_STAGE);
           const uint32_t sfa = tmem + SF_COL + stage * 16, sfb = sfa + 4;
-          tmem_copy_scales(sfa, sf);
+          tmem_copy_scales<PAIR>(sfa, sf);
 #pragma unroll
-          for (int j = 0; j < BN / 128; ++j) tmem_copy_scales(sfb + 4 * j, sf + 512 * (1 + j));
+          for (int j = 0; j < BN / 128; ++j) tmem_copy_scales<PAIR>(sfb + 4 * j, sf + 512 * (1 + j));
 #pragma unroll
-          for (int kk = 0; kk < BK / 32; ++kk)
-            umma_mxf8(tmem + acc * BN, sdesc_sw128(a0 + kk * 32, 16, 1024), sdesc_sw128(b0 + kk * 32, 16, 1024), IDESC,
-                      sfa, sfb, k != 0 || kk != 0);
-          umma_commit(&empty[stage]);
+          for (int kk = 0; kk < BK / 32; ++kk) {
+            const uint64_t ad = sdesc_sw128(a0 + kk * 32, 16, 1024), bd = sdesc_sw128(b0 + kk * 32, 16, 1024);
+            if constexpr (PAIR) umma_mxf8_pair(tmem + acc * BN, ad, bd, IDESC, sfa, sfb, k != 0 || kk != 0);
+            else umma_mxf8(tmem + acc * BN, ad, bd, IDESC, sfa, sfb, k != 0 || kk != 0);
+          }
+          if constexpr (PAIR) umma_commit_pair(&empty[stage]);
+          else umma_commit(&empty[stage]);
           if (++stage == STAGES) stage = 0, phase ^= 1;
         }
-        umma_commit(&acc_full[acc]);
-      }
-    }
-  } else if (warp < 4) {
-    // scale bytes: lane l holds rows l, l + 32, l + 64, l + 96 of each 128, PF stages ahead of their use
-    constexpr int PF = 4;
-    const bool isb = warp == 3;
-    const int parts = isb ? BN / 128 : 1;
-    const Scale sc = isb ? args.sb : args.sa;
-    const int rows = isb ? args.N : args.M;
-    uint32_t w[PF][BN / 128][4];
-    int ltile = blockIdx.x, lk = 0;  // the next stage to load
-    auto load = [&](uint32_t (&d)[BN / 128][4]) {
-      if (ltile >= args.num_tiles) return;
-      int mb, nb;
-      tile_coords(ltile, args.m_blocks, args.n_blocks, mb, nb);
-      const int base = isb ? nb * BN : mb * BM;
-#pragma unroll
-      for (int p = 0; p < BN / 128; ++p)
-        if (p < parts) {
-#pragma unroll
-          for (int j = 0; j < 4; ++j) d[p][j] = scale_of(sc, base + p * 128 + j * 32 + lane, rows, lk);
-        }
-      if (++lk == args.k_iters) lk = 0, ltile += gridDim.x;
-    };
-#pragma unroll
-    for (int i = 0; i < PF; ++i) load(w[i]);
-    const long mine = (args.num_tiles - 1 - (int)blockIdx.x) / (int)gridDim.x + 1;  // grid <= num_tiles
-    const long total = mine * args.k_iters;
-    int stage = 0;
-    uint32_t phase = 0;
-    bool ok = true;
-    for (long it = 0; it < total && ok; it += PF) {
-#pragma unroll
-      for (int i = 0; i < PF; ++i) {
-        if (it + i >= total || !ok) break;
-        if (*abort_flag || !mbar_wait(&empty[stage], phase ^ 1, args.err)) {
-          *abort_flag = 1;
-          ok = false;
-          break;
-        }
-        uint8_t* sf = smem + L::SF_OFF + stage * L::SF_STAGE + (isb ? 512 : 0);
-#pragma unroll
-        for (int p = 0; p < BN / 128; ++p)
-          if (p < parts)
-            *reinterpret_cast<uint4*>(sf + p * 512 + lane * 16) =
-                make_uint4(w[i][p][0] * 0x01010101u, w[i][p][1] * 0x01010101u, w[i][p][2] * 0x01010101u,
-                           w[i][p][3] * 0x01010101u);
-        fence_proxy_async_smem();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&full[stage]);
-        load(w[i]);
-        if (++stage == STAGES) stage = 0, phase ^= 1;
+        if constexpr (PAIR) umma_commit_pair(&acc_full[acc]);
+        else umma_commit(&acc_full[acc]);
       }
     }
   } else {
-    const int quad = warp & 3, half = (warp - 4) >> 2;  // TMEM lanes 32 quad .., columns half * BN / 2 ..
-    uint8_t* stg = smem + L::STG_OFF + (warp - 4) * 2048;
+    const int quad = warp & 3, half = (warp - 2) >> 2;  // TMEM lanes 32 quad .., columns half * BN / 2 ..
+    uint8_t* stg = smem + L::STG_OFF + (warp - 2) * 2048;
     constexpr int COLS = BN / 2;
     int t = 0;
-    for (int tile = blockIdx.x; tile < args.num_tiles; tile += gridDim.x, ++t) {
+    for (int tile = unit; tile < args.num_tiles; tile += units, ++t) {
       const int acc = t % ACCS;
       const uint32_t acc_phase = (t / ACCS) & 1;
       int mb, nb;
@@ -344,20 +345,33 @@ __global__ void __launch_bounds__(384, 1)
       }
       tc_fence_after();
       const uint32_t tb = tmem + ((uint32_t)(quad * 32) << 16) + acc * BN + half * COLS;
-      const int row0 = mb * BM + quad * 32, col0 = nb * BN + half * COLS;
+      const int row0 = mb * TILE_M + cta * BM + quad * 32, col0 = nb * BN + half * COLS;
       if constexpr (OUT == OUT_BF16) {
         uint32_t h[COLS / 2];
 #pragma unroll
-        for (int c = 0; c < COLS; c += 32) {
-          float v[32];
-          tmem_ld32(tb + c, v);
-          if (args.R != nullptr) add_residual(args, row0 + lane, col0 + c, v);
+        for (int c = 0; c < COLS; c += 64) {
+          uint32_t r[2][32];
+          tmem_ld32_async(tb + c, r[0]);
+          tmem_ld32_async(tb + c + 32, r[1]);
+          tmem_wait_ld();
+          tmem_regs(r[0]);
+          tmem_regs(r[1]);
 #pragma unroll
-          for (int i = 0; i < 16; ++i) h[c / 2 + i] = pack_bf16x2(v[2 * i], v[2 * i + 1]);
+          for (int p = 0; p < 2; ++p) {
+            float v[32];
+#pragma unroll
+            for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(r[p][i]);
+            if (args.R != nullptr) add_residual(args, row0 + lane, col0 + c + 32 * p, v);
+#pragma unroll
+            for (int i = 0; i < 16; ++i) h[c / 2 + 16 * p + i] = pack_bf16x2(v[2 * i], v[2 * i + 1]);
+          }
         }
         tc_fence_before();
         __syncwarp();
-        if (lane == 0) mbar_arrive(&acc_empty[acc]);
+        if (lane == 0) {
+          if constexpr (PAIR) mbar_arrive_cluster(mapa_shared(smem_u32(&acc_empty[acc]), 0));
+          else mbar_arrive(&acc_empty[acc]);
+        }
 #pragma unroll
         for (int c = 0; c < COLS; c += 32) {
 #pragma unroll
@@ -382,14 +396,31 @@ __global__ void __launch_bounds__(384, 1)
         }
         tc_fence_before();
         __syncwarp();
-        if (lane == 0) mbar_arrive(&acc_empty[acc]);
+        if (lane == 0) {
+          if constexpr (PAIR) mbar_arrive_cluster(mapa_shared(smem_u32(&acc_empty[acc]), 0));
+          else mbar_arrive(&acc_empty[acc]);
+        }
       }
     }
   }
   tc_fence_before();
   __syncthreads();
+  if constexpr (PAIR) cluster_sync();  // no remote arrive or operand read targets a CTA that has left
   tc_fence_after();
-  if (warp == 1) tmem_dealloc(tmem, TMEM_COLS);
+  if (warp == 1) {
+    if constexpr (PAIR) tmem_dealloc_pair(tmem, TMEM_COLS);
+    else tmem_dealloc(tmem, TMEM_COLS);
+  }
+}
+
+// Scale tiles of a plain e8m0 scale tensor [row groups, k blocks] (strides in bytes): one block of 128
+// threads per tile, thread r its row.
+__global__ void __launch_bounds__(128) scale_tiles_kernel(const uint8_t* __restrict__ s, long row_stride, long blk_stride,
+                                                          int gran, int rows, int kb, uint32_t* __restrict__ tiles) {
+  const int mt = blockIdx.x / kb, k = blockIdx.x % kb, r = threadIdx.x;
+  const int row = min(mt * 128 + r, rows - 1);
+  const uint32_t b = s[(long)(gran == 1 ? row : mt) * row_stride + k * blk_stride];
+  tiles[(long)blockIdx.x * 128 + (r & 31) * 4 + (r >> 5)] = b * 0x01010101u;
 }
 
 // ---------------------------------------------------------------- host side
@@ -405,8 +436,8 @@ static PFN_cuTensorMapEncodeTiled_v12000 encode_fn() {
   return fn;
 }
 
-// [rows, inner] bytes, boxes of 128 rows x 128 bytes; bytes past the matrix read as zero
-static CUtensorMap make_map(const void* base, long inner, long rows, long pitch) {
+static CUtensorMap make_map(CUtensorMapDataType type, CUtensorMapSwizzle swizzle, const void* base, long inner, long rows,
+                            long pitch, int box_inner, int box_rows) {
   static thread_local bool bound = false;
   if (!bound) {  // the driver call needs a current context on this thread (autograd's workers)
     DTB_CUDA(cudaFree(nullptr));
@@ -415,24 +446,48 @@ static CUtensorMap make_map(const void* base, long inner, long rows, long pitch)
   CUtensorMap m;
   cuuint64_t dims[2] = {(cuuint64_t)inner, (cuuint64_t)rows};
   cuuint64_t strides[1] = {(cuuint64_t)pitch};
-  cuuint32_t box[2] = {128, 128};
+  cuuint32_t box[2] = {(cuuint32_t)box_inner, (cuuint32_t)box_rows};
   cuuint32_t estr[2] = {1, 1};
-  CUresult r = encode_fn()(&m, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(base), dims, strides, box, estr,
-                           CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
-                           CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  CUresult r = encode_fn()(&m, type, 2, const_cast<void*>(base), dims, strides, box, estr,
+                           CU_TENSOR_MAP_INTERLEAVE_NONE, swizzle, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                           CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   DTB_CHECK(r == CUDA_SUCCESS, "cuTensorMapEncodeTiled failed (%d): inner=%ld rows=%ld pitch=%ld base=%p", (int)r, inner, rows, pitch, base);
   return m;
 }
+// codes: boxes of 128 rows x 128 bytes; bytes past the matrix read as zero
+static CUtensorMap code_map(const torch::Tensor& t) {
+  const long rows = t.size(0), k = t.size(1);
+  return make_map(CU_TENSOR_MAP_DATA_TYPE_UINT8, CU_TENSOR_MAP_SWIZZLE_128B, t.data_ptr(), k, rows,
+                  rows > 1 ? t.stride(0) : (k + 15) / 16 * 16, 128, 128);
+}
+// scale tiles [row blocks, k blocks, 512 bytes]: one tile per box
+static CUtensorMap tile_map(const torch::Tensor& t) {
+  return make_map(CU_TENSOR_MAP_DATA_TYPE_UINT32, CU_TENSOR_MAP_SWIZZLE_NONE, t.data_ptr(), 128, t.size(0) * t.size(1),
+                  512, 128, 1);
+}
 
-template <int BN, int OUT>
-static void launch(const CUtensorMap& ta, const CUtensorMap& tb, GemmArgs& g, cudaStream_t st) {
-  using L = Smem<BN>;
-  auto kern = fp8_gemm_kernel<BN, OUT>;
+template <int BN, bool PAIR, int OUT>
+static void launch(const CUtensorMap* t, GemmArgs& g, cudaStream_t st) {
+  using L = Smem<BN, PAIR>;
+  constexpr int CTAS = PAIR ? 2 : 1;
+  auto kern = fp8_gemm_kernel<BN, PAIR, OUT>;
   DTB_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, L::TOTAL));
+  g.m_blocks = (g.M + CTAS * BM - 1) / (CTAS * BM);
   g.n_blocks = (g.N + BN - 1) / BN;
   g.num_tiles = g.m_blocks * g.n_blocks;
-  kern<<<std::min(g.num_tiles, device_sm_count()), 384, L::TOTAL, st>>>(ta, tb, g);
-  DTB_LAUNCH_CHECK();
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(CTAS * std::min(g.num_tiles, device_sm_count() / CTAS), 1, 1);
+  cfg.blockDim = dim3(320, 1, 1);
+  cfg.dynamicSmemBytes = L::TOTAL;
+  cfg.stream = st;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = CTAS;
+  attr[0].val.clusterDim.y = 1;
+  attr[0].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = PAIR ? 1 : 0;
+  DTB_CUDA(cudaLaunchKernelEx(&cfg, kern, t[0], t[1], t[2], t[3], g));
 }
 
 }  // namespace fp8
@@ -440,16 +495,10 @@ static void launch(const CUtensorMap& ta, const CUtensorMap& tb, GemmArgs& g, cu
 
 using namespace dtb;
 
-static fp8::Scale fp8_scale(const char* which, const torch::Tensor& q, const torch::Tensor& s, int64_t gran) {
-  const long kb = (q.size(1) + 127) / 128, groups = (q.size(0) + gran - 1) / gran;
-  DTB_CHECK(gran == 1 || gran == 128, "fp8_gemm: %s: blocks have 1 or 128 rows", which);
-  DTB_CHECK(s.device() == q.device() && s.scalar_type() == at::kFloat8_e8m0fnu && s.dim() == 2 && s.size(0) == groups && s.size(1) == kb, "fp8_gemm: %s: scales must be e8m0 [%ld, %ld]", which, groups, kb);
-  return {reinterpret_cast<const uint8_t*>(s.data_ptr()), s.stride(0), s.stride(1), (int)gran};
-}
-
 // D [M, N] = A [M, K] B [N, K]^T (+ R): D bf16 (R bf16, optional) or fp32 (accumulate: D += the product).
-void fp8_gemm(torch::Tensor A, torch::Tensor sA, int64_t granA, torch::Tensor B, torch::Tensor sB, int64_t granB,
-              torch::Tensor D, c10::optional<torch::Tensor> R, bool accumulate) {
+// tA, tB: the operands' scale tiles, uint8 [ceil(rows / 128), ceil(K / 128), 512].
+void fp8_gemm(torch::Tensor A, torch::Tensor tA, torch::Tensor B, torch::Tensor tB, torch::Tensor D,
+              c10::optional<torch::Tensor> R, bool accumulate) {
   for (const torch::Tensor* t : {&A, &B})
     DTB_CHECK(t->is_cuda() && t->device() == A.device() && t->scalar_type() == at::kFloat8_e4m3fn && t->dim() == 2 && (t->numel() == 0 || ((t->size(1) == 1 || t->stride(1) == 1) && t->stride(0) % 16 == 0 && (reinterpret_cast<uintptr_t>(t->data_ptr()) & 15) == 0)), "fp8_gemm: operands must be 2-D e4m3 on one GPU, rows contiguous and starting on 16-byte boundaries");
   const long M = A.size(0), N = B.size(0), K = A.size(1);
@@ -462,8 +511,10 @@ void fp8_gemm(torch::Tensor A, torch::Tensor sA, int64_t granA, torch::Tensor B,
   g.M = (int)M;
   g.N = (int)N;
   g.K = (int)K;
-  g.sa = fp8_scale("A", A, sA, granA);
-  g.sb = fp8_scale("B", B, sB, granB);
+  const torch::Tensor* q[2] = {&A, &B};
+  const torch::Tensor* t[2] = {&tA, &tB};
+  for (int i = 0; i < 2; ++i)
+    DTB_CHECK(t[i]->device() == A.device() && t[i]->scalar_type() == at::kByte && t[i]->is_contiguous() && t[i]->dim() == 3 && t[i]->size(0) == (q[i]->size(0) + 127) / 128 && t[i]->size(1) == (K + 127) / 128 && t[i]->size(2) == 512 && t[i]->size(0) * t[i]->size(1) < (1L << 31) && (reinterpret_cast<uintptr_t>(t[i]->data_ptr()) & 15) == 0, "fp8_gemm: scale tiles must be contiguous uint8 [ceil(rows / 128), ceil(K / 128), 512]");
   g.D = D.data_ptr();
   g.ldd = M > 1 ? D.stride(0) : N;
   g.err = dtb_error_word();
@@ -481,15 +532,28 @@ void fp8_gemm(torch::Tensor A, torch::Tensor sA, int64_t granA, torch::Tensor B,
     else if (!accumulate) D.zero_();
     return;
   }
-  g.m_blocks = (g.M + fp8::BM - 1) / fp8::BM;
   g.k_iters = (g.K + fp8::BK - 1) / fp8::BK;
   auto st = at::cuda::getCurrentCUDAStream();
-  const CUtensorMap ta = fp8::make_map(A.data_ptr(), K, M, M > 1 ? A.stride(0) : (K + 15) / 16 * 16);
-  const CUtensorMap tb = fp8::make_map(B.data_ptr(), K, N, N > 1 ? B.stride(0) : (K + 15) / 16 * 16);
-  // 256-column tiles once they fill the SMs
-  const bool wide = (long)g.m_blocks * ((N + 255) / 256) >= device_sm_count();
+  const CUtensorMap maps[4] = {fp8::code_map(A), fp8::code_map(B), fp8::tile_map(tA), fp8::tile_map(tB)};
+  // pairs once their 256 x 256 tiles fill the SMs
+  const bool pair = ((M + 255) / 256) * ((N + 255) / 256) >= device_sm_count() / 2;
   const int out = D.scalar_type() == at::kBFloat16 ? fp8::OUT_BF16 : accumulate ? fp8::OUT_ACC_F32 : fp8::OUT_F32;
-  if (out == fp8::OUT_BF16) wide ? fp8::launch<256, fp8::OUT_BF16>(ta, tb, g, st) : fp8::launch<128, fp8::OUT_BF16>(ta, tb, g, st);
-  else if (out == fp8::OUT_F32) wide ? fp8::launch<256, fp8::OUT_F32>(ta, tb, g, st) : fp8::launch<128, fp8::OUT_F32>(ta, tb, g, st);
-  else wide ? fp8::launch<256, fp8::OUT_ACC_F32>(ta, tb, g, st) : fp8::launch<128, fp8::OUT_ACC_F32>(ta, tb, g, st);
+  if (out == fp8::OUT_BF16) pair ? fp8::launch<256, true, fp8::OUT_BF16>(maps, g, st) : fp8::launch<128, false, fp8::OUT_BF16>(maps, g, st);
+  else if (out == fp8::OUT_F32) pair ? fp8::launch<256, true, fp8::OUT_F32>(maps, g, st) : fp8::launch<128, false, fp8::OUT_F32>(maps, g, st);
+  else pair ? fp8::launch<256, true, fp8::OUT_ACC_F32>(maps, g, st) : fp8::launch<128, false, fp8::OUT_ACC_F32>(maps, g, st);
+}
+
+// The scale tiles of plain scales: e8m0 [ceil(rows / gran), k blocks], gran 1 or 128.
+torch::Tensor fp8_scale_tiles(torch::Tensor s, int64_t gran, int64_t rows) {
+  DTB_CHECK(s.is_cuda() && s.scalar_type() == at::kFloat8_e8m0fnu && s.dim() == 2 && (gran == 1 || gran == 128) && rows >= 0 && rows < (1L << 30) && s.size(0) == (rows + gran - 1) / gran, "fp8_scale_tiles: e8m0 scales of 1 x 128 or 128 x 128 blocks");
+  const c10::cuda::CUDAGuard guard(s.device());
+  const long mt = (rows + 127) / 128, kb = s.size(1);
+  DTB_CHECK(mt * kb < (1L << 31), "fp8_scale_tiles: too large");
+  auto t = torch::empty({mt, kb, 512}, s.options().dtype(at::kByte));
+  if (mt * kb == 0) return t;
+  fp8::scale_tiles_kernel<<<(unsigned)(mt * kb), 128, 0, at::cuda::getCurrentCUDAStream()>>>(
+      reinterpret_cast<const uint8_t*>(s.data_ptr()), s.stride(0), s.stride(1), (int)gran, (int)rows, (int)kb,
+      reinterpret_cast<uint32_t*>(t.data_ptr()));
+  DTB_LAUNCH_CHECK();
+  return t;
 }

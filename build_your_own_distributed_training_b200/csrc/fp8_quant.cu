@@ -14,8 +14,8 @@
 // codes go through 16 KB of shared memory in 8-byte chunks (8 rows of one column) at chunk
 // rg ^ (column / 8), which is free of bank conflicts on the way in, and leave as 16-byte stores.
 //
-// Scales of 1 x 128 blocks are stored block-major, s[block][row]: the product reads the scales of 128
-// rows of one block together.
+// Scales leave twice: plain (1 x 128 blocks block-major, s[block][row]), for whoever reads the codes, and
+// as the 512-byte tiles that the product copies to tensor memory as they are (fp8_gemm.cu).
 #include <ATen/cuda/CUDAContext.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <cuda_fp8.h>
@@ -60,7 +60,13 @@ struct QuantArgs {
   uint8_t* qt;        // [C, qt_ld] transposed codes, or null
   long qt_ld;
   uint8_t* st;        // 1 x 128 of the transpose: [R / 128][C]
+  uint32_t* t;        // scale tiles of the codes as they lie: [R / 128][C / 128][128]
+  uint32_t* tt;       // and of the transpose: [C / 128][R / 128][128]
 };
+
+// word of row r (0..127) in a scale tile, and its value
+__device__ __forceinline__ int tile_word(int r) { return (r & 31) * 4 + (r >> 5); }
+__device__ __forceinline__ uint32_t tile_value(uint32_t byte) { return byte * 0x01010101u; }
 
 // One 128 x 128 tile per block of 256 threads: thread (rg, cg) holds rows rg * 8 + i, columns cg * 8 + k.
 template <typename T, bool SQUARE, bool WIDE>
@@ -104,13 +110,21 @@ __global__ void __launch_bounds__(256) quant_tile_kernel(const QuantArgs a) {
     for (int w = 0; w < 8; ++w) m = max(m, colmax[0][w]);
 #pragma unroll
     for (int i = 0; i < 8; ++i) rmax[i] = m;
-    if (tid == 0) a.s[(long)blockIdx.y * gridDim.x + blockIdx.x] = (uint8_t)scale_byte(m);
+    const uint32_t b = scale_byte(m);
+    const long at = (long)blockIdx.y * gridDim.x + blockIdx.x, att = (long)blockIdx.x * gridDim.y + blockIdx.y;
+    if (tid == 0) a.s[at] = (uint8_t)b;
+    if (tid < 128 && a.t != nullptr) a.t[at * 128 + tid] = tile_value(b);
+    if (tid >= 128 && a.tt != nullptr) a.tt[att * 128 + tid - 128] = tile_value(b);
   } else if (a.q != nullptr) {
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
 #pragma unroll
       for (int o = 1; o < 16; o <<= 1) rmax[i] = max(rmax[i], __shfl_xor_sync(0xffffffffu, rmax[i], o));
-      if (cg == i && r0 + i < a.R) a.s[(long)blockIdx.x * a.R + r0 + i] = (uint8_t)scale_byte(rmax[i]);
+      if (cg == i) {
+        const uint32_t b = scale_byte(rmax[i]);
+        if (r0 + i < a.R) a.s[(long)blockIdx.x * a.R + r0 + i] = (uint8_t)b;
+        a.t[((long)blockIdx.y * gridDim.x + blockIdx.x) * 128 + tile_word(rg * 8 + i)] = tile_value(b);
+      }
     }
   }
   if (a.q != nullptr) {
@@ -144,7 +158,10 @@ __global__ void __launch_bounds__(256) quant_tile_kernel(const QuantArgs a) {
       for (int w = 0; w < 8; ++w) m = max(m, colmax[w][cg * 8 + k]);
       const uint32_t b = scale_byte(m);
       f[k] = inv_scale(b);
-      if (rg == k && c0 + k < a.C) a.st[(long)blockIdx.y * a.C + c0 + k] = (uint8_t)b;
+      if (rg == k) {
+        if (c0 + k < a.C) a.st[(long)blockIdx.y * a.C + c0 + k] = (uint8_t)b;
+        a.tt[((long)blockIdx.x * gridDim.y + blockIdx.y) * 128 + tile_word(cg * 8 + k)] = tile_value(b);
+      }
     }
   }
 #pragma unroll
@@ -193,7 +210,10 @@ __global__ void __launch_bounds__(256) quant_rows_kernel(const QuantArgs a) {
   for (int o = 1; o < 16; o <<= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, o));
   if (!live) return;
   const uint32_t b = scale_byte(m);
-  if (cg == 0) a.s[(long)blk * a.R + row] = (uint8_t)b;
+  if (cg == 0) {
+    a.s[(long)blk * a.R + row] = (uint8_t)b;
+    a.t[((row >> 7) * cb + blk) * 128 + tile_word((int)(row & 127))] = tile_value(b);
+  }
   const float f = inv_scale(b);
   uint2 o;
   o.x = cvt4(v.at(0) * f, v.at(1) * f, v.at(2) * f, v.at(3) * f);
@@ -206,10 +226,10 @@ __global__ void __launch_bounds__(256) quant_rows_kernel(const QuantArgs a) {
 
 using namespace dtb;
 
-// x [R, C] -> {codes [R, C], scales, transposed codes [C, R], their scales}.  square: 128 x 128 blocks, scales
-// [R/128, C/128] and their transpose; else 1 x 128 along the last axis of each output, scales [R, C/128] and
-// [C, R/128] (block-major in memory).  Codes lie in rows padded to 16 bytes.  `plain` / `transposed` select
-// which of the two are made (undefined tensors stand for the other).
+// x [R, C] -> {codes [R, C], scales, scale tiles, transposed codes [C, R], their scales, their scale tiles}.
+// square: 128 x 128 blocks, scales [R/128, C/128] and their transpose; else 1 x 128 along the last axis of
+// each output, scales [R, C/128] and [C, R/128] (block-major in memory).  Codes lie in rows padded to 16
+// bytes.  `plain` / `transposed` select which of the two are made (undefined tensors stand for the other).
 std::vector<torch::Tensor> fp8_quantize(torch::Tensor x, bool square, bool plain, bool transposed) {
   DTB_CHECK(x.is_cuda() && x.dim() == 2 && is_float_type(x.scalar_type()) && (x.numel() == 0 || x.size(1) == 1 || x.stride(1) == 1), "fp8_quantize: x must be a 2-D CUDA tensor of fp32, bf16 or fp16 with contiguous columns");
   DTB_CHECK(plain || transposed, "fp8_quantize: nothing asked for");
@@ -221,7 +241,10 @@ std::vector<torch::Tensor> fp8_quantize(torch::Tensor x, bool square, bool plain
     return torch::empty({rows, pitch}, x.options().dtype(at::kFloat8_e4m3fn)).narrow(1, 0, cols);
   };
   auto opts = x.options().dtype(at::kFloat8_e8m0fnu);
-  torch::Tensor q, s, qt, st;
+  auto tiles = [&](long rb, long cb) { return torch::empty({rb, cb, 512}, x.options().dtype(at::kByte)); };
+  torch::Tensor q, s, t, qt, st, tt;
+  if (plain) t = tiles(RB, CB);
+  if (transposed) tt = tiles(CB, RB);
   if (plain) q = codes(R, C);
   if (transposed) qt = codes(C, R);
   if (square) {
@@ -231,7 +254,7 @@ std::vector<torch::Tensor> fp8_quantize(torch::Tensor x, bool square, bool plain
     if (plain) s = torch::empty({CB, R}, opts).t();
     if (transposed) st = torch::empty({RB, C}, opts).t();
   }
-  if (R == 0 || C == 0) return {q, s, qt, st};
+  if (R == 0 || C == 0) return {q, s, t, qt, st, tt};
   fp8::QuantArgs a{};
   a.x = x.data_ptr();
   a.ld = x.stride(0);
@@ -241,6 +264,8 @@ std::vector<torch::Tensor> fp8_quantize(torch::Tensor x, bool square, bool plain
     a.q = reinterpret_cast<uint8_t*>(q.data_ptr());
     a.q_ld = (C + 15) / 16 * 16;
   }
+  if (plain) a.t = reinterpret_cast<uint32_t*>(t.data_ptr());
+  if (transposed) a.tt = reinterpret_cast<uint32_t*>(tt.data_ptr());
   if (square || plain) a.s = reinterpret_cast<uint8_t*>(s.data_ptr());
   if (transposed) {
     a.qt = reinterpret_cast<uint8_t*>(qt.data_ptr());
@@ -267,5 +292,5 @@ std::vector<torch::Tensor> fp8_quantize(torch::Tensor x, bool square, bool plain
     }
   });
   DTB_LAUNCH_CHECK();
-  return {q, s, qt, st};
+  return {q, s, t, qt, st, tt};
 }

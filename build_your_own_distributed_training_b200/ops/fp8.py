@@ -31,10 +31,13 @@ E4M3, E8M0 = torch.float8_e4m3fn, torch.float8_e8m0fnu
 
 class Fp8Blocks(NamedTuple):
     """``values``: e4m3 ``[rows, cols]``; ``scales``: e8m0 ``[rows, ceil(cols / 128)]`` (one for each
-    1 x 128 block) or ``[ceil(rows / 128), ceil(cols / 128)]`` (128 x 128 blocks)."""
+    1 x 128 block) or ``[ceil(rows / 128), ceil(cols / 128)]`` (128 x 128 blocks); ``tiles`` (optional,
+    CUDA): the scales as the tensor-core kernel takes them, made by :func:`quantize_fp8` and from
+    ``scales`` in each product where absent."""
 
     values: torch.Tensor
     scales: torch.Tensor
+    tiles: torch.Tensor | None = None
 
     @property
     def rows_per_scale(self) -> int:
@@ -71,8 +74,8 @@ def _quantize_cpu(x: torch.Tensor, rows: int) -> Fp8Blocks:
 def _quantize(x: torch.Tensor, square: bool, plain: bool, transposed: bool) -> tuple[Fp8Blocks | None, Fp8Blocks | None]:
     """Codes as they lie and / or of the transpose, from one read of ``x``."""
     if x.is_cuda:
-        q, s, qt, st = native().fp8_quantize(x, square, plain, transposed)
-        return Fp8Blocks(q, s) if plain else None, Fp8Blocks(qt, st) if transposed else None
+        q, s, t, qt, st, tt = native().fp8_quantize(x, square, plain, transposed)
+        return Fp8Blocks(q, s, t) if plain else None, Fp8Blocks(qt, st, tt) if transposed else None
     a = _quantize_cpu(x.float(), BLOCK if square else 1) if plain else None
     b = _quantize_cpu(x.float().t(), BLOCK if square else 1) if transposed else None
     return a, b
@@ -99,8 +102,12 @@ def _aligned(b: Fp8Blocks) -> Fp8Blocks:
         r, c = v.shape
         pad = torch.empty(r, -(-c // 16) * 16, device=v.device, dtype=torch.uint8)[:, :c]
         pad.copy_(v.view(torch.uint8))
-        return Fp8Blocks(pad.view(E4M3), b.scales)
+        return Fp8Blocks(pad.view(E4M3), b.scales, b.tiles)
     return b
+
+
+def _tiles(b: Fp8Blocks, gran: int) -> torch.Tensor:
+    return b.tiles if b.tiles is not None else native().fp8_scale_tiles(b.scales, gran, b.values.shape[0])
 
 
 def fp8_matmul(a: Fp8Blocks, b: Fp8Blocks, *, residual: torch.Tensor | None = None, out: torch.Tensor | None = None,
@@ -123,7 +130,7 @@ def fp8_matmul(a: Fp8Blocks, b: Fp8Blocks, *, residual: torch.Tensor | None = No
         raise ValueError(f"residual is {tuple(residual.shape)}, the product {shape}")
     if a.values.is_cuda:
         a, b = _aligned(a), _aligned(b)
-        native().fp8_gemm(a.values, a.scales, ga, b.values, b.scales, gb, out, residual, accumulate)
+        native().fp8_gemm(a.values, _tiles(a, ga), b.values, _tiles(b, gb), out, residual, accumulate)
         return out
     y = a.dequantize() @ b.dequantize().t()
     if residual is not None:
@@ -138,23 +145,23 @@ class _LinearFp8Fn(torch.autograd.Function):
         xq, xt = _quantize(x2, False, True, need_w)
         wq, wt = _quantize(weight, True, True, need_x)
         y = fp8_matmul(xq, wq, residual=residual, out_dtype=x2.dtype)
-        ctx.save_for_backward(*(xt or (None, None)), *(wt or (None, None)))
+        ctx.save_for_backward(*(xt or (None,) * 3), *(wt or (None,) * 3))
         ctx.main_grad, ctx.need = main_grad, (need_x, need_w, residual is not None)
         ctx.wshape, ctx.wdtype = weight.shape, weight.dtype
         return y
 
     @staticmethod
     def backward(ctx, dy):  # type: ignore[override]
-        xv, xs, wv, ws = ctx.saved_tensors
+        saved = ctx.saved_tensors
         need_x, need_w, has_res = ctx.need
         dy2 = dy.contiguous()
         dx = dw = None
         if need_x or need_w:
             g, gt = _quantize(dy2, False, need_x, need_w)
         if need_x:
-            dx = fp8_matmul(g, Fp8Blocks(wv, ws), out_dtype=dy.dtype)
+            dx = fp8_matmul(g, Fp8Blocks(*saved[3:]), out_dtype=dy.dtype)
         if need_w:
-            mg, xt = ctx.main_grad, Fp8Blocks(xv, xs)
+            mg, xt = ctx.main_grad, Fp8Blocks(*saved[:3])
             if mg is not None:
                 store = grad_state.take_fresh(mg)
                 fp8_matmul(gt, xt, out=mg.view(ctx.wshape), accumulate=not store)

@@ -176,12 +176,15 @@ def test_refusals():
     with pytest.raises(ValueError, match="bf16"):
         ops.linear_fp8(x.float(), w)
     a, b = ops.quantize_fp8(x), ops.quantize_fp8(w)
+    out = torch.empty(4, 8, device=DEV)
+    for bad in ((a.values, a.tiles, b.values, b.tiles, out.half(), None, False),       # result type
+                (a.values, a.tiles, b.values[:, :60], b.tiles, out, None, False),      # shapes
+                (a.values, a.tiles[:, :, :256], b.values, b.tiles, out, None, False),  # scale tiles
+                (a.values, a.tiles, b.values, b.tiles, out.to(BF), None, True)):       # bf16 accumulation
+        with pytest.raises(RuntimeError):
+            native().fp8_gemm(*bad)
     with pytest.raises(RuntimeError):
-        native().fp8_gemm(a.values, a.scales, 1, b.values, b.scales, 1, torch.empty(4, 8, device=DEV, dtype=HF), None, False)
-    with pytest.raises(RuntimeError):
-        native().fp8_gemm(a.values, a.scales, 1, b.values[:, :60], b.scales, 1, torch.empty(4, 8, device=DEV), None, False)
-    with pytest.raises(RuntimeError):
-        native().fp8_gemm(a.values, a.scales, 2, b.values, b.scales, 1, torch.empty(4, 8, device=DEV), None, False)
+        native().fp8_scale_tiles(a.scales, 2, 4)
 
 
 def test_kept_weights_on_another_stream_and_repeats():
