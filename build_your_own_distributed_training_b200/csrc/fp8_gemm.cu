@@ -12,23 +12,23 @@
 //   warp 1       one thread issues, per stage, the tcgen05.cp of the stage's scales (shared memory -> tensor
 //                memory) and four block-scaled MMAs (kind::mxf8f6f4, 32 deep);
 //   warps 2-9    epilogue: two warpgroups, each half of the tile's columns.
-// The hardware applies a scale to 32 elements; a block of 128 is four of them, so a 128-deep stage has one
-// scale byte per row, repeated in the four byte places of its 32-bit word, and every MMA of the stage reads
-// the word's byte 0.  Powers of two make the scaling exact: the sum is the fp32 accumulation of the codes'
-// products in tensor memory, over all of K, with no promotion pass through registers.
+// The hardware applies a scale to 32 elements, one byte of a row's 32-bit scale word; a block of 128 is four
+// of them, so the four MMAs of a 128-deep stage read the same byte, and a word serves four stages.  Powers of
+// two make the scaling exact: the sum is the fp32 accumulation of the codes' products in tensor memory, over
+// all of K, with no promotion pass through registers.
 //
-// Scale tiles: for each 128 rows and each 128-block of K the 512 bytes that tcgen05.cp takes (row r: the
-// 32-bit word at (r % 32) * 16 + (r / 32) * 4), written by the quantisation kernels, 3% of the codes' bytes.
-// Gathering scale bytes from a plain [rows, blocks] tensor inside this kernel was measured and left: two
-// warps per CTA could not keep up (their loads' latency came back once per stage), 1230 against
-// 2700 TFLOP/s at 8192 x 11008 x 4096.
+// Scale tiles: for each 128 rows and each 512 of K the 512 bytes that tcgen05.cp takes (row r: the 32-bit
+// word at (r % 32) * 16 + (r / 32) * 4, byte i the scale of the i-th block of 128), written by the
+// quantisation kernels.  They come with every fourth stage.  Gathering scale bytes from a plain [rows,
+// blocks] tensor in this kernel was measured and left: two warps per CTA could not keep up (their loads'
+// latency came back once per stage), 1230 TFLOP/s at 8192 x 11008 x 4096 where the rest ran at 2290.
 //
 // What bounds it: a 128 x 256 x 128 step takes the tensor cores 512 cycles, in which one CTA alone would
 // move 48 KB into shared memory and read 48 KB from it, 192 bytes a cycle against the 128 there are.  A pair
 // halves B's share: 64 KB per CTA and step, 128 bytes a cycle.
 //
 // Tensor memory: the accumulator takes 256 columns (one 256-column tile, or two 128-column tiles in turn),
-// the scales 16 columns per stage.  With 256-column tiles the accumulator is read into registers as bf16
+// the scales 16 columns for each of four 512-deep steps in turn.  With 256-column tiles the accumulator is read into registers as bf16
 // before the tile is stored, so the MMAs of the next tile wait only for that read.
 #include <ATen/cuda/CUDAContext.h>
 #include <c10/cuda/CUDAGuard.h>
@@ -51,12 +51,14 @@ struct GemmArgs {
   long ldd;
   const __nv_bfloat16* R;  // OUT_BF16: residual, or null
   long ldr;
-  int m_blocks, n_blocks, k_iters, num_tiles;
+  int m_blocks, n_blocks, k_iters, k_quads, num_tiles;
   int vec;                 // D (and R) rows start on 16 bytes
   int* err;
 };
 
 constexpr int BM = 128, BK = 128, STAGES = 6, GROUP_M = 16;
+constexpr int SF_STEP = 4;   // stages that a scale tile serves
+constexpr int SF_SLOTS = 4;  // places in tensor memory: a slot comes round after 12 stages, the ring has 6
 constexpr uint32_t TMEM_COLS = 512, SF_COL = 256;
 
 // PAIR: each CTA of a pair holds half of B's columns
@@ -70,13 +72,12 @@ struct Smem {
   static constexpr int STG_BYTES = 8 * 2048;             // per epilogue warp: 32 rows x 64 bytes
   static constexpr int BAR_OFF = STG_OFF + STG_BYTES;
   static constexpr int TOTAL = BAR_OFF + 256 + 1024;     // + alignment slack
-  static constexpr int TX = STAGE + SF_STAGE;            // bytes that land per stage and CTA
   static_assert(TOTAL <= 232448, "shared memory per CTA");
 };
 
-// kind::mxf8f6f4: e4m3 x e4m3 -> fp32, both K-major, e8m0 scales, scale byte 0 of either operand
-__host__ __device__ constexpr uint32_t idesc_mxf8(int M, int N) {
-  return (1u << 23) | ((uint32_t)(N >> 3) << 17) | ((uint32_t)(M >> 4) << 24);
+// kind::mxf8f6f4: e4m3 x e4m3 -> fp32, both K-major, e8m0 scales, byte `sf` of either operand's scale words
+__host__ __device__ constexpr uint32_t idesc_mxf8(int M, int N, uint32_t sf) {
+  return (sf << 4) | (sf << 29) | (1u << 23) | ((uint32_t)(N >> 3) << 17) | ((uint32_t)(M >> 4) << 24);
 }
 __device__ __forceinline__ void umma_mxf8(uint32_t d, uint64_t ad, uint64_t bd, uint32_t idesc, uint32_t sfa,
                                           uint32_t sfb, uint32_t accumulate) {
@@ -258,24 +259,30 @@ __global__ void __launch_bounds__(320, 1)
             break;
           }
           uint8_t* sa = smem + stage * L::STAGE;
-          uint8_t* sf = smem + L::SF_OFF + stage * L::SF_STAGE;
           // row blocks of this CTA; a pair's CTAs both take all of B's scales, for their own tensor memory
           const int arow = mb * CTAS + cta, brow = nb * (BN / 128);
+          const bool with_sf = k % SF_STEP == 0;
+          uint8_t* sf = smem + L::SF_OFF + stage * L::SF_STAGE;
+          const int kq = k / SF_STEP;
           // a pair's bytes complete on the leader's barrier
-          if (leader) mbar_arrive_expect_tx(&full[stage], CTAS * L::TX);
+          if (leader) mbar_arrive_expect_tx(&full[stage], CTAS * (L::STAGE + (with_sf ? L::SF_STAGE : 0)));
           if constexpr (PAIR) {
             const uint32_t fb = mapa_shared(smem_u32(&full[stage]), 0);
             tma_load_2d_pair(sa, &tmA, fb, k * BK, arow * BM);
             tma_load_2d_pair(sa + L::A_BYTES, &tmB, fb, k * BK, (brow + cta) * 128);
-            tma_load_2d_pair(sf, &tmSA, fb, 0, arow * args.k_iters + k);
+            if (with_sf) {
+              tma_load_2d_pair(sf, &tmSA, fb, 0, arow * args.k_quads + kq);
 #pragma unroll
-            for (int j = 0; j < BN / 128; ++j)
-              tma_load_2d_pair(sf + 512 * (1 + j), &tmSB, fb, 0, (brow + j) * args.k_iters + k);
+              for (int j = 0; j < BN / 128; ++j)
+                tma_load_2d_pair(sf + 512 * (1 + j), &tmSB, fb, 0, (brow + j) * args.k_quads + kq);
+            }
           } else {
             tma_load_2d(sa, &tmA, &full[stage], k * BK, arow * BM);
             tma_load_2d(sa + L::A_BYTES, &tmB, &full[stage], k * BK, brow * 128);
-            tma_load_2d(sf, &tmSA, &full[stage], 0, arow * args.k_iters + k);
-            tma_load_2d(sf + 512, &tmSB, &full[stage], 0, brow * args.k_iters + k);
+            if (with_sf) {
+              tma_load_2d(sf, &tmSA, &full[stage], 0, arow * args.k_quads + kq);
+              tma_load_2d(sf + 512, &tmSB, &full[stage], 0, brow * args.k_quads + kq);
+            }
           }
           issued |= 1u << stage;
           issued_phase = (issued_phase & ~(1u << stage)) | (phase << stage);
@@ -289,11 +296,14 @@ __global__ void __launch_bounds__(320, 1)
           if (issued >> s & 1) mbar_wait(&full[s], issued_phase >> s & 1, args.err);
     }
   } else if (warp == 1) {
-    if (lane == 0 && leader) {
-      int stage = 0, t = 0;
+    // the whole warp walks the stages, so that descriptors and addresses stay warp-uniform; one lane issues
+    if (leader) {
+      int stage = 0, t = 0, slot = SF_SLOTS - 1;
       uint32_t phase = 0;
       bool ok = true;
-      constexpr uint32_t IDESC = idesc_mxf8(TILE_M, BN);
+      // descriptors of the ring's first stage; a stage or a 32-byte step only adds to the address field
+      const uint64_t ad0 = sdesc_sw128(smem_u32(smem), 16, 1024), bd0 = sdesc_sw128(smem_u32(smem) + L::A_BYTES, 16, 1024);
+      const uint32_t sf0 = smem_u32(smem + L::SF_OFF);
       for (int tile = unit; tile < args.num_tiles && ok; tile += units, ++t) {
         const int acc = t % ACCS;
         const uint32_t acc_phase = (t / ACCS) & 1;
@@ -309,24 +319,34 @@ __global__ void __launch_bounds__(320, 1)
             break;
           }
           tc_fence_after();
-          const uint32_t a0 = smem_u32(smem + stage * L::STAGE), b0 = a0 + L::A_BYTES;
-          const uint32_t sf = smem_u32(smem + L::SF_OFF + stage * L::SF_STAGE);
-          const uint32_t sfa = tmem + SF_COL + stage * 16, sfb = sfa + 4;
-          tmem_copy_scales<PAIR>(sfa, sf);
+          const uint32_t sub = k % SF_STEP;
+          if (sub == 0) slot = (slot + 1) % SF_SLOTS;
+          const uint32_t sfa = tmem + SF_COL + slot * 16, sfb = sfa + 4;
+          const uint64_t ad = ad0 + stage * (L::STAGE >> 4), bd = bd0 + stage * (L::STAGE >> 4);
+          const uint32_t idesc = idesc_mxf8(TILE_M, BN, 0) | (sub << 4) | (sub << 29);
+          if (lane == 0) {
+            if (sub == 0) {
+              const uint32_t sf = sf0 + stage * L::SF_STAGE;
+              tmem_copy_scales<PAIR>(sfa, sf);
 #pragma unroll
-          for (int j = 0; j < BN / 128; ++j) tmem_copy_scales<PAIR>(sfb + 4 * j, sf + 512 * (1 + j));
+              for (int j = 0; j < BN / 128; ++j) tmem_copy_scales<PAIR>(sfb + 4 * j, sf + 512 * (1 + j));
+            }
 #pragma unroll
-          for (int kk = 0; kk < BK / 32; ++kk) {
-            const uint64_t ad = sdesc_sw128(a0 + kk * 32, 16, 1024), bd = sdesc_sw128(b0 + kk * 32, 16, 1024);
-            if constexpr (PAIR) umma_mxf8_pair(tmem + acc * BN, ad, bd, IDESC, sfa, sfb, k != 0 || kk != 0);
-            else umma_mxf8(tmem + acc * BN, ad, bd, IDESC, sfa, sfb, k != 0 || kk != 0);
+            for (int kk = 0; kk < BK / 32; ++kk) {
+              if constexpr (PAIR) umma_mxf8_pair(tmem + acc * BN, ad + 2 * kk, bd + 2 * kk, idesc, sfa, sfb, k != 0 || kk != 0);
+              else umma_mxf8(tmem + acc * BN, ad + 2 * kk, bd + 2 * kk, idesc, sfa, sfb, k != 0 || kk != 0);
+            }
+            if constexpr (PAIR) umma_commit_pair(&empty[stage]);
+            else umma_commit(&empty[stage]);
           }
-          if constexpr (PAIR) umma_commit_pair(&empty[stage]);
-          else umma_commit(&empty[stage]);
+          __syncwarp();
           if (++stage == STAGES) stage = 0, phase ^= 1;
         }
-        if constexpr (PAIR) umma_commit_pair(&acc_full[acc]);
-        else umma_commit(&acc_full[acc]);
+        if (lane == 0) {
+          if constexpr (PAIR) umma_commit_pair(&acc_full[acc]);
+          else umma_commit(&acc_full[acc]);
+        }
+        __syncwarp();
       }
     }
   } else {
@@ -414,13 +434,16 @@ __global__ void __launch_bounds__(320, 1)
 }
 
 // Scale tiles of a plain e8m0 scale tensor [row groups, k blocks] (strides in bytes): one block of 128
-// threads per tile, thread r its row.
+// threads per tile, thread r its row.  Blocks past K get scale 1.
 __global__ void __launch_bounds__(128) scale_tiles_kernel(const uint8_t* __restrict__ s, long row_stride, long blk_stride,
-                                                          int gran, int rows, int kb, uint32_t* __restrict__ tiles) {
-  const int mt = blockIdx.x / kb, k = blockIdx.x % kb, r = threadIdx.x;
+                                                          int gran, int rows, int kb, int kq, uint32_t* __restrict__ tiles) {
+  const int mt = blockIdx.x / kq, k = blockIdx.x % kq * SF_STEP, r = threadIdx.x;
   const int row = min(mt * 128 + r, rows - 1);
-  const uint32_t b = s[(long)(gran == 1 ? row : mt) * row_stride + k * blk_stride];
-  tiles[(long)blockIdx.x * 128 + (r & 31) * 4 + (r >> 5)] = b * 0x01010101u;
+  const uint8_t* p = s + (long)(gran == 1 ? row : mt) * row_stride + k * blk_stride;
+  uint32_t w = 0;
+#pragma unroll
+  for (int i = 0; i < SF_STEP; ++i) w |= (k + i < kb ? (uint32_t)p[i * blk_stride] : 127u) << (8 * i);
+  tiles[(long)blockIdx.x * 128 + (r & 31) * 4 + (r >> 5)] = w;
 }
 
 // ---------------------------------------------------------------- host side
@@ -460,7 +483,7 @@ static CUtensorMap code_map(const torch::Tensor& t) {
   return make_map(CU_TENSOR_MAP_DATA_TYPE_UINT8, CU_TENSOR_MAP_SWIZZLE_128B, t.data_ptr(), k, rows,
                   rows > 1 ? t.stride(0) : (k + 15) / 16 * 16, 128, 128);
 }
-// scale tiles [row blocks, k blocks, 512 bytes]: one tile per box
+// scale tiles [row blocks, k blocks / 4, 512 bytes]: one tile per box
 static CUtensorMap tile_map(const torch::Tensor& t) {
   return make_map(CU_TENSOR_MAP_DATA_TYPE_UINT32, CU_TENSOR_MAP_SWIZZLE_NONE, t.data_ptr(), 128, t.size(0) * t.size(1),
                   512, 128, 1);
@@ -496,7 +519,7 @@ static void launch(const CUtensorMap* t, GemmArgs& g, cudaStream_t st) {
 using namespace dtb;
 
 // D [M, N] = A [M, K] B [N, K]^T (+ R): D bf16 (R bf16, optional) or fp32 (accumulate: D += the product).
-// tA, tB: the operands' scale tiles, uint8 [ceil(rows / 128), ceil(K / 128), 512].
+// tA, tB: the operands' scale tiles, uint8 [ceil(rows / 128), ceil(K / 512), 512].
 void fp8_gemm(torch::Tensor A, torch::Tensor tA, torch::Tensor B, torch::Tensor tB, torch::Tensor D,
               c10::optional<torch::Tensor> R, bool accumulate) {
   for (const torch::Tensor* t : {&A, &B})
@@ -514,7 +537,7 @@ void fp8_gemm(torch::Tensor A, torch::Tensor tA, torch::Tensor B, torch::Tensor 
   const torch::Tensor* q[2] = {&A, &B};
   const torch::Tensor* t[2] = {&tA, &tB};
   for (int i = 0; i < 2; ++i)
-    DTB_CHECK(t[i]->device() == A.device() && t[i]->scalar_type() == at::kByte && t[i]->is_contiguous() && t[i]->dim() == 3 && t[i]->size(0) == (q[i]->size(0) + 127) / 128 && t[i]->size(1) == (K + 127) / 128 && t[i]->size(2) == 512 && t[i]->size(0) * t[i]->size(1) < (1L << 31) && (reinterpret_cast<uintptr_t>(t[i]->data_ptr()) & 15) == 0, "fp8_gemm: scale tiles must be contiguous uint8 [ceil(rows / 128), ceil(K / 128), 512]");
+    DTB_CHECK(t[i]->device() == A.device() && t[i]->scalar_type() == at::kByte && t[i]->is_contiguous() && t[i]->dim() == 3 && t[i]->size(0) == (q[i]->size(0) + 127) / 128 && t[i]->size(1) == (K + 511) / 512 && t[i]->size(2) == 512 && t[i]->size(0) * t[i]->size(1) < (1L << 31) && (reinterpret_cast<uintptr_t>(t[i]->data_ptr()) & 15) == 0, "fp8_gemm: scale tiles must be contiguous uint8 [ceil(rows / 128), ceil(K / 512), 512]");
   g.D = D.data_ptr();
   g.ldd = M > 1 ? D.stride(0) : N;
   g.err = dtb_error_word();
@@ -532,6 +555,7 @@ void fp8_gemm(torch::Tensor A, torch::Tensor tA, torch::Tensor B, torch::Tensor 
     else if (!accumulate) D.zero_();
     return;
   }
+  g.k_quads = (g.K + 511) / 512;
   g.k_iters = (g.K + fp8::BK - 1) / fp8::BK;
   auto st = at::cuda::getCurrentCUDAStream();
   const CUtensorMap maps[4] = {fp8::code_map(A), fp8::code_map(B), fp8::tile_map(tA), fp8::tile_map(tB)};
@@ -547,12 +571,12 @@ void fp8_gemm(torch::Tensor A, torch::Tensor tA, torch::Tensor B, torch::Tensor 
 torch::Tensor fp8_scale_tiles(torch::Tensor s, int64_t gran, int64_t rows) {
   DTB_CHECK(s.is_cuda() && s.scalar_type() == at::kFloat8_e8m0fnu && s.dim() == 2 && (gran == 1 || gran == 128) && rows >= 0 && rows < (1L << 30) && s.size(0) == (rows + gran - 1) / gran, "fp8_scale_tiles: e8m0 scales of 1 x 128 or 128 x 128 blocks");
   const c10::cuda::CUDAGuard guard(s.device());
-  const long mt = (rows + 127) / 128, kb = s.size(1);
-  DTB_CHECK(mt * kb < (1L << 31), "fp8_scale_tiles: too large");
-  auto t = torch::empty({mt, kb, 512}, s.options().dtype(at::kByte));
-  if (mt * kb == 0) return t;
-  fp8::scale_tiles_kernel<<<(unsigned)(mt * kb), 128, 0, at::cuda::getCurrentCUDAStream()>>>(
-      reinterpret_cast<const uint8_t*>(s.data_ptr()), s.stride(0), s.stride(1), (int)gran, (int)rows, (int)kb,
+  const long mt = (rows + 127) / 128, kb = s.size(1), kq = (kb + fp8::SF_STEP - 1) / fp8::SF_STEP;
+  DTB_CHECK(mt * kq < (1L << 31), "fp8_scale_tiles: too large");
+  auto t = torch::empty({mt, kq, 512}, s.options().dtype(at::kByte));
+  if (mt * kq == 0) return t;
+  fp8::scale_tiles_kernel<<<(unsigned)(mt * kq), 128, 0, at::cuda::getCurrentCUDAStream()>>>(
+      reinterpret_cast<const uint8_t*>(s.data_ptr()), s.stride(0), s.stride(1), (int)gran, (int)rows, (int)kb, (int)kq,
       reinterpret_cast<uint32_t*>(t.data_ptr()));
   DTB_LAUNCH_CHECK();
   return t;

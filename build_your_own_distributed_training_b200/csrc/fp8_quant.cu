@@ -60,13 +60,14 @@ struct QuantArgs {
   uint8_t* qt;        // [C, qt_ld] transposed codes, or null
   long qt_ld;
   uint8_t* st;        // 1 x 128 of the transpose: [R / 128][C]
-  uint32_t* t;        // scale tiles of the codes as they lie: [R / 128][C / 128][128]
-  uint32_t* tt;       // and of the transpose: [C / 128][R / 128][128]
+  uint8_t* t;         // scale tiles of the codes as they lie: [R / 128][C / 512][512]
+  uint8_t* tt;        // and of the transpose: [C / 128][R / 512][512]
 };
 
-// word of row r (0..127) in a scale tile, and its value
-__device__ __forceinline__ int tile_word(int r) { return (r & 31) * 4 + (r >> 5); }
-__device__ __forceinline__ uint32_t tile_value(uint32_t byte) { return byte * 0x01010101u; }
+// Byte of (row r of 128, k block `kb`) from the start of its row block's scale tiles.
+__device__ __forceinline__ long tile_byte(int r, long kb) {
+  return (kb >> 2) * 512 + (r & 31) * 16 + (r >> 5) * 4 + (kb & 3);
+}
 
 // One 128 x 128 tile per block of 256 threads: thread (rg, cg) holds rows rg * 8 + i, columns cg * 8 + k.
 template <typename T, bool SQUARE, bool WIDE>
@@ -75,6 +76,7 @@ __global__ void __launch_bounds__(256) quant_tile_kernel(const QuantArgs a) {
   __shared__ uint32_t colmax[8][128];
   const int tid = threadIdx.x, cg = tid & 15, rg = tid >> 4, warp = tid >> 5, lane = tid & 31;
   const int r0 = blockIdx.y * 128 + rg * 8, c0 = blockIdx.x * 128 + cg * 8;
+  const long tq = (gridDim.x + 3) >> 2, ttq = (gridDim.y + 3) >> 2;  // scale tiles per row block
   const T* x = reinterpret_cast<const T*>(a.x);
   Pack<T, 8> v[8];
 #pragma unroll
@@ -110,11 +112,10 @@ __global__ void __launch_bounds__(256) quant_tile_kernel(const QuantArgs a) {
     for (int w = 0; w < 8; ++w) m = max(m, colmax[0][w]);
 #pragma unroll
     for (int i = 0; i < 8; ++i) rmax[i] = m;
-    const uint32_t b = scale_byte(m);
-    const long at = (long)blockIdx.y * gridDim.x + blockIdx.x, att = (long)blockIdx.x * gridDim.y + blockIdx.y;
-    if (tid == 0) a.s[at] = (uint8_t)b;
-    if (tid < 128 && a.t != nullptr) a.t[at * 128 + tid] = tile_value(b);
-    if (tid >= 128 && a.tt != nullptr) a.tt[att * 128 + tid - 128] = tile_value(b);
+    const uint8_t b = (uint8_t)scale_byte(m);
+    if (tid == 0) a.s[(long)blockIdx.y * gridDim.x + blockIdx.x] = b;
+    if (tid < 128 && a.t != nullptr) a.t[blockIdx.y * tq * 512 + tile_byte(tid, blockIdx.x)] = b;
+    if (tid >= 128 && a.tt != nullptr) a.tt[blockIdx.x * ttq * 512 + tile_byte(tid - 128, blockIdx.y)] = b;
   } else if (a.q != nullptr) {
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
@@ -123,7 +124,7 @@ __global__ void __launch_bounds__(256) quant_tile_kernel(const QuantArgs a) {
       if (cg == i) {
         const uint32_t b = scale_byte(rmax[i]);
         if (r0 + i < a.R) a.s[(long)blockIdx.x * a.R + r0 + i] = (uint8_t)b;
-        a.t[((long)blockIdx.y * gridDim.x + blockIdx.x) * 128 + tile_word(rg * 8 + i)] = tile_value(b);
+        a.t[blockIdx.y * tq * 512 + tile_byte(rg * 8 + i, blockIdx.x)] = (uint8_t)b;
       }
     }
   }
@@ -160,7 +161,7 @@ __global__ void __launch_bounds__(256) quant_tile_kernel(const QuantArgs a) {
       f[k] = inv_scale(b);
       if (rg == k) {
         if (c0 + k < a.C) a.st[(long)blockIdx.y * a.C + c0 + k] = (uint8_t)b;
-        a.tt[((long)blockIdx.x * gridDim.y + blockIdx.y) * 128 + tile_word(cg * 8 + k)] = tile_value(b);
+        a.tt[blockIdx.x * ttq * 512 + tile_byte(cg * 8 + k, blockIdx.y)] = (uint8_t)b;
       }
     }
   }
@@ -212,7 +213,7 @@ __global__ void __launch_bounds__(256) quant_rows_kernel(const QuantArgs a) {
   const uint32_t b = scale_byte(m);
   if (cg == 0) {
     a.s[(long)blk * a.R + row] = (uint8_t)b;
-    a.t[((row >> 7) * cb + blk) * 128 + tile_word((int)(row & 127))] = tile_value(b);
+    a.t[(row >> 7) * ((cb + 3) >> 2) * 512 + tile_byte((int)(row & 127), blk)] = (uint8_t)b;
   }
   const float f = inv_scale(b);
   uint2 o;
@@ -241,7 +242,7 @@ std::vector<torch::Tensor> fp8_quantize(torch::Tensor x, bool square, bool plain
     return torch::empty({rows, pitch}, x.options().dtype(at::kFloat8_e4m3fn)).narrow(1, 0, cols);
   };
   auto opts = x.options().dtype(at::kFloat8_e8m0fnu);
-  auto tiles = [&](long rb, long cb) { return torch::empty({rb, cb, 512}, x.options().dtype(at::kByte)); };
+  auto tiles = [&](long rb, long cb) { return torch::empty({rb, (cb + 3) / 4, 512}, x.options().dtype(at::kByte)); };
   torch::Tensor q, s, t, qt, st, tt;
   if (plain) t = tiles(RB, CB);
   if (transposed) tt = tiles(CB, RB);
@@ -264,8 +265,8 @@ std::vector<torch::Tensor> fp8_quantize(torch::Tensor x, bool square, bool plain
     a.q = reinterpret_cast<uint8_t*>(q.data_ptr());
     a.q_ld = (C + 15) / 16 * 16;
   }
-  if (plain) a.t = reinterpret_cast<uint32_t*>(t.data_ptr());
-  if (transposed) a.tt = reinterpret_cast<uint32_t*>(tt.data_ptr());
+  if (plain) a.t = t.data_ptr<uint8_t>();
+  if (transposed) a.tt = tt.data_ptr<uint8_t>();
   if (square || plain) a.s = reinterpret_cast<uint8_t*>(s.data_ptr());
   if (transposed) {
     a.qt = reinterpret_cast<uint8_t*>(qt.data_ptr());
