@@ -110,6 +110,44 @@ __device__ __forceinline__ void tmem_copy_scales(uint32_t taddr, uint32_t saddr)
     asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(desc) : "memory");
 }
 
+// The issuing warps run their loops with all 32 lanes and let one elected lane issue, so that addresses,
+// descriptors and branches stay warp-uniform: with a single-lane loop an MMA took 95 cycles to issue and a
+// stage's bookkeeping 400, more than the tensor cores need for the stage.
+__device__ __forceinline__ bool elect_one() {
+  uint32_t p;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "elect.sync _|p, 0xffffffff;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(p));
+  return p != 0;
+}
+// mbar_wait for a whole warp: the same answer in every lane, false after 2 s (error word set)
+__device__ __forceinline__ bool warp_wait(uint32_t bar, uint32_t parity, int* err) {
+  uint32_t ok;
+  asm volatile(
+      "{\n\t.reg .pred p, q;\n\t.reg .u64 t, u;\n\t"
+      "mov.u32 %0, 1;\n\t"
+      "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+      "@p bra DONE;\n\t"
+      "mov.u64 t, %%globaltimer;\n\t"
+      "AGAIN:\n\t"
+      "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+      "@p bra DONE;\n\t"
+      "mov.u64 u, %%globaltimer;\n\t"
+      "sub.u64 u, u, t;\n\t"
+      "setp.lt.u64 q, u, 2000000000;\n\t"
+      "@q bra AGAIN;\n\t"
+      "mov.u32 %0, 0;\n\t"
+      "DONE:\n\t}"
+      : "=&r"(ok)
+      : "r"(bar), "r"(parity)
+      : "memory");
+  if (__all_sync(0xffffffffu, ok != 0)) return true;
+  if (err) atomicExch(err, ERR_MBAR_TIMEOUT);
+  return false;
+}
+
 __device__ __forceinline__ void tile_coords(int tile, int mblocks, int nblocks, int& mb, int& nb) {
   const int per_group = GROUP_M * nblocks;
   const int g = tile / per_group, first = g * GROUP_M;
@@ -205,7 +243,6 @@ __global__ void __launch_bounds__(320, 1)
   uint64_t* acc_full = empty + STAGES;
   uint64_t* acc_empty = acc_full + 2;
   uint32_t* tmem_holder = reinterpret_cast<uint32_t*>(acc_empty + 2);
-  volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_holder + 1);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int cta = PAIR ? (int)cluster_ctarank() : 0;
   const bool leader = cta == 0;
@@ -220,7 +257,6 @@ __global__ void __launch_bounds__(320, 1)
       mbar_init(&acc_full[i], 1);
       mbar_init(&acc_empty[i], 8 * CTAS);
     }
-    *abort_flag = 0;
     if constexpr (PAIR) fence_mbar_init_cluster();
     else fence_mbar_init();
     tma_prefetch_desc(&tmA);
@@ -241,62 +277,64 @@ __global__ void __launch_bounds__(320, 1)
   __syncthreads();
   if constexpr (PAIR) cluster_sync();  // the peer's barriers exist before any remote arrive
   tc_fence_after();
-  const uint32_t tmem = *tmem_holder;
+  // all 512 columns are allocated, so the allocation starts at column 0: a constant base keeps the
+  // addresses below warp-uniform
+  if (*tmem_holder != 0 && threadIdx.x == 0) atomicExch(args.err, ERR_BAD_ARG);
+  constexpr uint32_t tmem = 0;
 
   if (warp == 0) {
-    if (lane == 0) {
-      int stage = 0;
-      uint32_t phase = 0;
-      uint32_t issued = 0, issued_phase = 0;  // bit per stage
-      bool ok = true;
-      for (int tile = unit; tile < args.num_tiles && ok; tile += units) {
-        int mb, nb;
-        tile_coords(tile, args.m_blocks, args.n_blocks, mb, nb);
-        for (int k = 0; k < args.k_iters; ++k) {
-          if (*abort_flag || !mbar_wait(&empty[stage], phase ^ 1, args.err)) {
-            *abort_flag = 1;
-            ok = false;
-            break;
-          }
-          uint8_t* sa = smem + stage * L::STAGE;
-          // row blocks of this CTA; a pair's CTAs both take all of B's scales, for their own tensor memory
-          const int arow = mb * CTAS + cta, brow = nb * (BN / 128);
-          const bool with_sf = k % SF_STEP == 0;
-          uint8_t* sf = smem + L::SF_OFF + stage * L::SF_STAGE;
-          const int kq = k / SF_STEP;
-          // a pair's bytes complete on the leader's barrier
+    int stage = 0;
+    uint32_t phase = 0, issued = 0, issued_phase = 0;  // a bit per stage
+    bool ok = true;
+    for (int tile = unit; tile < args.num_tiles && ok; tile += units) {
+      int mb, nb;
+      tile_coords(tile, args.m_blocks, args.n_blocks, mb, nb);
+      // row blocks of this CTA; a pair's CTAs both take all of B's scales, for their own tensor memory
+      const int arow = mb * CTAS + cta, brow = nb * (BN / 128);
+      int sa_tile = arow * args.k_quads, sb_tile = brow * args.k_quads;
+      for (int k = 0; k < args.k_iters; ++k) {
+        if (!warp_wait(smem_u32(&empty[stage]), phase ^ 1, args.err)) {
+          ok = false;
+          break;
+        }
+        uint8_t* sa = smem + stage * L::STAGE;
+        uint8_t* sf = smem + L::SF_OFF + stage * L::SF_STAGE;
+        const bool with_sf = k % SF_STEP == 0;
+        // a pair's bytes complete on the leader's barrier
+        const uint32_t fb = PAIR ? mapa_shared(smem_u32(&full[stage]), 0) : 0;
+        if (elect_one()) {
           if (leader) mbar_arrive_expect_tx(&full[stage], CTAS * (L::STAGE + (with_sf ? L::SF_STAGE : 0)));
           if constexpr (PAIR) {
-            const uint32_t fb = mapa_shared(smem_u32(&full[stage]), 0);
             tma_load_2d_pair(sa, &tmA, fb, k * BK, arow * BM);
             tma_load_2d_pair(sa + L::A_BYTES, &tmB, fb, k * BK, (brow + cta) * 128);
             if (with_sf) {
-              tma_load_2d_pair(sf, &tmSA, fb, 0, arow * args.k_quads + kq);
+              tma_load_2d_pair(sf, &tmSA, fb, 0, sa_tile);
 #pragma unroll
               for (int j = 0; j < BN / 128; ++j)
-                tma_load_2d_pair(sf + 512 * (1 + j), &tmSB, fb, 0, (brow + j) * args.k_quads + kq);
+                tma_load_2d_pair(sf + 512 * (1 + j), &tmSB, fb, 0, sb_tile + j * args.k_quads);
             }
           } else {
             tma_load_2d(sa, &tmA, &full[stage], k * BK, arow * BM);
             tma_load_2d(sa + L::A_BYTES, &tmB, &full[stage], k * BK, brow * 128);
             if (with_sf) {
-              tma_load_2d(sf, &tmSA, &full[stage], 0, arow * args.k_quads + kq);
-              tma_load_2d(sf + 512, &tmSB, &full[stage], 0, brow * args.k_quads + kq);
+              tma_load_2d(sf, &tmSA, &full[stage], 0, sa_tile);
+              tma_load_2d(sf + 512, &tmSB, &full[stage], 0, sb_tile);
             }
           }
-          issued |= 1u << stage;
-          issued_phase = (issued_phase & ~(1u << stage)) | (phase << stage);
-          if (++stage == STAGES) stage = 0, phase ^= 1;
         }
+        __syncwarp();
+        if (with_sf) ++sa_tile, ++sb_tile;
+        issued |= 1u << stage;
+        issued_phase = (issued_phase & ~(1u << stage)) | (phase << stage);
+        if (++stage == STAGES) stage = 0, phase ^= 1;
       }
-      // copies in flight land before the shared memory goes away (a pair's follower has no barrier of its
-      // own for them: its bounded waits outlast its last copy by far)
-      if (!ok && leader)
-        for (int s = 0; s < STAGES; ++s)
-          if (issued >> s & 1) mbar_wait(&full[s], issued_phase >> s & 1, args.err);
     }
+    // copies in flight land before the shared memory goes away (a pair's follower has no barrier of its own
+    // for them: its bounded waits outlast its last copy by far)
+    if (!ok && leader)
+      for (int s = 0; s < STAGES; ++s)
+        if (issued >> s & 1) warp_wait(smem_u32(&full[s]), issued_phase >> s & 1, args.err);
   } else if (warp == 1) {
-    // the whole warp walks the stages, so that descriptors and addresses stay warp-uniform; one lane issues
     if (leader) {
       int stage = 0, t = 0, slot = SF_SLOTS - 1;
       uint32_t phase = 0;
@@ -307,14 +345,10 @@ __global__ void __launch_bounds__(320, 1)
       for (int tile = unit; tile < args.num_tiles && ok; tile += units, ++t) {
         const int acc = t % ACCS;
         const uint32_t acc_phase = (t / ACCS) & 1;
-        if (*abort_flag || !mbar_wait(&acc_empty[acc], acc_phase ^ 1, args.err)) {
-          *abort_flag = 1;
-          break;
-        }
+        if (!warp_wait(smem_u32(&acc_empty[acc]), acc_phase ^ 1, args.err)) break;
         tc_fence_after();
         for (int k = 0; k < args.k_iters; ++k) {
-          if (*abort_flag || !mbar_wait(&full[stage], phase, args.err)) {
-            *abort_flag = 1;
+          if (!warp_wait(smem_u32(&full[stage]), phase, args.err)) {
             ok = false;
             break;
           }
@@ -324,7 +358,7 @@ __global__ void __launch_bounds__(320, 1)
           const uint32_t sfa = tmem + SF_COL + slot * 16, sfb = sfa + 4;
           const uint64_t ad = ad0 + stage * (L::STAGE >> 4), bd = bd0 + stage * (L::STAGE >> 4);
           const uint32_t idesc = idesc_mxf8(TILE_M, BN, 0) | (sub << 4) | (sub << 29);
-          if (lane == 0) {
+          if (elect_one()) {
             if (sub == 0) {
               const uint32_t sf = sf0 + stage * L::SF_STAGE;
               tmem_copy_scales<PAIR>(sfa, sf);
@@ -342,7 +376,7 @@ __global__ void __launch_bounds__(320, 1)
           __syncwarp();
           if (++stage == STAGES) stage = 0, phase ^= 1;
         }
-        if (lane == 0) {
+        if (elect_one()) {
           if constexpr (PAIR) umma_commit_pair(&acc_full[acc]);
           else umma_commit(&acc_full[acc]);
         }
@@ -359,10 +393,7 @@ __global__ void __launch_bounds__(320, 1)
       const uint32_t acc_phase = (t / ACCS) & 1;
       int mb, nb;
       tile_coords(tile, args.m_blocks, args.n_blocks, mb, nb);
-      if (*abort_flag || !mbar_wait(&acc_full[acc], acc_phase, args.err)) {
-        *abort_flag = 1;
-        break;
-      }
+      if (!warp_wait(smem_u32(&acc_full[acc]), acc_phase, args.err)) break;
       tc_fence_after();
       const uint32_t tb = tmem + ((uint32_t)(quad * 32) << 16) + acc * BN + half * COLS;
       const int row0 = mb * TILE_M + cta * BM + quad * 32, col0 = nb * BN + half * COLS;
