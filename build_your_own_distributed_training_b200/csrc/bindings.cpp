@@ -79,6 +79,10 @@ std::vector<torch::Tensor> fp8_quantize(torch::Tensor x, bool square, bool plain
 void fp8_gemm(torch::Tensor A, torch::Tensor tA, torch::Tensor B, torch::Tensor tB, torch::Tensor D,
               c10::optional<torch::Tensor> R, bool accumulate);
 torch::Tensor fp8_scale_tiles(torch::Tensor s, int64_t gran, int64_t rows);
+void fp8_product(torch::Tensor A, torch::Tensor sA, c10::optional<torch::Tensor> tA, torch::Tensor B, torch::Tensor sB,
+                 c10::optional<torch::Tensor> tB, torch::Tensor D, c10::optional<torch::Tensor> R, bool accumulate);
+torch::Tensor linear_fp8_kept(torch::Tensor x, torch::Tensor values, torch::Tensor scales,
+                              c10::optional<torch::Tensor> tiles, c10::optional<torch::Tensor> residual);
 torch::Tensor qk_norm_rope_autograd(torch::Tensor x, torch::Tensor wq, torch::Tensor wk, torch::Tensor cos_t,
                                     torch::Tensor sin_t, c10::optional<torch::Tensor> pos, int64_t nq, int64_t nkv,
                                     int64_t hd, int64_t seqlen, double eps);
@@ -143,6 +147,8 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("token_logprobs_bwd", &token_logprobs_bwd);
   m.def("fp8_quantize", &fp8_quantize, "e4m3 codes with a power-of-two scale per block of 128, as they lie and / or transposed");
   m.def("fp8_scale_tiles", &fp8_scale_tiles, "scale tiles for fp8_gemm from plain e8m0 scales");
+  m.def("fp8_product", &fp8_product, "product of e4m3 operands by the kernel that fits their number of rows");
+  m.def("linear_fp8_kept", &linear_fp8_kept, "8-bit linear layer with kept 8-bit weights");
   m.def("fp8_gemm", &fp8_gemm, "tcgen05 block-scaled product of e4m3 operands");
   m.def("swiglu_fwd", &swiglu_fwd, "silu(g) * u of packed [g | u]");
   m.def("qk_norm_rope", &qk_norm_rope_autograd, "qk_norm_rope_fwd as an autograd node");

@@ -19,7 +19,8 @@ std::vector<Tensor> token_logprobs_fwd(Tensor x, Tensor tokens, double temperatu
 void token_logprobs_bwd(Tensor x, Tensor tokens, Tensor state, c10::optional<Tensor> g_lp, c10::optional<Tensor> g_ent,
                         double temperature, Tensor dx);
 std::vector<Tensor> fp8_quantize(Tensor x, bool square, bool plain, bool transposed);
-void fp8_gemm(Tensor A, Tensor tA, Tensor B, Tensor tB, Tensor D, c10::optional<Tensor> R, bool accumulate);
+void fp8_product(Tensor A, Tensor sA, c10::optional<Tensor> tA, Tensor B, Tensor sB, c10::optional<Tensor> tB, Tensor D,
+                 c10::optional<Tensor> R, bool accumulate);
 
 namespace {
 
@@ -94,8 +95,8 @@ struct LinearFp8 : public Function<LinearFp8> {
     auto xq = fp8_quantize(x, false, true, need_w);  // codes, scales, tiles; of the transpose: 3, 4, 5
     auto wq = fp8_quantize(w, true, true, need_x);
     Tensor y = torch::empty({x.size(0), w.size(0)}, x.options());
-    fp8_gemm(xq[0], xq[2], wq[0], wq[2], y, residual, false);
-    ctx->save_for_backward({xq[3], xq[5], wq[3], wq[5]});
+    fp8_product(xq[0], xq[1], xq[2], wq[0], wq[1], wq[2], y, residual, false);
+    ctx->save_for_backward({xq[3], xq[4], xq[5], wq[3], wq[4], wq[5]});
     ctx->saved_data["t"] = w.scalar_type();
     ctx->saved_data["r"] = residual.has_value();
     return y;
@@ -108,13 +109,13 @@ struct LinearFp8 : public Function<LinearFp8> {
       Tensor g = grads[0].contiguous();
       auto gq = fp8_quantize(g, false, need_x, need_w);
       if (need_x) {
-        dx = torch::empty({g.size(0), s[2].size(0)}, g.options());
-        fp8_gemm(gq[0], gq[2], s[2], s[3], dx, c10::nullopt, false);
+        dx = torch::empty({g.size(0), s[3].size(0)}, g.options());
+        fp8_product(gq[0], gq[1], gq[2], s[3], s[4], s[5], dx, c10::nullopt, false);
       }
       if (need_w) {
         const auto t = ctx->saved_data["t"].toScalarType();
         dw = torch::empty({g.size(1), s[0].size(0)}, g.options().dtype(t == at::kHalf ? at::kFloat : t));
-        fp8_gemm(gq[3], gq[5], s[0], s[1], dw, c10::nullopt, false);
+        fp8_product(gq[3], gq[4], gq[5], s[0], s[1], s[2], dw, c10::nullopt, false);
         dw = dw.to(t);
       }
     }
@@ -137,4 +138,13 @@ std::vector<Tensor> token_logprobs_autograd(Tensor x, Tensor tokens, double temp
 // x [T, K] bf16, w [N, K], residual [T, N] bf16 or none
 Tensor linear_fp8_autograd(Tensor x, Tensor w, c10::optional<Tensor> residual) {
   return LinearFp8::apply(x, w, residual);
+}
+
+// x [T, K] bf16 with weights kept in 8 bits: values [N, K] e4m3, scales e8m0, their tiles or none
+Tensor linear_fp8_kept(Tensor x, Tensor values, Tensor scales, c10::optional<Tensor> tiles,
+                       c10::optional<Tensor> residual) {
+  auto xq = fp8_quantize(x, false, true, false);
+  Tensor y = torch::empty({x.size(0), values.size(0)}, x.options());
+  fp8_product(xq[0], xq[1], xq[2], values, scales, tiles, y, residual, false);
+  return y;
 }

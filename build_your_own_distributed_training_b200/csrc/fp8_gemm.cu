@@ -28,8 +28,8 @@
 // halves B's share: 64 KB per CTA and step, 128 bytes a cycle.
 //
 // Tensor memory: the accumulator takes 256 columns (one 256-column tile, or two 128-column tiles in turn),
-// the scales 16 columns for each of four 512-deep steps in turn.  With 256-column tiles the accumulator is read into registers as bf16
-// before the tile is stored, so the MMAs of the next tile wait only for that read.
+// the scales 16 columns for each of eight 512-deep steps in turn.  The accumulator is read into registers
+// before the tile is stored, so with 256-column tiles the MMAs of the next tile wait only for that read.
 #include <ATen/cuda/CUDAContext.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <cudaTypedefs.h>
@@ -52,13 +52,15 @@ struct GemmArgs {
   const __nv_bfloat16* R;  // OUT_BF16: residual, or null
   long ldr;
   int m_blocks, n_blocks, k_iters, k_quads, num_tiles;
+  int splits, k_per;       // K in `splits` parts of k_per blocks (a multiple of SF_STEP); part p writes D + p * M * ldd
   int vec;                 // D (and R) rows start on 16 bytes
   int* err;
 };
 
 constexpr int BM = 128, BK = 128, STAGES = 6, GROUP_M = 16;
 constexpr int SF_STEP = 4;   // stages that a scale tile serves
-constexpr int SF_SLOTS = 4;  // places in tensor memory: a slot comes round after 12 stages, the ring has 6
+constexpr int SF_SLOTS = 8;  // places in tensor memory: a slot comes round after 8 stages at least, when the MMAs
+                             // of the ring's 6 earlier ones have been waited for
 constexpr uint32_t TMEM_COLS = 512, SF_COL = 256;
 
 // PAIR: each CTA of a pair holds half of B's columns
@@ -160,44 +162,42 @@ __device__ __forceinline__ void tile_coords(int tile, int mblocks, int nblocks, 
 // 32 rows x 64 bytes staged by the warp (16-byte chunks swizzled by the row) -> global rows
 __device__ __forceinline__ uint32_t stg_off(int row, int chunk) { return row * 64 + ((chunk ^ ((row >> 1) & 3)) << 4); }
 
+// Vector stores: lane covers rows lane / 4 + 8 i, 16-byte chunk lane % 4, eight 64-byte row pieces per
+// access.  Rows that do not start on 16 bytes: an element per lane, consecutive lanes on consecutive columns.
 template <int OUT>
-__device__ __forceinline__ void store_segment(const GemmArgs& a, uint8_t* stg, int row0, int col, int lane) {
-  // lane covers rows lane / 4 + 8 i, 16-byte chunk lane % 4: eight 64-byte row pieces per access
-  constexpr int ES = OUT == OUT_BF16 ? 2 : 4, PER = 16 / ES;
+__device__ __forceinline__ void store_segment(const GemmArgs& a, uint8_t* stg, int row0, int col, int part_row, int lane) {
+  constexpr int ES = OUT == OUT_BF16 ? 2 : 4, PER = 16 / ES, COLS = 64 / ES;
   __syncwarp();
+  if (a.vec && col + COLS <= a.N) {
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const int r = (lane >> 2) + 8 * i, row = row0 + r, c = col + (lane & 3) * PER;
-    if (row >= a.M || c >= a.N) continue;
-    uint4 v = *reinterpret_cast<const uint4*>(stg + stg_off(r, lane & 3));
-    const bool vec = a.vec && c + PER <= a.N;
-    if constexpr (OUT == OUT_BF16) {
-      __nv_bfloat16* d = reinterpret_cast<__nv_bfloat16*>(a.D) + (long)row * a.ldd + c;
-      if (vec) {
+    for (int i = 0; i < 4; ++i) {
+      const int r = (lane >> 2) + 8 * i, row = row0 + r;
+      if (row >= a.M) continue;
+      const uint4 v = *reinterpret_cast<const uint4*>(stg + stg_off(r, lane & 3));
+      uint8_t* d = reinterpret_cast<uint8_t*>(a.D) + ((long)(part_row + row) * a.ldd + col + (lane & 3) * PER) * ES;
+      if constexpr (OUT == OUT_ACC_F32)
+        // each element is added to once, by one thread: the reduction happens in L2 and nothing waits for the
+        // old value
+        asm volatile("red.global.add.v4.f32 [%0], {%1, %2, %3, %4};" ::"l"(d), "f"(__uint_as_float(v.x)),
+                     "f"(__uint_as_float(v.y)), "f"(__uint_as_float(v.z)), "f"(__uint_as_float(v.w))
+                     : "memory");
+      else
         *reinterpret_cast<uint4*>(d) = v;
+    }
+  } else {
+    constexpr int ROWS = 32 / COLS;  // rows per access: 1 (bf16) or 2 (fp32)
+    const int c = lane % COLS;
+#pragma unroll 4
+    for (int i = 0; i < 32; i += ROWS) {
+      const int r = i + lane / COLS, row = row0 + r;
+      if (row >= a.M || col + c >= a.N) continue;
+      const uint8_t* e = stg + stg_off(r, c / PER) + (c % PER) * ES;
+      const long at = (long)(part_row + row) * a.ldd + col + c;
+      if constexpr (OUT == OUT_BF16) {
+        reinterpret_cast<__nv_bfloat16*>(a.D)[at] = *reinterpret_cast<const __nv_bfloat16*>(e);
       } else {
-        const __nv_bfloat16* e = reinterpret_cast<const __nv_bfloat16*>(&v);
-#pragma unroll
-        for (int k = 0; k < PER; ++k)
-          if (c + k < a.N) d[k] = e[k];
-      }
-    } else {
-      float* d = reinterpret_cast<float*>(a.D) + (long)row * a.ldd + c;
-      float e[4] = {__uint_as_float(v.x), __uint_as_float(v.y), __uint_as_float(v.z), __uint_as_float(v.w)};
-      if (vec) {
-        if constexpr (OUT == OUT_ACC_F32) {
-          // each element is added to once, by one thread: the reduction happens in L2, nothing waits for
-          // the old value (accumulating 8192 x 11008 with loads held the accumulator 280 us longer)
-          asm volatile("red.global.add.v4.f32 [%0], {%1, %2, %3, %4};" ::"l"(d), "f"(e[0]), "f"(e[1]), "f"(e[2]),
-                       "f"(e[3])
-                       : "memory");
-        } else {
-          *reinterpret_cast<float4*>(d) = make_float4(e[0], e[1], e[2], e[3]);
-        }
-      } else {
-#pragma unroll
-        for (int k = 0; k < PER; ++k)
-          if (c + k < a.N) d[k] = OUT == OUT_ACC_F32 ? d[k] + e[k] : e[k];
+        float* d = reinterpret_cast<float*>(a.D) + at;
+        *d = (OUT == OUT_ACC_F32 ? *d : 0.f) + *reinterpret_cast<const float*>(e);
       }
     }
   }
@@ -286,13 +286,15 @@ __global__ void __launch_bounds__(320, 1)
     int stage = 0;
     uint32_t phase = 0, issued = 0, issued_phase = 0;  // a bit per stage
     bool ok = true;
-    for (int tile = unit; tile < args.num_tiles && ok; tile += units) {
+    for (int u = unit; u < args.num_tiles * args.splits && ok; u += units) {
+      const int tile = u / args.splits, k0 = (u - tile * args.splits) * args.k_per;
+      const int k1 = min(args.k_iters, k0 + args.k_per);
       int mb, nb;
       tile_coords(tile, args.m_blocks, args.n_blocks, mb, nb);
       // row blocks of this CTA; a pair's CTAs both take all of B's scales, for their own tensor memory
       const int arow = mb * CTAS + cta, brow = nb * (BN / 128);
-      int sa_tile = arow * args.k_quads, sb_tile = brow * args.k_quads;
-      for (int k = 0; k < args.k_iters; ++k) {
+      int sa_tile = arow * args.k_quads + k0 / SF_STEP, sb_tile = brow * args.k_quads + k0 / SF_STEP;
+      for (int k = k0; k < k1; ++k) {
         if (!warp_wait(smem_u32(&empty[stage]), phase ^ 1, args.err)) {
           ok = false;
           break;
@@ -342,12 +344,13 @@ __global__ void __launch_bounds__(320, 1)
       // descriptors of the ring's first stage; a stage or a 32-byte step only adds to the address field
       const uint64_t ad0 = sdesc_sw128(smem_u32(smem), 16, 1024), bd0 = sdesc_sw128(smem_u32(smem) + L::A_BYTES, 16, 1024);
       const uint32_t sf0 = smem_u32(smem + L::SF_OFF);
-      for (int tile = unit; tile < args.num_tiles && ok; tile += units, ++t) {
+      for (int u = unit; u < args.num_tiles * args.splits && ok; u += units, ++t) {
+        const int k0 = u % args.splits * args.k_per, k1 = min(args.k_iters, k0 + args.k_per);
         const int acc = t % ACCS;
         const uint32_t acc_phase = (t / ACCS) & 1;
         if (!warp_wait(smem_u32(&acc_empty[acc]), acc_phase ^ 1, args.err)) break;
         tc_fence_after();
-        for (int k = 0; k < args.k_iters; ++k) {
+        for (int k = k0; k < k1; ++k) {
           if (!warp_wait(smem_u32(&full[stage]), phase, args.err)) {
             ok = false;
             break;
@@ -367,8 +370,8 @@ __global__ void __launch_bounds__(320, 1)
             }
 #pragma unroll
             for (int kk = 0; kk < BK / 32; ++kk) {
-              if constexpr (PAIR) umma_mxf8_pair(tmem + acc * BN, ad + 2 * kk, bd + 2 * kk, idesc, sfa, sfb, k != 0 || kk != 0);
-              else umma_mxf8(tmem + acc * BN, ad + 2 * kk, bd + 2 * kk, idesc, sfa, sfb, k != 0 || kk != 0);
+              if constexpr (PAIR) umma_mxf8_pair(tmem + acc * BN, ad + 2 * kk, bd + 2 * kk, idesc, sfa, sfb, k != k0 || kk != 0);
+              else umma_mxf8(tmem + acc * BN, ad + 2 * kk, bd + 2 * kk, idesc, sfa, sfb, k != k0 || kk != 0);
             }
             if constexpr (PAIR) umma_commit_pair(&empty[stage]);
             else umma_commit(&empty[stage]);
@@ -388,7 +391,9 @@ __global__ void __launch_bounds__(320, 1)
     uint8_t* stg = smem + L::STG_OFF + (warp - 2) * 2048;
     constexpr int COLS = BN / 2;
     int t = 0;
-    for (int tile = unit; tile < args.num_tiles; tile += units, ++t) {
+    for (int u = unit; u < args.num_tiles * args.splits; u += units, ++t) {
+      const int tile = u / args.splits;
+      const int part_row = (u - tile * args.splits) * args.M;  // the part's first row in D
       const int acc = t % ACCS;
       const uint32_t acc_phase = (t / ACCS) & 1;
       int mb, nb;
@@ -397,59 +402,43 @@ __global__ void __launch_bounds__(320, 1)
       tc_fence_after();
       const uint32_t tb = tmem + ((uint32_t)(quad * 32) << 16) + acc * BN + half * COLS;
       const int row0 = mb * TILE_M + cta * BM + quad * 32, col0 = nb * BN + half * COLS;
-      if constexpr (OUT == OUT_BF16) {
-        uint32_t h[COLS / 2];
+      // the whole share into registers (COLS fp32), so that the accumulator is free before the stores begin
+      uint32_t v[COLS / 32][32];
 #pragma unroll
-        for (int c = 0; c < COLS; c += 64) {
-          uint32_t r[2][32];
-          tmem_ld32_async(tb + c, r[0]);
-          tmem_ld32_async(tb + c + 32, r[1]);
-          tmem_wait_ld();
-          tmem_regs(r[0]);
-          tmem_regs(r[1]);
+      for (int c = 0; c < COLS / 32; ++c) tmem_ld32_async(tb + c * 32, v[c]);
+      tmem_wait_ld();
 #pragma unroll
-          for (int p = 0; p < 2; ++p) {
-            float v[32];
+      for (int c = 0; c < COLS / 32; ++c) tmem_regs(v[c]);
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) {
+        if constexpr (PAIR) mbar_arrive_cluster(mapa_shared(smem_u32(&acc_empty[acc]), 0));
+        else mbar_arrive(&acc_empty[acc]);
+      }
 #pragma unroll
-            for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(r[p][i]);
-            if (args.R != nullptr) add_residual(args, row0 + lane, col0 + c + 32 * p, v);
+      for (int c = 0; c < COLS / 32; ++c) {
+        const int col = col0 + c * 32;
+        if (col >= args.N) break;
+        float f[32];
 #pragma unroll
-            for (int i = 0; i < 16; ++i) h[c / 2 + 16 * p + i] = pack_bf16x2(v[2 * i], v[2 * i + 1]);
-          }
-        }
-        tc_fence_before();
-        __syncwarp();
-        if (lane == 0) {
-          if constexpr (PAIR) mbar_arrive_cluster(mapa_shared(smem_u32(&acc_empty[acc]), 0));
-          else mbar_arrive(&acc_empty[acc]);
-        }
-#pragma unroll
-        for (int c = 0; c < COLS; c += 32) {
+        for (int i = 0; i < 32; ++i) f[i] = __uint_as_float(v[c][i]);
+        if constexpr (OUT == OUT_BF16) {
+          if (args.R != nullptr) add_residual(args, row0 + lane, col, f);
 #pragma unroll
           for (int i = 0; i < 4; ++i)
             *reinterpret_cast<uint4*>(stg + stg_off(lane, i)) =
-                make_uint4(h[c / 2 + 4 * i], h[c / 2 + 4 * i + 1], h[c / 2 + 4 * i + 2], h[c / 2 + 4 * i + 3]);
-          store_segment<OUT>(args, stg, row0, col0 + c, lane);
-        }
-      } else {
-#pragma unroll 1
-        for (int c = 0; c < COLS; c += 32) {
-          float v[32];
-          tmem_ld32(tb + c, v);
+                make_uint4(pack_bf16x2(f[8 * i], f[8 * i + 1]), pack_bf16x2(f[8 * i + 2], f[8 * i + 3]),
+                           pack_bf16x2(f[8 * i + 4], f[8 * i + 5]), pack_bf16x2(f[8 * i + 6], f[8 * i + 7]));
+          store_segment<OUT>(args, stg, row0, col, part_row, lane);
+        } else {
 #pragma unroll
           for (int g = 0; g < 2; ++g) {
 #pragma unroll
             for (int i = 0; i < 4; ++i)
               *reinterpret_cast<float4*>(stg + stg_off(lane, i)) =
-                  make_float4(v[16 * g + 4 * i], v[16 * g + 4 * i + 1], v[16 * g + 4 * i + 2], v[16 * g + 4 * i + 3]);
-            store_segment<OUT>(args, stg, row0, col0 + c + 16 * g, lane);
+                  make_float4(f[16 * g + 4 * i], f[16 * g + 4 * i + 1], f[16 * g + 4 * i + 2], f[16 * g + 4 * i + 3]);
+            store_segment<OUT>(args, stg, row0, col + 16 * g, part_row, lane);
           }
-        }
-        tc_fence_before();
-        __syncwarp();
-        if (lane == 0) {
-          if constexpr (PAIR) mbar_arrive_cluster(mapa_shared(smem_u32(&acc_empty[acc]), 0));
-          else mbar_arrive(&acc_empty[acc]);
         }
       }
     }
@@ -475,6 +464,52 @@ __global__ void __launch_bounds__(128) scale_tiles_kernel(const uint8_t* __restr
 #pragma unroll
   for (int i = 0; i < SF_STEP; ++i) w |= (k + i < kb ? (uint32_t)p[i * blk_stride] : 127u) << (8 * i);
   tiles[(long)blockIdx.x * 128 + (r & 31) * 4 + (r >> 5)] = w;
+}
+
+// D = sum over the parts of K, in part order (+ R): parts [splits, M, N] fp32.
+__global__ void __launch_bounds__(256) join_parts_kernel(const float* __restrict__ parts, int splits, int M, int N, void* D,
+                                                         long ldd, const __nv_bfloat16* R, long ldr, int out) {
+  // launched so that it may start before the product has ended: the parts are there after this
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  const long i = (long)blockIdx.x * 256 + threadIdx.x, mn = (long)M * N;
+  if (i >= mn) return;
+  const long row = i / N, col = i - row * N;
+  float s = 0.f;
+#pragma unroll 8
+  for (int p = 0; p < splits; ++p) s += parts[p * mn + i];
+  if (out == OUT_BF16) {
+    if (R != nullptr) s += __bfloat162float(R[row * ldr + col]);
+    reinterpret_cast<__nv_bfloat16*>(D)[row * ldd + col] = __float2bfloat16_rn(s);
+  } else {
+    float* d = reinterpret_cast<float*>(D) + row * ldd + col;
+    *d = out == OUT_ACC_F32 ? *d + s : s;
+  }
+}
+
+// Codes whose rows do not start on 16 bytes -> rows padded to 16 bytes (zeros behind the codes).  A thread
+// makes 16 bytes from the five 4-byte words that hold them; no word that begins past the row's end is read.
+__global__ void __launch_bounds__(256) pad_rows_kernel(const uint8_t* __restrict__ q, long ld, int rows, int K,
+                                                       uint4* __restrict__ out) {
+  const int per = (K + 15) >> 4;
+  const long i = (long)blockIdx.x * 256 + threadIdx.x;
+  if (i >= (long)rows * per) return;
+  const long row = i / per;
+  const int k = (int)(i - row * per) * 16;
+  const uintptr_t p = reinterpret_cast<uintptr_t>(q + row * ld + k), end = reinterpret_cast<uintptr_t>(q + row * ld + K);
+  const uint32_t sel = 0x3210u + 0x1111u * (uint32_t)(p & 3);
+  uint32_t u[5], w[4];
+#pragma unroll
+  for (int j = 0; j < 5; ++j) {
+    const uintptr_t a = (p & ~uintptr_t(3)) + 4 * j;
+    u[j] = a < end && (j < 4 || (p & 3)) ? __ldg(reinterpret_cast<const uint32_t*>(a)) : 0u;
+  }
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    const int left = K - (k + 4 * j);
+    w[j] = __byte_perm(u[j], u[j + 1], sel);
+    w[j] = left >= 4 ? w[j] : left <= 0 ? 0u : w[j] & (0xffffffffu >> (32 - 8 * left));
+  }
+  out[i] = make_uint4(w[0], w[1], w[2], w[3]);
 }
 
 // ---------------------------------------------------------------- host side
@@ -530,7 +565,7 @@ static void launch(const CUtensorMap* t, GemmArgs& g, cudaStream_t st) {
   g.n_blocks = (g.N + BN - 1) / BN;
   g.num_tiles = g.m_blocks * g.n_blocks;
   cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3(CTAS * std::min(g.num_tiles, device_sm_count() / CTAS), 1, 1);
+  cfg.gridDim = dim3(CTAS * std::min(g.num_tiles * g.splits, device_sm_count() / CTAS), 1, 1);
   cfg.blockDim = dim3(320, 1, 1);
   cfg.dynamicSmemBytes = L::TOTAL;
   cfg.stream = st;
@@ -590,9 +625,48 @@ void fp8_gemm(torch::Tensor A, torch::Tensor tA, torch::Tensor B, torch::Tensor 
   g.k_iters = (g.K + fp8::BK - 1) / fp8::BK;
   auto st = at::cuda::getCurrentCUDAStream();
   const CUtensorMap maps[4] = {fp8::code_map(A), fp8::code_map(B), fp8::tile_map(tA), fp8::tile_map(tB)};
-  // pairs once their 256 x 256 tiles fill the SMs
-  const bool pair = ((M + 255) / 256) * ((N + 255) / 256) >= device_sm_count() / 2;
+  // Pairs once their 256 x 256 tiles fill the SMs.  Below that 128 x 128 tiles, and where those are fewer than
+  // the SMs (few tokens: the weights' bytes bound the product) K is cut into parts whose fp32 sums a second
+  // kernel adds in order: the least (rounds of units) x (blocks per unit + 2 for a unit's start and end).
+  // 48 x 4096 x 11008: 28 us in one part, 13 in six; 1 x 22016 x 4096: 34 and 21.
+  const int sms = device_sm_count();
+  const bool pair = ((M + 255) / 256) * ((N + 255) / 256) >= sms / 2;
   const int out = D.scalar_type() == at::kBFloat16 ? fp8::OUT_BF16 : accumulate ? fp8::OUT_ACC_F32 : fp8::OUT_F32;
+  g.splits = 1;
+  g.k_per = g.k_iters;
+  if (!pair) {
+    const long tiles = ((M + 127) / 128) * ((N + 127) / 128);
+    auto cost = [&](long splits, long k_per) { return (tiles * splits + sms - 1) / sms * (k_per + 2) + (splits > 1 ? 8 : 0); };
+    long best = cost(1, g.k_iters);
+    for (int k_per = fp8::SF_STEP; k_per < g.k_iters; k_per += fp8::SF_STEP) {
+      const long splits = (g.k_iters + k_per - 1) / k_per;
+      if (splits * M * N * 4 <= (64L << 20) && cost(splits, k_per) < best) {
+        best = cost(splits, k_per);
+        g.splits = (int)splits;
+        g.k_per = k_per;
+      }
+    }
+  }
+  if (g.splits > 1) {
+    auto parts = torch::empty({g.splits, M, N}, D.options().dtype(at::kFloat));
+    fp8::GemmArgs p = g;
+    p.D = parts.data_ptr();
+    p.ldd = N;
+    p.R = nullptr;
+    p.vec = N % 4 == 0;
+    fp8::launch<128, false, fp8::OUT_F32>(maps, p, st);
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3((unsigned)((M * N + 255) / 256), 1, 1);
+    cfg.blockDim = dim3(256, 1, 1);
+    cfg.stream = st;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    DTB_CUDA(cudaLaunchKernelEx(&cfg, fp8::join_parts_kernel, (const float*)parts.data_ptr<float>(), g.splits, g.M, g.N, g.D, g.ldd, g.R, g.ldr, out));
+    return;
+  }
   if (out == fp8::OUT_BF16) pair ? fp8::launch<256, true, fp8::OUT_BF16>(maps, g, st) : fp8::launch<128, false, fp8::OUT_BF16>(maps, g, st);
   else if (out == fp8::OUT_F32) pair ? fp8::launch<256, true, fp8::OUT_F32>(maps, g, st) : fp8::launch<128, false, fp8::OUT_F32>(maps, g, st);
   else pair ? fp8::launch<256, true, fp8::OUT_ACC_F32>(maps, g, st) : fp8::launch<128, false, fp8::OUT_ACC_F32>(maps, g, st);
@@ -611,4 +685,32 @@ torch::Tensor fp8_scale_tiles(torch::Tensor s, int64_t gran, int64_t rows) {
       reinterpret_cast<uint32_t*>(t.data_ptr()));
   DTB_LAUNCH_CHECK();
   return t;
+}
+
+// The codes with rows on 16-byte boundaries: a padded copy where they are not.
+static torch::Tensor fp8_aligned(torch::Tensor q) {
+  if (q.numel() == 0 || ((reinterpret_cast<uintptr_t>(q.data_ptr()) & 15) == 0 && (q.size(1) == 1 || q.stride(1) == 1) &&
+                         (q.size(0) == 1 || q.stride(0) % 16 == 0)))
+    return q;
+  if (q.size(1) > 1 && q.stride(1) != 1) q = q.contiguous();
+  const long rows = q.size(0), K = q.size(1), per = (K + 15) / 16;
+  DTB_CHECK(rows < (1L << 30) && K < (1L << 30) && (rows * per + 255) / 256 < (1L << 31), "fp8_product: too large");
+  auto pad = torch::empty({rows, per * 16}, q.options());
+  fp8::pad_rows_kernel<<<(unsigned)((rows * per + 255) / 256), 256, 0, at::cuda::getCurrentCUDAStream()>>>(
+      reinterpret_cast<const uint8_t*>(q.data_ptr()), rows > 1 ? q.stride(0) : K, (int)rows, (int)K,
+      reinterpret_cast<uint4*>(pad.data_ptr()));
+  DTB_LAUNCH_CHECK();
+  return pad.narrow(1, 0, K);
+}
+
+// fp8_gemm for operands as a user holds them: codes in rows of any alignment, plain scales, scale tiles or none.
+void fp8_product(torch::Tensor A, torch::Tensor sA, c10::optional<torch::Tensor> tA, torch::Tensor B, torch::Tensor sB,
+                 c10::optional<torch::Tensor> tB, torch::Tensor D, c10::optional<torch::Tensor> R, bool accumulate) {
+  for (const torch::Tensor* t : {&A, &B})
+    DTB_CHECK(t->is_cuda() && t->scalar_type() == at::kFloat8_e4m3fn && t->dim() == 2, "fp8_product: operands must be 2-D e4m3 on the GPU");
+  const c10::cuda::CUDAGuard guard(A.device());
+  auto tiles = [](const torch::Tensor& q, const torch::Tensor& s, const c10::optional<torch::Tensor>& t) {
+    return t.has_value() ? *t : fp8_scale_tiles(s, s.size(0) == (q.size(0) + 127) / 128 ? 128 : 1, q.size(0));
+  };
+  fp8_gemm(fp8_aligned(A), tiles(A, sA, tA), fp8_aligned(B), tiles(B, sB, tB), D, R, accumulate);
 }

@@ -95,21 +95,6 @@ def quantize_fp8(x: torch.Tensor, *, square: bool = False) -> Fp8Blocks:
     return _quantize(x, square, True, False)[0]
 
 
-def _aligned(b: Fp8Blocks) -> Fp8Blocks:
-    """Rows on 16-byte boundaries, as the tensor-memory loads need them (a copy where they are not)."""
-    v = b.values
-    if v.is_cuda and v.numel() and ((v.shape[0] > 1 and v.stride(0) % 16) or v.stride(1) != 1 or v.data_ptr() % 16):
-        r, c = v.shape
-        pad = torch.empty(r, -(-c // 16) * 16, device=v.device, dtype=torch.uint8)[:, :c]
-        pad.copy_(v.view(torch.uint8))
-        return Fp8Blocks(pad.view(E4M3), b.scales, b.tiles)
-    return b
-
-
-def _tiles(b: Fp8Blocks, gran: int) -> torch.Tensor:
-    return b.tiles if b.tiles is not None else native().fp8_scale_tiles(b.scales, gran, b.values.shape[0])
-
-
 def fp8_matmul(a: Fp8Blocks, b: Fp8Blocks, *, residual: torch.Tensor | None = None, out: torch.Tensor | None = None,
                out_dtype: torch.dtype = torch.bfloat16, accumulate: bool = False) -> torch.Tensor:
     """``a [M, K] @ b [N, K]^T (+ residual)`` in bf16 or fp32; ``accumulate`` adds to the fp32 ``out``."""
@@ -118,7 +103,7 @@ def fp8_matmul(a: Fp8Blocks, b: Fp8Blocks, *, residual: torch.Tensor | None = No
     for t in (a, b):
         if t.values.dtype != E4M3 or t.scales.dtype != E8M0:
             raise ValueError(f"fp8_matmul takes e4m3 codes with e8m0 scales, got {t.values.dtype} and {t.scales.dtype}")
-    ga, gb = a.rows_per_scale, b.rows_per_scale
+        t.rows_per_scale  # noqa: B018 - raises when the scales do not fit
     shape = (a.values.shape[0], b.values.shape[0])
     if out is None:
         if accumulate:
@@ -129,8 +114,7 @@ def fp8_matmul(a: Fp8Blocks, b: Fp8Blocks, *, residual: torch.Tensor | None = No
     if residual is not None and tuple(residual.shape) != shape:
         raise ValueError(f"residual is {tuple(residual.shape)}, the product {shape}")
     if a.values.is_cuda:
-        a, b = _aligned(a), _aligned(b)
-        native().fp8_gemm(a.values, _tiles(a, ga), b.values, _tiles(b, gb), out, residual, accumulate)
+        native().fp8_product(a.values, a.scales, a.tiles, b.values, b.scales, b.tiles, out, residual, accumulate)
         return out
     y = a.dequantize() @ b.dequantize().t()
     if residual is not None:
@@ -195,7 +179,10 @@ def linear_fp8(x: torch.Tensor, weight: torch.Tensor | Fp8Blocks, *, residual: t
     if isinstance(weight, Fp8Blocks):
         if torch.is_grad_enabled() and (x.requires_grad or (residual is not None and residual.requires_grad)):
             raise ValueError("weights kept in 8 bits have no backward: call linear_fp8 with the weight tensor")
-        y = fp8_matmul(_quantize(x2, False, True, False)[0], weight, residual=r2, out_dtype=x.dtype)
+        if x.is_cuda:
+            y = native().linear_fp8_kept(x2, *weight, r2)
+        else:
+            y = fp8_matmul(_quantize(x2, False, True, False)[0], weight, residual=r2, out_dtype=x.dtype)
     else:
         w = weight if weight.is_contiguous() else weight.contiguous()
         y = native().linear_fp8(x2, w, r2) if x.is_cuda and main_grad is None else _LinearFp8Fn.apply(x2, w, r2, main_grad)
