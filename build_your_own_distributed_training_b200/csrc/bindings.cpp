@@ -71,7 +71,7 @@ torch::Tensor qk_norm_rope_bwd(torch::Tensor g, torch::Tensor x, torch::Tensor w
                                int64_t nkv, int64_t hd, int64_t seqlen, double eps, torch::Tensor dwq,
                                torch::Tensor dwk, bool accumulate);
 std::vector<torch::Tensor> token_logprobs_fwd(torch::Tensor x, torch::Tensor tokens, double temperature, int64_t top_k,
-                                              int64_t ignore);
+                                              int64_t ignore, bool want_state);
 void token_logprobs_bwd(torch::Tensor x, torch::Tensor tokens, torch::Tensor state, c10::optional<torch::Tensor> g_lp,
                         c10::optional<torch::Tensor> g_ent, double temperature, torch::Tensor dx);
 void swiglu_fwd(torch::Tensor gu, torch::Tensor act);

@@ -15,7 +15,8 @@ Tensor qk_norm_rope_bwd(Tensor g, Tensor x, Tensor wq, Tensor wk, Tensor cos_t, 
                         c10::optional<Tensor> pos, int64_t nq, int64_t nkv, int64_t hd, int64_t seqlen, double eps,
                         Tensor dwq, Tensor dwk, bool accumulate);
 Tensor dropout_add(Tensor x, c10::optional<Tensor> residual, int64_t cut, int64_t seed, int64_t start);
-std::vector<Tensor> token_logprobs_fwd(Tensor x, Tensor tokens, double temperature, int64_t top_k, int64_t ignore);
+std::vector<Tensor> token_logprobs_fwd(Tensor x, Tensor tokens, double temperature, int64_t top_k, int64_t ignore,
+                                       bool want_state);
 void token_logprobs_bwd(Tensor x, Tensor tokens, Tensor state, c10::optional<Tensor> g_lp, c10::optional<Tensor> g_ent,
                         double temperature, Tensor dx);
 std::vector<Tensor> fp8_quantize(Tensor x, bool square, bool plain, bool transposed);
@@ -66,12 +67,13 @@ Tensor row_grad(const Tensor& g) { return g.defined() ? g.to(at::kFloat).contigu
 struct TokenLogProbs : public Function<TokenLogProbs> {
   static variable_list forward(AutogradContext* ctx, const Tensor& x, const Tensor& tokens, double temperature,
                                int64_t top_k, int64_t ignore) {
-    auto r = token_logprobs_fwd(x, tokens, temperature, top_k, ignore);  // logprob, entropy, state, top
-    ctx->save_for_backward({x, tokens, r[2]});
+    auto r = token_logprobs_fwd(x, tokens, temperature, top_k, ignore, true);
+    ctx->save_for_backward({x, tokens, r.back()});
+    r.pop_back();
     ctx->saved_data["t"] = temperature;
-    ctx->mark_non_differentiable({r[3], r[4]});
+    if (top_k > 0) ctx->mark_non_differentiable({r[2], r[3]});
     ctx->set_materialize_grads(false);
-    return {r[0], r[1], r[3], r[4]};
+    return r;
   }
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
     const auto s = ctx->get_saved_variables();
@@ -82,7 +84,7 @@ struct TokenLogProbs : public Function<TokenLogProbs> {
     if (pitch > 2 * V + 1024) pitch = V;
     Tensor dx = torch::empty({M, pitch}, x.options());
     if (pitch != V) dx = dx.narrow(1, 0, V);
-    const Tensor gl = row_grad(grads[0]), ge = row_grad(grads[1]);
+    const Tensor gl = row_grad(grads[0]), ge = row_grad(grads[1]);  // (of the tokens' shape)
     token_logprobs_bwd(x, s[1], s[2], gl.defined() ? c10::optional<Tensor>(gl) : c10::nullopt,
                        ge.defined() ? c10::optional<Tensor>(ge) : c10::nullopt, ctx->saved_data["t"].toDouble(), dx);
     return {dx, {}, {}, {}, {}};
@@ -125,14 +127,24 @@ struct LinearFp8 : public Function<LinearFp8> {
 
 }  // namespace
 
+// (a call that nothing will differentiate skips the node)
+static bool tracked(const Tensor& t) { return t.requires_grad() && at::GradMode::is_enabled(); }
+
 Tensor qk_norm_rope_autograd(Tensor x, Tensor wq, Tensor wk, Tensor cos_t, Tensor sin_t, c10::optional<Tensor> pos,
                              int64_t nq, int64_t nkv, int64_t hd, int64_t seqlen, double eps) {
+  if (!tracked(x) && !tracked(wq) && !tracked(wk)) return qk_norm_rope_fwd(x, wq, wk, cos_t, sin_t, pos, nq, nkv, hd, seqlen, eps);
   return QkNormRope::apply(x, wq, wk, cos_t, sin_t, pos, nq, nkv, hd, seqlen, eps);
 }
 Tensor dropout_add_autograd(Tensor x, c10::optional<Tensor> residual, int64_t cut, int64_t seed, int64_t start) {
+  if (!tracked(x) && !(residual.has_value() && tracked(*residual))) return dropout_add(x, residual, cut, seed, start);
   return DropoutAdd::apply(x, residual, cut, seed, start);
 }
+// logits [..., V], tokens [...] -> {logprob, entropy} or {logprob, entropy, top log probabilities, top tokens}
 std::vector<Tensor> token_logprobs_autograd(Tensor x, Tensor tokens, double temperature, int64_t top_k, int64_t ignore) {
+  if (x.dim() != 2) x = x.reshape({-1, x.size(-1)});
+  if (x.stride(1) != 1 && x.numel() > 0) x = x.contiguous();
+  if (!tokens.is_contiguous()) tokens = tokens.contiguous();
+  if (!tracked(x)) return token_logprobs_fwd(x, tokens, temperature, top_k, ignore, false);
   return TokenLogProbs::apply(x, tokens, temperature, top_k, ignore);
 }
 // x [T, K] bf16, w [N, K], residual [T, N] bf16 or none

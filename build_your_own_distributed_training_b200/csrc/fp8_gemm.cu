@@ -52,6 +52,7 @@ struct GemmArgs {
   const __nv_bfloat16* R;  // OUT_BF16: residual, or null
   long ldr;
   int m_blocks, n_blocks, k_iters, k_quads, num_tiles;
+  int a_bytes;             // bytes of A's box: fewer than 128 rows of it when M is smaller
   int splits, k_per;       // K in `splits` parts of k_per blocks (a multiple of SF_STEP); part p writes D + p * M * ldd
   int vec;                 // D (and R) rows start on 16 bytes
   int* err;
@@ -305,7 +306,7 @@ __global__ void __launch_bounds__(320, 1)
         // a pair's bytes complete on the leader's barrier
         const uint32_t fb = PAIR ? mapa_shared(smem_u32(&full[stage]), 0) : 0;
         if (elect_one()) {
-          if (leader) mbar_arrive_expect_tx(&full[stage], CTAS * (L::STAGE + (with_sf ? L::SF_STAGE : 0)));
+          if (leader) mbar_arrive_expect_tx(&full[stage], CTAS * (args.a_bytes + L::B_BYTES + (with_sf ? L::SF_STAGE : 0)));
           if constexpr (PAIR) {
             tma_load_2d_pair(sa, &tmA, fb, k * BK, arow * BM);
             tma_load_2d_pair(sa + L::A_BYTES, &tmB, fb, k * BK, (brow + cta) * 128);
@@ -543,11 +544,11 @@ static CUtensorMap make_map(CUtensorMapDataType type, CUtensorMapSwizzle swizzle
   DTB_CHECK(r == CUDA_SUCCESS, "cuTensorMapEncodeTiled failed (%d): inner=%ld rows=%ld pitch=%ld base=%p", (int)r, inner, rows, pitch, base);
   return m;
 }
-// codes: boxes of 128 rows x 128 bytes; bytes past the matrix read as zero
-static CUtensorMap code_map(const torch::Tensor& t) {
+// codes: boxes of `box_rows` rows x 128 bytes; bytes past the matrix read as zero
+static CUtensorMap code_map(const torch::Tensor& t, int box_rows) {
   const long rows = t.size(0), k = t.size(1);
   return make_map(CU_TENSOR_MAP_DATA_TYPE_UINT8, CU_TENSOR_MAP_SWIZZLE_128B, t.data_ptr(), k, rows,
-                  rows > 1 ? t.stride(0) : (k + 15) / 16 * 16, 128, 128);
+                  rows > 1 ? t.stride(0) : (k + 15) / 16 * 16, 128, box_rows);
 }
 // scale tiles [row blocks, k blocks / 4, 512 bytes]: one tile per box
 static CUtensorMap tile_map(const torch::Tensor& t) {
@@ -624,29 +625,38 @@ void fp8_gemm(torch::Tensor A, torch::Tensor tA, torch::Tensor B, torch::Tensor 
   g.k_quads = (g.K + 511) / 512;
   g.k_iters = (g.K + fp8::BK - 1) / fp8::BK;
   auto st = at::cuda::getCurrentCUDAStream();
-  const CUtensorMap maps[4] = {fp8::code_map(A), fp8::code_map(B), fp8::tile_map(tA), fp8::tile_map(tB)};
-  // Pairs once their 256 x 256 tiles fill the SMs.  Below that 128 x 128 tiles, and where those are fewer than
-  // the SMs (few tokens: the weights' bytes bound the product) K is cut into parts whose fp32 sums a second
-  // kernel adds in order: the least (rounds of units) x (blocks per unit + 2 for a unit's start and end).
-  // 48 x 4096 x 11008: 28 us in one part, 13 in six; 1 x 22016 x 4096: 34 and 21.
+  // Few tokens: A's box holds only as many rows (a stage's 256 rows of 128 bytes would take the copy engine
+  // longer than the weights' bytes take to arrive).  The tile's other rows keep whatever the shared memory
+  // holds; a row of A reaches only its own row of the result, and those are not stored.
+  const int a_rows = M <= 16 ? 16 : M <= 32 ? 32 : M <= 64 ? 64 : 128;
+  g.a_bytes = a_rows * fp8::BK;
+  const CUtensorMap maps[4] = {fp8::code_map(A, a_rows), fp8::code_map(B, 128), fp8::tile_map(tA), fp8::tile_map(tB)};
+  // Which kernel, and K in how many parts: the least modelled time.  A 128-deep stage takes about 500 cycles on a
+  // single CTA (128 x 128 tile) and 700 on a pair (256 x 256) when nothing else holds it up; a unit of work
+  // costs two stages more for its start and end, and parts of K, whose fp32 sums a second kernel adds in
+  // order, about 11 stages more and their bytes (100 cycles for 275 kB).  Parts fill the SMs where tiles are few (a few tokens against the weights).
+  // 48 x 4096 x 11008: one part 28 us, six 16; 1 x 22016 x 4096: pairs 30 us, single CTAs in four parts 19.
   const int sms = device_sm_count();
-  const bool pair = ((M + 255) / 256) * ((N + 255) / 256) >= sms / 2;
-  const int out = D.scalar_type() == at::kBFloat16 ? fp8::OUT_BF16 : accumulate ? fp8::OUT_ACC_F32 : fp8::OUT_F32;
+  const long tiles = ((M + 127) / 128) * ((N + 127) / 128), tiles2 = ((M + 255) / 256) * ((N + 255) / 256);
+  auto cost = [&](long splits, long k_per) { return (tiles * splits + sms - 1) / sms * (k_per + 2) * 5 + (splits > 1 ? 55 + splits * M * N * 8 / 275000 : 0); };
+  const long pair_cost = (tiles2 + sms / 2 - 1) / (sms / 2) * (g.k_iters + 2) * 7;
+  long best = cost(1, g.k_iters);
   g.splits = 1;
   g.k_per = g.k_iters;
-  if (!pair) {
-    const long tiles = ((M + 127) / 128) * ((N + 127) / 128);
-    auto cost = [&](long splits, long k_per) { return (tiles * splits + sms - 1) / sms * (k_per + 2) + (splits > 1 ? 8 : 0); };
-    long best = cost(1, g.k_iters);
-    for (int k_per = fp8::SF_STEP; k_per < g.k_iters; k_per += fp8::SF_STEP) {
-      const long splits = (g.k_iters + k_per - 1) / k_per;
-      if (splits * M * N * 4 <= (64L << 20) && cost(splits, k_per) < best) {
-        best = cost(splits, k_per);
-        g.splits = (int)splits;
-        g.k_per = k_per;
-      }
+  for (int k_per = fp8::SF_STEP; k_per < g.k_iters; k_per += fp8::SF_STEP) {
+    const long splits = (g.k_iters + k_per - 1) / k_per;
+    if (splits * M * N * 4 <= (64L << 20) && cost(splits, k_per) < best) {
+      best = cost(splits, k_per);
+      g.splits = (int)splits;
+      g.k_per = k_per;
     }
   }
+  const bool pair = pair_cost < best;
+  if (pair) {
+    g.splits = 1;
+    g.k_per = g.k_iters;
+  }
+  const int out = D.scalar_type() == at::kBFloat16 ? fp8::OUT_BF16 : accumulate ? fp8::OUT_ACC_F32 : fp8::OUT_F32;
   if (g.splits > 1) {
     auto parts = torch::empty({g.splits, M, N}, D.options().dtype(at::kFloat));
     fp8::GemmArgs p = g;

@@ -9,10 +9,11 @@
 // gu n,  dx = r (gu w - n mean(gu w n)),  dv = g.  r is recomputed from x, which the backward reads
 // anyway, so nothing but the input is saved.
 //
-// Both directions are bound by memory.  A group of L lanes holds one head, each lane VEC elements of
-// the first half and their partners of the second, so the rotation needs no exchange and the only
-// cross-lane step is the L-lane sum.  A warp stays on one token: its cos/sin row and the weights are
-// read once and live in registers while the token's heads stream through.  Statistics, rotation and
+// Both directions are bound by memory.  A group of L lanes holds one head, each lane 4 elements of the
+// first half and their partners of the second, so the rotation needs no exchange and the only cross-lane
+// step is the L-lane sum.  (8 + 8 elements a lane filled the register file in the backward: 121 us for 8192
+// tokens of 48 heads of 128.)  A warp stays on one token: its cos/sin row is read once and lives in
+// registers while the token's heads stream through, several heads per lane group in flight.  Statistics, rotation and
 // weight gradients are fp32; y and dx are rounded once, to the storage type.
 //
 // dw: every warp adds up the heads of its tokens in registers, the block's warps are added in order
@@ -100,13 +101,23 @@ __device__ __forceinline__ void load_table(const Args& a, const Lane<VEC, NP>& l
 template <int VEC, int NP>
 __device__ __forceinline__ void load_weight(const void* w, int wdt, const Lane<VEC, NP>& ln, int half,
                                             float (&lo)[NP][VEC], float (&hi)[NP][VEC]) {
+  // a weight of the model's type is a few hundred bytes that stay in L1
 #pragma unroll
-  for (int i = 0; i < NP; ++i)
+  for (int i = 0; i < NP; ++i) {
+    if (wdt == DT_F32) {
 #pragma unroll
-    for (int v = 0; v < VEC; ++v) {
-      lo[i][v] = ln.on[i] ? load_as(w, ln.off[i] + v, wdt) : 0.f;
-      hi[i][v] = ln.on[i] ? load_as(w, ln.off[i] + half + v, wdt) : 0.f;
+      for (int v = 0; v < VEC; ++v) {
+        lo[i][v] = ln.on[i] ? __ldg(reinterpret_cast<const float*>(w) + ln.off[i] + v) : 0.f;
+        hi[i][v] = ln.on[i] ? __ldg(reinterpret_cast<const float*>(w) + ln.off[i] + half + v) : 0.f;
+      }
+    } else {
+#pragma unroll
+      for (int v = 0; v < VEC; ++v) {
+        lo[i][v] = ln.on[i] ? load_as(w, ln.off[i] + v, wdt) : 0.f;
+        hi[i][v] = ln.on[i] ? load_as(w, ln.off[i] + half + v, wdt) : 0.f;
+      }
     }
+  }
 }
 
 __device__ __forceinline__ float group_sum(float v, int lanes) {
@@ -114,88 +125,155 @@ __device__ __forceinline__ float group_sum(float v, int lanes) {
   return v;
 }
 
-// U heads are in flight per lane group.
+// A token's heads come in three runs, [0, nq) queries, [nq, nq + nkv) keys and as many values; each run is
+// walked by itself, so the weight of a run is one set of registers and nothing is selected per element.  A
+// warp takes `per` heads of the run at a time, one per lane group, and every `split`-th such step; U steps
+// are in flight.
+enum : int { Q = 0, K = 1, V = 2 };
+
+template <typename T, int VEC, int NP>
+__device__ __forceinline__ void load_head(Pack<T, VEC> (&lo)[NP], Pack<T, VEC> (&hi)[NP], const T* p, int half,
+                                          const Lane<VEC, NP>& ln, bool live) {
+#pragma unroll
+  for (int i = 0; i < NP; ++i)
+    if (live && ln.on[i]) {
+      lo[i].load(p + ln.off[i]);
+      hi[i].load(p + half + ln.off[i]);
+    } else {
+#pragma unroll
+      for (int v = 0; v < VEC; ++v) lo[i].set(v, 0.f), hi[i].set(v, 0.f);
+    }
+}
+template <typename T, int VEC, int NP>
+__device__ __forceinline__ void store_head(const Pack<T, VEC> (&lo)[NP], const Pack<T, VEC> (&hi)[NP], T* p, int half,
+                                           const Lane<VEC, NP>& ln, bool live) {
+#pragma unroll
+  for (int i = 0; i < NP; ++i)
+    if (live && ln.on[i]) {
+      lo[i].store(p + ln.off[i]);
+      hi[i].store(p + half + ln.off[i]);
+    }
+}
+
+template <int KIND, typename T, int VEC, int NP, int U>
+__device__ __forceinline__ void fwd_run(const Args& a, const T* x, T* y, const Lane<VEC, NP>& ln, int grp, int part,
+                                        const float (&c)[NP][VEC], const float (&s)[NP][VEC]) {
+  const int half = a.hd >> 1, per = 32 / a.lanes, stride = per * a.split;
+  const int first = KIND == Q ? 0 : KIND == K ? a.nq : a.nq + a.nkv, end = first + (KIND == Q ? a.nq : a.nkv);
+  const float inv_hd = 1.f / (float)a.hd;
+  float wl[NP][VEC], wh[NP][VEC];
+  if constexpr (KIND != V) load_weight(KIND == Q ? a.wq : a.wk, a.wdt, ln, half, wl, wh);
+  for (int h0 = first + part * per; h0 < end; h0 += U * stride) {
+    Pack<T, VEC> lo[U][NP], hi[U][NP];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int h = h0 + u * stride + grp;
+      load_head(lo[u], hi[u], x + (long)h * a.hd, half, ln, h < end);
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int h = h0 + u * stride + grp;
+      if constexpr (KIND != V) {
+        float ss = 0.f;
+#pragma unroll
+        for (int i = 0; i < NP; ++i)
+#pragma unroll
+          for (int v = 0; v < VEC; ++v) {
+            const float p = lo[u][i].at(v), q = hi[u][i].at(v);
+            ss = fmaf(p, p, fmaf(q, q, ss));
+          }
+        const float r = rsqrtf(group_sum(ss, a.lanes) * inv_hd + a.eps);
+#pragma unroll
+        for (int i = 0; i < NP; ++i)
+#pragma unroll
+          for (int v = 0; v < VEC; ++v) {
+            const float ul = lo[u][i].at(v) * r * wl[i][v], uh = hi[u][i].at(v) * r * wh[i][v];
+            lo[u][i].set(v, ul * c[i][v] - uh * s[i][v]);
+            hi[u][i].set(v, uh * c[i][v] + ul * s[i][v]);
+          }
+      }
+      store_head(lo[u], hi[u], y + (long)h * a.hd, half, ln, h < end);
+    }
+  }
+}
+
 template <typename T, int VEC, int NP, int U>
 __global__ void __launch_bounds__(NT) qk_fwd_kernel(const Args a) {
   const int lane = threadIdx.x & 31;
   const long item = (long)blockIdx.x * (NT / 32) + (threadIdx.x >> 5);
   if (item >= a.tokens * a.split) return;
   const long token = item / a.split;
-  const int part = (int)(item % a.split);
-  const int half = a.hd >> 1, heads = a.nq + 2 * a.nkv, per = 32 / a.lanes;
-  const Lane<VEC, NP> ln(lane & (a.lanes - 1), a.lanes, half);
-  const int grp = lane / a.lanes;
+  const int part = (int)(item % a.split), grp = lane / a.lanes;
+  const Lane<VEC, NP> ln(lane & (a.lanes - 1), a.lanes, a.hd >> 1);
   const T* x = reinterpret_cast<const T*>(a.x) + token * a.ld;
   T* y = reinterpret_cast<T*>(a.out) + token * a.ldo;
-  float c[NP][VEC], s[NP][VEC], wl[2][NP][VEC], wh[2][NP][VEC];
+  float c[NP][VEC], s[NP][VEC];
   load_table(a, ln, token, c, s, lane);
-  load_weight(a.wq, a.wdt, ln, half, wl[0], wh[0]);
-  load_weight(a.wk, a.wdt, ln, half, wl[1], wh[1]);
+  fwd_run<Q, T, VEC, NP, U>(a, x, y, ln, grp, part, c, s);
+  fwd_run<K, T, VEC, NP, U>(a, x, y, ln, grp, part, c, s);
+  fwd_run<V, T, VEC, NP, U>(a, x, y, ln, grp, part, c, s);
+}
+
+template <int KIND, typename T, int VEC, int NP, int U>
+__device__ __forceinline__ void bwd_run(const Args& a, const T* x, const T* g, T* dx, const Lane<VEC, NP>& ln, int grp,
+                                        int part, const float (&c)[NP][VEC], const float (&s)[NP][VEC],
+                                        float (&dl)[NP][VEC], float (&dh)[NP][VEC]) {
+  const int half = a.hd >> 1, per = 32 / a.lanes, stride = per * a.split;
+  const int first = KIND == Q ? 0 : KIND == K ? a.nq : a.nq + a.nkv, end = first + (KIND == Q ? a.nq : a.nkv);
   const float inv_hd = 1.f / (float)a.hd;
-  const int stride = per * a.split;
-  for (int h0 = part * per; h0 < heads; h0 += U * stride) {
-    Pack<T, VEC> lo[U][NP], hi[U][NP];
+  float wl[NP][VEC], wh[NP][VEC];
+  if constexpr (KIND != V) load_weight(KIND == Q ? a.wq : a.wk, a.wdt, ln, half, wl, wh);
+  for (int h0 = first + part * per; h0 < end; h0 += U * stride) {
+    Pack<T, VEC> gl[U][NP], gh[U][NP], xl[U][NP], xh[U][NP];
 #pragma unroll
     for (int u = 0; u < U; ++u) {
       const int h = h0 + u * stride + grp;
-#pragma unroll
-      for (int i = 0; i < NP; ++i)
-        if (h < heads && ln.on[i]) {
-          lo[u][i].load(x + (long)h * a.hd + ln.off[i]);
-          hi[u][i].load(x + (long)h * a.hd + half + ln.off[i]);
-        } else {
-#pragma unroll
-          for (int v = 0; v < VEC; ++v) lo[u][i].set(v, 0.f), hi[u][i].set(v, 0.f);
-        }
+      load_head(gl[u], gh[u], g + (long)h * a.hd, half, ln, h < end);
+      if constexpr (KIND != V) load_head(xl[u], xh[u], x + (long)h * a.hd, half, ln, h < end);
     }
 #pragma unroll
     for (int u = 0; u < U; ++u) {
       const int h = h0 + u * stride + grp;
-      float ss = 0.f;
-#pragma unroll
-      for (int i = 0; i < NP; ++i)
-#pragma unroll
-        for (int v = 0; v < VEC; ++v) {
-          const float p = lo[u][i].at(v), q = hi[u][i].at(v);
-          ss = fmaf(p, p, fmaf(q, q, ss));
-        }
-      ss = group_sum(ss, a.lanes);
-      if (h >= heads) continue;
-      if (h < a.nq + a.nkv) {
-        const float r = rsqrtf(ss * inv_hd + a.eps);
-        const bool key = h >= a.nq;
+      if constexpr (KIND != V) {
+        // gu = R^T g; with n = x r, mean(gu w n) = r mean(gu w x), so both sums go over the lanes together
+        float ul[NP][VEC], uh[NP][VEC], ss = 0.f, dot = 0.f;
 #pragma unroll
         for (int i = 0; i < NP; ++i)
 #pragma unroll
           for (int v = 0; v < VEC; ++v) {
-            const float ul = lo[u][i].at(v) * r * (key ? wl[1][i][v] : wl[0][i][v]);
-            const float uh = hi[u][i].at(v) * r * (key ? wh[1][i][v] : wh[0][i][v]);
-            lo[u][i].set(v, ul * c[i][v] - uh * s[i][v]);
-            hi[u][i].set(v, uh * c[i][v] + ul * s[i][v]);
+            const float p = xl[u][i].at(v), q = xh[u][i].at(v), e = gl[u][i].at(v), f = gh[u][i].at(v);
+            ul[i][v] = e * c[i][v] + f * s[i][v];
+            uh[i][v] = f * c[i][v] - e * s[i][v];
+            ss = fmaf(p, p, fmaf(q, q, ss));
+            dot = fmaf(ul[i][v] * wl[i][v], p, fmaf(uh[i][v] * wh[i][v], q, dot));
+          }
+        ss = group_sum(ss, a.lanes);
+        dot = group_sum(dot, a.lanes);
+        const float r = rsqrtf(ss * inv_hd + a.eps), m = r * dot * inv_hd;  // m = mean(gu w n)
+#pragma unroll
+        for (int i = 0; i < NP; ++i)
+#pragma unroll
+          for (int v = 0; v < VEC; ++v) {
+            const float nl = xl[u][i].at(v) * r, nh = xh[u][i].at(v) * r;
+            gl[u][i].set(v, r * (ul[i][v] * wl[i][v] - nl * m));
+            gh[u][i].set(v, r * (uh[i][v] * wh[i][v] - nh * m));
+            // (heads past the run were loaded as zeros and add nothing)
+            dl[i][v] = fmaf(ul[i][v], nl, dl[i][v]);
+            dh[i][v] = fmaf(uh[i][v], nh, dh[i][v]);
           }
       }
-#pragma unroll
-      for (int i = 0; i < NP; ++i)
-        if (ln.on[i]) {
-          lo[u][i].store(y + (long)h * a.hd + ln.off[i]);
-          hi[u][i].store(y + (long)h * a.hd + half + ln.off[i]);
-        }
+      store_head(gl[u], gh[u], dx + (long)h * a.hd, half, ln, h < end);
     }
   }
 }
 
-template <typename T, int VEC, int NP>
-__global__ void __launch_bounds__(NT) qk_bwd_kernel(const Args a) {
+template <typename T, int VEC, int NP, int U>
+__global__ void __launch_bounds__(NT, VEC > 1 ? 2 : 1) qk_bwd_kernel(const Args a) {
   extern __shared__ float sh[];  // [NT / 32][2 hd]
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int half = a.hd >> 1, heads = a.nq + 2 * a.nkv, per = 32 / a.lanes;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, half = a.hd >> 1;
   const Lane<VEC, NP> ln(lane & (a.lanes - 1), a.lanes, half);
   const int grp = lane / a.lanes;
-  const float inv_hd = 1.f / (float)a.hd;
-  const int stride = per * a.split;
-  float wl[2][NP][VEC], wh[2][NP][VEC], dl[2][NP][VEC], dh[2][NP][VEC];
-  load_weight(a.wq, a.wdt, ln, half, wl[0], wh[0]);
-  load_weight(a.wk, a.wdt, ln, half, wl[1], wh[1]);
+  float dl[2][NP][VEC], dh[2][NP][VEC];
 #pragma unroll
   for (int t = 0; t < 2; ++t)
 #pragma unroll
@@ -211,69 +289,9 @@ __global__ void __launch_bounds__(NT) qk_bwd_kernel(const Args a) {
     T* dx = reinterpret_cast<T*>(a.out) + token * a.ldo;
     float c[NP][VEC], s[NP][VEC];
     load_table(a, ln, token, c, s, lane);
-    for (int h0 = part * per; h0 < heads; h0 += stride) {
-      const int h = h0 + grp;
-      const bool norm = h < a.nq + a.nkv;
-      Pack<T, VEC> xl[NP], xh[NP], gl[NP], gh[NP];
-#pragma unroll
-      for (int i = 0; i < NP; ++i) {
-        if (h < heads && ln.on[i]) {
-          gl[i].load(g + (long)h * a.hd + ln.off[i]);
-          gh[i].load(g + (long)h * a.hd + half + ln.off[i]);
-        } else {
-#pragma unroll
-          for (int v = 0; v < VEC; ++v) gl[i].set(v, 0.f), gh[i].set(v, 0.f);
-        }
-        if (norm && ln.on[i]) {
-          xl[i].load(x + (long)h * a.hd + ln.off[i]);
-          xh[i].load(x + (long)h * a.hd + half + ln.off[i]);
-        } else {
-#pragma unroll
-          for (int v = 0; v < VEC; ++v) xl[i].set(v, 0.f), xh[i].set(v, 0.f);
-        }
-      }
-      // one exchange for both sums: sum x^2 and sum gu w x (n = x r, so mean(gu w n) = r mean(gu w x))
-      float ss = 0.f, dot = 0.f;
-      const bool key = h >= a.nq;
-#pragma unroll
-      for (int i = 0; i < NP; ++i)
-#pragma unroll
-        for (int v = 0; v < VEC; ++v) {
-          const float p = xl[i].at(v), q = xh[i].at(v), e = gl[i].at(v), f = gh[i].at(v);
-          const float ul = e * c[i][v] + f * s[i][v], uh = f * c[i][v] - e * s[i][v];
-          ss = fmaf(p, p, fmaf(q, q, ss));
-          dot += ul * (key ? wl[1][i][v] : wl[0][i][v]) * p + uh * (key ? wh[1][i][v] : wh[0][i][v]) * q;
-        }
-      ss = group_sum(ss, a.lanes);
-      dot = group_sum(dot, a.lanes);
-      if (h >= heads) continue;
-      if (norm) {
-        const float r = rsqrtf(ss * inv_hd + a.eps);
-        const float m = r * dot * inv_hd;  // mean(gu w n)
-#pragma unroll
-        for (int i = 0; i < NP; ++i)
-#pragma unroll
-          for (int v = 0; v < VEC; ++v) {
-            const float nl = xl[i].at(v) * r, nh = xh[i].at(v) * r, e = gl[i].at(v), f = gh[i].at(v);
-            const float ul = e * c[i][v] + f * s[i][v], uh = f * c[i][v] - e * s[i][v];
-            gl[i].set(v, r * (ul * (key ? wl[1][i][v] : wl[0][i][v]) - nl * m));
-            gh[i].set(v, r * (uh * (key ? wh[1][i][v] : wh[0][i][v]) - nh * m));
-            if (key) {
-              dl[1][i][v] += ul * nl;
-              dh[1][i][v] += uh * nh;
-            } else {
-              dl[0][i][v] += ul * nl;
-              dh[0][i][v] += uh * nh;
-            }
-          }
-      }
-#pragma unroll
-      for (int i = 0; i < NP; ++i)
-        if (ln.on[i]) {
-          gl[i].store(dx + (long)h * a.hd + ln.off[i]);
-          gh[i].store(dx + (long)h * a.hd + half + ln.off[i]);
-        }
-    }
+    bwd_run<Q, T, VEC, NP, U>(a, x, g, dx, ln, grp, part, c, s, dl[0], dh[0]);
+    bwd_run<K, T, VEC, NP, U>(a, x, g, dx, ln, grp, part, c, s, dl[1], dh[1]);
+    bwd_run<V, T, VEC, NP, U>(a, x, g, dx, ln, grp, part, c, s, dl[0], dh[0]);
   }
   // the groups of a warp, then the warps of the block, in a fixed order
 #pragma unroll
@@ -332,8 +350,7 @@ using namespace dtb;
 
 namespace {
 
-// Fills what both directions share and chooses the lane layout: 16-byte vectors when the head is a
-// multiple of 16 elements and every row starts on a 16-byte boundary, single elements otherwise.
+// Fills what both directions share; whether the vector kernels apply (single elements otherwise).
 bool qk_common(qk::Args& a, const char* op, const torch::Tensor& x, const torch::Tensor& wq, const torch::Tensor& wk,
                const torch::Tensor& cos_t, const torch::Tensor& sin_t, const c10::optional<torch::Tensor>& pos,
                int64_t nq, int64_t nkv, int64_t hd, int64_t seqlen, double eps) {
@@ -369,8 +386,9 @@ bool qk_common(qk::Args& a, const char* op, const torch::Tensor& x, const torch:
   a.hd = (int)hd;
   a.eps = (float)eps;
   a.err = dtb_error_word();
-  const long es = (long)x.element_size();
-  return hd % 16 == 0 && (reinterpret_cast<uintptr_t>(a.x) & 15) == 0 && (a.ld * es) % 16 == 0 &&
+  // 4 elements at a time: a head of 8 n elements, every row on a boundary of 4 elements
+  const long es = (long)x.element_size(), bound = 4 * es;
+  return hd % 8 == 0 && hd <= 256 && reinterpret_cast<uintptr_t>(a.x) % bound == 0 && (a.ld * es) % bound == 0 &&
          (reinterpret_cast<uintptr_t>(a.cos_t) & 15) == 0 && (reinterpret_cast<uintptr_t>(a.sin_t) & 15) == 0;
 }
 
@@ -378,7 +396,7 @@ void qk_lanes(qk::Args& a, bool vec) {
   int lanes = 32;
   if (vec) {
     lanes = 1;
-    while (lanes * 16 < a.hd) lanes *= 2;
+    while (lanes * 8 < a.hd) lanes *= 2;
   }
   a.lanes = lanes;
   // few tokens: their heads are spread over more warps, down to one round of heads per warp
@@ -405,7 +423,7 @@ torch::Tensor qk_norm_rope_fwd(torch::Tensor x, torch::Tensor wq, torch::Tensor 
   DTB_CHECK(blocks < (1L << 31), "qk_norm_rope: too many tokens");
   auto st = at::cuda::getCurrentCUDAStream();
   DTB_FLOAT_TYPES(x.scalar_type(), {
-    if (vec) qk::qk_fwd_kernel<T, 8, 1, sizeof(T) == 4 ? 2 : 4><<<(unsigned)blocks, qk::NT, 0, st>>>(a);
+    if (vec) qk::qk_fwd_kernel<T, 4, 1, 4><<<(unsigned)blocks, qk::NT, 0, st>>>(a);
     else qk::qk_fwd_kernel<T, 1, 8, 1><<<(unsigned)blocks, qk::NT, 0, st>>>(a);
   });
   DTB_LAUNCH_CHECK();
@@ -435,17 +453,18 @@ torch::Tensor qk_norm_rope_bwd(torch::Tensor g, torch::Tensor x, torch::Tensor w
   a.ldg = g.stride(0);
   a.out = dx.data_ptr();
   a.ldo = dx.stride(0);
-  vec = vec && (reinterpret_cast<uintptr_t>(a.g) & 15) == 0 && (a.ldg * (long)x.element_size()) % 16 == 0;
+  const long bound = 4 * (long)x.element_size();
+  vec = vec && reinterpret_cast<uintptr_t>(a.g) % bound == 0 && (a.ldg * (long)x.element_size()) % bound == 0;
   qk_lanes(a, vec);
   const int warps = qk::NT / 32;
-  const int blocks = (int)std::min<long>((a.tokens * a.split + warps - 1) / warps, (long)device_sm_count() * 2);
+  const int blocks = (int)std::min<long>((a.tokens * a.split + warps - 1) / warps, (long)device_sm_count() * 2);  // one wave: two blocks an SM
   auto part = torch::empty({blocks, 2 * hd}, x.options().dtype(at::kFloat));
   a.part = part.data_ptr<float>();
   auto st = at::cuda::getCurrentCUDAStream();
   const size_t smem = sizeof(float) * warps * 2 * hd;
   DTB_FLOAT_TYPES(x.scalar_type(), {
-    if (vec) qk::qk_bwd_kernel<T, 8, 1><<<blocks, qk::NT, smem, st>>>(a);
-    else qk::qk_bwd_kernel<T, 1, 8><<<blocks, qk::NT, smem, st>>>(a);
+    if (vec) qk::qk_bwd_kernel<T, 4, 1, sizeof(T) == 4 ? 2 : 4><<<blocks, qk::NT, smem, st>>>(a);
+    else qk::qk_bwd_kernel<T, 1, 8, 1><<<blocks, qk::NT, smem, st>>>(a);
   });
   DTB_LAUNCH_CHECK();
   qk::qk_dw_reduce_kernel<<<(unsigned)((2 * hd + 31) / 32), 1024, 0, st>>>(

@@ -108,7 +108,7 @@ struct FwdArgs {
   float* entropy;
   float* top_v;      // [M, k]
   int64_t* top_i;    // [M, k]
-  float4* state;     // [M]
+  float4* state;     // [M], or null when nothing will ask for the gradient
   int* err;
 };
 
@@ -157,7 +157,7 @@ __global__ void __launch_bounds__(NT) logprob_fwd_kernel(const FwdArgs a, int cs
       if (tid == 0) {
         a.logprob[row] = 0.f;
         a.entropy[row] = 0.f;
-        a.state[row] = make_float4(0.f, 0.f, 0.f, __int_as_float(ROW_ZERO));
+        if (a.state) a.state[row] = make_float4(0.f, 0.f, 0.f, __int_as_float(ROW_ZERO));
       }
       if (TOP && tid < a.top_k) {
         a.top_v[row * a.top_k + tid] = -INFINITY;
@@ -310,7 +310,7 @@ __global__ void __launch_bounds__(NT) logprob_fwd_kernel(const FwdArgs a, int cs
       const float ent = ln_s - acc.a / acc.s / kLog2e;
       a.logprob[row] = bad ? nan : empty ? -INFINITY : (xt - acc.m) * a.invT - ln_s;
       a.entropy[row] = bad ? nan : empty ? 0.f : ent;
-      a.state[row] = make_float4(acc.m, log2f(acc.s), ent, __int_as_float(bad ? ROW_NAN : empty ? ROW_ZERO : ROW_OK));
+      if (a.state) a.state[row] = make_float4(acc.m, log2f(acc.s), ent, __int_as_float(bad ? ROW_NAN : empty ? ROW_ZERO : ROW_OK));
     }
     if (TOP && lane < a.top_k) {
       a.top_v[row * a.top_k + lane] = bad ? nan : empty ? -INFINITY : (key_value(list) - acc.m) * a.invT - ln_s;
@@ -370,11 +370,7 @@ __global__ void __launch_bounds__(256) logprob_bwd_kernel(const BwdArgs a) {
       o.set(e, d);
     }
     if (whole) {
-      if constexpr (VEC * sizeof(TO) == 8) {
-        *reinterpret_cast<uint2*>(dx + e0) = *reinterpret_cast<const uint2*>(&o.e[0]);
-      } else {
-        o.store(dx + e0);
-      }
+      o.store(dx + e0);
     } else {
 #pragma unroll
       for (int e = 0; e < VEC; ++e)
@@ -411,17 +407,26 @@ static void lp_check_logits(const char* op, const torch::Tensor& x, const torch:
   DTB_CHECK(temperature > 0, "%s: temperature must be positive", op);
 }
 
-// -> {logprob [M], entropy [M], state [M, 4], top log probabilities [M, k], top tokens [M, k]}
+// x [M, V], tokens of any shape with M entries -> {logprob, entropy} of the tokens' shape, then {top log
+// probabilities, top tokens} of that shape and k when top_k > 0, then the backward's state [M, 4] if asked for.
 std::vector<torch::Tensor> token_logprobs_fwd(torch::Tensor x, torch::Tensor tokens, double temperature, int64_t top_k,
-                                              int64_t ignore) {
+                                              int64_t ignore, bool want_state) {
   lp_check_logits("token_log_probs", x, tokens, temperature);
   DTB_CHECK(top_k >= 0 && top_k <= lp::MAX_TOP && top_k <= x.size(1), "token_log_probs: top_k must lie in [0, %d] and not exceed the vocabulary", lp::MAX_TOP);
   const c10::cuda::CUDAGuard guard(x.device());
   const long M = x.size(0);
-  auto f32 = x.options().dtype(at::kFloat);
-  auto logprob = torch::empty({M}, f32), entropy = torch::empty({M}, f32), state = torch::empty({M, 4}, f32);
-  auto top_v = torch::empty({M, top_k}, f32), top_i = torch::empty({M, top_k}, tokens.options());
-  if (M == 0) return {logprob, entropy, state, top_v, top_i};
+  auto f32 = x.options().dtype(at::kFloat).requires_grad(false);
+  std::vector<torch::Tensor> r;
+  r.push_back(torch::empty(tokens.sizes(), f32));
+  r.push_back(torch::empty(tokens.sizes(), f32));
+  if (top_k > 0) {
+    auto shape = tokens.sizes().vec();
+    shape.push_back(top_k);
+    r.push_back(torch::empty(shape, f32));
+    r.push_back(torch::empty(shape, tokens.options()));
+  }
+  if (want_state) r.push_back(torch::empty({M, 4}, f32));
+  if (M == 0) return r;
   lp::FwdArgs a{};
   a.x = x.data_ptr();
   a.ld = x.stride(0);
@@ -430,11 +435,13 @@ std::vector<torch::Tensor> token_logprobs_fwd(torch::Tensor x, torch::Tensor tok
   a.V = (int)x.size(1);
   a.invT = (float)(1.0 / temperature);
   a.top_k = (int)top_k;
-  a.logprob = logprob.data_ptr<float>();
-  a.entropy = entropy.data_ptr<float>();
-  a.top_v = top_v.data_ptr<float>();
-  a.top_i = top_i.data_ptr<int64_t>();
-  a.state = reinterpret_cast<float4*>(state.data_ptr<float>());
+  a.logprob = r[0].data_ptr<float>();
+  a.entropy = r[1].data_ptr<float>();
+  if (top_k > 0) {
+    a.top_v = r[2].data_ptr<float>();
+    a.top_i = r[3].data_ptr<int64_t>();
+  }
+  if (want_state) a.state = reinterpret_cast<float4*>(r.back().data_ptr<float>());
   a.err = dtb_error_word();
   // One block of 512 threads per row; short rows take 128.  When the rows do not fill the machine a
   // cluster of blocks shares each row, as long as every block keeps a few vectors per thread.
@@ -450,7 +457,7 @@ std::vector<torch::Tensor> token_logprobs_fwd(torch::Tensor x, torch::Tensor tok
     else lp::launch_fwd<T, 512>(a, M, csize, top_k > 0, st);
   });
   DTB_LAUNCH_CHECK();
-  return {logprob, entropy, state, top_v, top_i};
+  return r;
 }
 
 // Gradient of the logits into dx ([M, V], the logits' type or bf16, contiguous columns).

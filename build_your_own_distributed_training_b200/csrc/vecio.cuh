@@ -25,14 +25,16 @@ __device__ __forceinline__ __nv_bfloat16 from_float<__nv_bfloat16>(float v) { re
 template <>
 __device__ __forceinline__ __half from_float<__half>(float v) { return __float2half_rn(v); }
 
-// VEC consecutive elements as they lie in memory: 16-byte words where VEC * sizeof(T) is a
-// multiple of 16 (the address must then be 16-byte aligned), single elements otherwise.
+// VEC consecutive elements as they lie in memory: moved as 16-byte words (8-byte ones where the elements fill
+// just that; the address must be aligned alike) or else one by one.
 template <typename T, int VEC>
 struct Pack {
-  static constexpr bool WIDE = (VEC * sizeof(T)) % 16 == 0;
-  static constexpr int WORDS = WIDE ? (int)(VEC * sizeof(T) / 16) : 1;
+  static constexpr int BYTES = VEC * (int)sizeof(T);
+  static constexpr bool WIDE = BYTES % 16 == 0, HALF = BYTES == 8;
+  static constexpr int WORDS = WIDE ? BYTES / 16 : 1;
   union {
     uint4 w[WORDS];
+    uint2 h;
     T e[VEC];
   };
   __device__ __forceinline__ Pack() {}
@@ -40,6 +42,8 @@ struct Pack {
     if constexpr (WIDE) {
 #pragma unroll
       for (int i = 0; i < WORDS; ++i) w[i] = __ldg(reinterpret_cast<const uint4*>(p) + i);
+    } else if constexpr (HALF) {
+      h = __ldg(reinterpret_cast<const uint2*>(p));
     } else {
 #pragma unroll
       for (int i = 0; i < VEC; ++i) e[i] = p[i];
@@ -49,6 +53,8 @@ struct Pack {
     if constexpr (WIDE) {
 #pragma unroll
       for (int i = 0; i < WORDS; ++i) reinterpret_cast<uint4*>(p)[i] = w[i];
+    } else if constexpr (HALF) {
+      *reinterpret_cast<uint2*>(p) = h;
     } else {
 #pragma unroll
       for (int i = 0; i < VEC; ++i) p[i] = e[i];

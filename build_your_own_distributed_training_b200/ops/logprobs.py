@@ -122,12 +122,10 @@ def token_log_probs(logits: torch.Tensor, tokens: torch.Tensor, *, temperature: 
     """
     V = logits.shape[-1]
     _check(tokens, logits.shape[:-1], V, temperature, top_k)
-    x = logits if logits.dim() == 2 else logits.reshape(-1, V)
-    if x.stride(1) != 1:
-        x = x.contiguous()
-    apply = native().token_logprobs if x.is_cuda else _TokenLogProbsFn.apply
-    lp, ent, top_v, top_i = apply(x, tokens.reshape(-1).contiguous(), float(temperature), int(top_k),
-                                  int(ignore_index))
+    if logits.is_cuda:
+        return TokenLogProbs(*native().token_logprobs(logits, tokens, temperature, top_k, ignore_index))
+    lp, ent, top_v, top_i = _TokenLogProbsFn.apply(logits.reshape(-1, V), tokens.reshape(-1), float(temperature),
+                                                   int(top_k), int(ignore_index))
     return _shaped(lp, ent, top_v, top_i, tokens.shape, top_k)
 
 
@@ -148,11 +146,13 @@ class _HeadLogProbsFn(torch.autograd.Function):
         outs = []
         for r0, r1 in _row_blocks(h.shape[0], w.shape[0]):
             logits = gemm.mm_nt(h[r0:r1], w, out_dtype=torch.float32)
-            outs.append(native().token_logprobs_fwd(logits, tokens[r0:r1], temperature, top_k, ignore))
-        lp, ent, state, top_v, top_i = (torch.cat(t) if len(outs) > 1 else t[0] for t in zip(*outs))
+            outs.append(native().token_logprobs_fwd(logits, tokens[r0:r1], temperature, top_k, ignore, True))
+        lp, ent, *top, state = (torch.cat(t) if len(outs) > 1 else t[0] for t in zip(*outs))
+        top_v, top_i = top or (None, None)
         ctx.save_for_backward(h, w, tokens, state)
         ctx.temperature, ctx.main_grad = temperature, main_grad
-        ctx.mark_non_differentiable(top_v, top_i)
+        if top:
+            ctx.mark_non_differentiable(*top)
         ctx.set_materialize_grads(False)
         return lp, ent, top_v, top_i
 
