@@ -19,6 +19,7 @@ std::vector<Tensor> token_logprobs_fwd(Tensor x, Tensor tokens, double temperatu
                                        bool want_state);
 void token_logprobs_bwd(Tensor x, Tensor tokens, Tensor state, c10::optional<Tensor> g_lp, c10::optional<Tensor> g_ent,
                         double temperature, Tensor dx);
+std::vector<Tensor> fp8_quantize_with_tiles(Tensor x, Tensor s, int64_t rows);
 std::vector<Tensor> fp8_quantize(Tensor x, bool square, bool plain, bool transposed);
 void fp8_product(Tensor A, Tensor sA, c10::optional<Tensor> tA, Tensor B, Tensor sB, c10::optional<Tensor> tB, Tensor D,
                  c10::optional<Tensor> R, bool accumulate);
@@ -155,8 +156,8 @@ Tensor linear_fp8_autograd(Tensor x, Tensor w, c10::optional<Tensor> residual) {
 // x [T, K] bf16 with weights kept in 8 bits: values [N, K] e4m3, scales e8m0, their tiles or none
 Tensor linear_fp8_kept(Tensor x, Tensor values, Tensor scales, c10::optional<Tensor> tiles,
                        c10::optional<Tensor> residual) {
-  auto xq = fp8_quantize(x, false, true, false);
+  auto xq = tiles.has_value() ? fp8_quantize(x, false, true, false) : fp8_quantize_with_tiles(x, scales, values.size(0));
   Tensor y = torch::empty({x.size(0), values.size(0)}, x.options());
-  fp8_product(xq[0], xq[1], xq[2], values, scales, tiles, y, residual, false);
+  fp8_product(xq[0], xq[1], xq[2], values, scales, tiles.has_value() ? tiles : xq[3], y, residual, false);
   return y;
 }

@@ -38,6 +38,7 @@
 #include <algorithm>
 
 #include "common.cuh"
+#include "fp8.cuh"
 #include "vecio.cuh"
 
 namespace dtb {
@@ -59,7 +60,6 @@ struct GemmArgs {
 };
 
 constexpr int BM = 128, BK = 128, STAGES = 6, GROUP_M = 16;
-constexpr int SF_STEP = 4;   // stages that a scale tile serves
 constexpr int SF_SLOTS = 8;  // places in tensor memory: a slot comes round after 8 stages at least, when the MMAs
                              // of the ring's 6 earlier ones have been waited for
 constexpr uint32_t TMEM_COLS = 512, SF_COL = 256;
@@ -278,6 +278,8 @@ __global__ void __launch_bounds__(320, 1)
   __syncthreads();
   if constexpr (PAIR) cluster_sync();  // the peer's barriers exist before any remote arrive
   tc_fence_after();
+  let_successor_start();
+  wait_for_predecessor();
   // all 512 columns are allocated, so the allocation starts at column 0: a constant base keeps the
   // addresses below warp-uniform
   if (*tmem_holder != 0 && threadIdx.x == 0) atomicExch(args.err, ERR_BAD_ARG);
@@ -454,24 +456,15 @@ __global__ void __launch_bounds__(320, 1)
   }
 }
 
-// Scale tiles of a plain e8m0 scale tensor [row groups, k blocks] (strides in bytes): one block of 128
-// threads per tile, thread r its row.  Blocks past K get scale 1.
-__global__ void __launch_bounds__(128) scale_tiles_kernel(const uint8_t* __restrict__ s, long row_stride, long blk_stride,
-                                                          int gran, int rows, int kb, int kq, uint32_t* __restrict__ tiles) {
-  const int mt = blockIdx.x / kq, k = blockIdx.x % kq * SF_STEP, r = threadIdx.x;
-  const int row = min(mt * 128 + r, rows - 1);
-  const uint8_t* p = s + (long)(gran == 1 ? row : mt) * row_stride + k * blk_stride;
-  uint32_t w = 0;
-#pragma unroll
-  for (int i = 0; i < SF_STEP; ++i) w |= (k + i < kb ? (uint32_t)p[i * blk_stride] : 127u) << (8 * i);
-  tiles[(long)blockIdx.x * 128 + (r & 31) * 4 + (r >> 5)] = w;
+__global__ void __launch_bounds__(128) scale_tiles_kernel(const TileJob t) {
+  let_successor_start();
+  make_tile_word(t, blockIdx.x, threadIdx.x);
 }
 
 // D = sum over the parts of K, in part order (+ R): parts [splits, M, N] fp32.
 __global__ void __launch_bounds__(256) join_parts_kernel(const float* __restrict__ parts, int splits, int M, int N, void* D,
                                                          long ldd, const __nv_bfloat16* R, long ldr, int out) {
-  // launched so that it may start before the product has ended: the parts are there after this
-  asm volatile("griddepcontrol.wait;" ::: "memory");
+  wait_for_predecessor();
   const long i = (long)blockIdx.x * 256 + threadIdx.x, mn = (long)M * N;
   if (i >= mn) return;
   const long row = i / N, col = i - row * N;
@@ -561,7 +554,13 @@ static void launch(const CUtensorMap* t, GemmArgs& g, cudaStream_t st) {
   using L = Smem<BN, PAIR>;
   constexpr int CTAS = PAIR ? 2 : 1;
   auto kern = fp8_gemm_kernel<BN, PAIR, OUT>;
-  DTB_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, L::TOTAL));
+  static bool configured[64] = {false};
+  int dev = 0;
+  DTB_CUDA(cudaGetDevice(&dev));
+  if (dev >= 64 || !configured[dev]) {
+    DTB_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, L::TOTAL));
+    if (dev < 64) configured[dev] = true;
+  }
   g.m_blocks = (g.M + CTAS * BM - 1) / (CTAS * BM);
   g.n_blocks = (g.N + BN - 1) / BN;
   g.num_tiles = g.m_blocks * g.n_blocks;
@@ -570,13 +569,15 @@ static void launch(const CUtensorMap* t, GemmArgs& g, cudaStream_t st) {
   cfg.blockDim = dim3(320, 1, 1);
   cfg.dynamicSmemBytes = L::TOTAL;
   cfg.stream = st;
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeClusterDimension;
-  attr[0].val.clusterDim.x = CTAS;
-  attr[0].val.clusterDim.y = 1;
-  attr[0].val.clusterDim.z = 1;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = CTAS;
+  attr[1].val.clusterDim.y = 1;
+  attr[1].val.clusterDim.z = 1;
   cfg.attrs = attr;
-  cfg.numAttrs = PAIR ? 1 : 0;
+  cfg.numAttrs = PAIR ? 2 : 1;
   DTB_CUDA(cudaLaunchKernelEx(&cfg, kern, t[0], t[1], t[2], t[3], g));
 }
 
@@ -690,9 +691,9 @@ torch::Tensor fp8_scale_tiles(torch::Tensor s, int64_t gran, int64_t rows) {
   DTB_CHECK(mt * kq < (1L << 31), "fp8_scale_tiles: too large");
   auto t = torch::empty({mt, kq, 512}, s.options().dtype(at::kByte));
   if (mt * kq == 0) return t;
-  fp8::scale_tiles_kernel<<<(unsigned)(mt * kq), 128, 0, at::cuda::getCurrentCUDAStream()>>>(
-      reinterpret_cast<const uint8_t*>(s.data_ptr()), s.stride(0), s.stride(1), (int)gran, (int)rows, (int)kb, (int)kq,
-      reinterpret_cast<uint32_t*>(t.data_ptr()));
+  const fp8::TileJob job{reinterpret_cast<const uint8_t*>(s.data_ptr()), s.stride(0), s.stride(1), (int)gran, (int)rows,
+                         (int)kb, (int)kq, reinterpret_cast<uint32_t*>(t.data_ptr()), (int)(mt * kq)};
+  fp8::scale_tiles_kernel<<<(unsigned)job.count, 128, 0, at::cuda::getCurrentCUDAStream()>>>(job);
   DTB_LAUNCH_CHECK();
   return t;
 }

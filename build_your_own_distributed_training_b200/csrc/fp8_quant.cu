@@ -24,6 +24,7 @@
 #include <algorithm>
 
 #include "common.cuh"
+#include "fp8.cuh"
 #include "vecio.cuh"
 
 namespace dtb {
@@ -155,6 +156,7 @@ __device__ __forceinline__ void transpose4(uint32_t a0, uint32_t a1, uint32_t a2
 // One 128 x 128 tile per block of 256 threads: thread (rg, cg) holds rows rg * 8 + i, columns cg * 8 + k.
 template <typename T, bool SQUARE, bool WIDE>
 __global__ void __launch_bounds__(256, sizeof(T) == 2 ? 3 : 2) quant_tile_kernel(const QuantArgs a) {
+  let_successor_start();
   __shared__ __align__(16) uint8_t sh[128 * 128];
   __shared__ __align__(16) uint32_t colmax[8][128];
   const int tid = threadIdx.x, cg = tid & 15, rg = tid >> 4, warp = tid >> 5, lane = tid & 31;
@@ -269,9 +271,17 @@ __global__ void __launch_bounds__(256, sizeof(T) == 2 ? 3 : 2) quant_tile_kernel
   }
 }
 
-// A few rows alone (1 x 128, codes as they lie): 16 lanes per block of 128.
+// A few rows alone (1 x 128, codes as they lie): 16 lanes per block of 128.  Blocks from `quant_blocks` on make
+// the scale tiles of the other operand, so that a few tokens against kept weights need one launch before the
+// product.
 template <typename T, bool WIDE>
-__global__ void __launch_bounds__(256) quant_rows_kernel(const QuantArgs a) {
+__global__ void __launch_bounds__(256) quant_rows_kernel(const QuantArgs a, int quant_blocks, const TileJob job) {
+  let_successor_start();
+  if ((int)blockIdx.x >= quant_blocks) {
+    const int t = ((int)blockIdx.x - quant_blocks) * 2 + (threadIdx.x >> 7);
+    if (t < job.count) make_tile_word(job, t, threadIdx.x & 127);
+    return;
+  }
   const int cb = (a.C + 127) / 128;
   const int item = blockIdx.x * 16 + (threadIdx.x >> 4), cg = threadIdx.x & 15;  // (row, block) pair
   const bool live = item < a.R * cb;
@@ -308,7 +318,7 @@ using namespace dtb;
 // square: 128 x 128 blocks, scales [R/128, C/128] and their transpose; else 1 x 128 along the last axis of
 // each output, scales [R, C/128] and [C, R/128] (block-major in memory).  Codes lie in rows padded to 16
 // bytes.  `plain` / `transposed` select which of the two are made (undefined tensors stand for the other).
-std::vector<torch::Tensor> fp8_quantize(torch::Tensor x, bool square, bool plain, bool transposed) {
+static std::vector<torch::Tensor> quantize(torch::Tensor x, bool square, bool plain, bool transposed, fp8::TileJob job) {
   DTB_CHECK(x.is_cuda() && x.dim() == 2 && is_float_type(x.scalar_type()) && (x.numel() == 0 || x.size(1) == 1 || x.stride(1) == 1), "fp8_quantize: x must be a 2-D CUDA tensor of fp32, bf16 or fp16 with contiguous columns");
   DTB_CHECK(plain || transposed, "fp8_quantize: nothing asked for");
   DTB_CHECK(x.size(0) < (1L << 31) - 256 && x.size(1) < (1L << 31) - 256, "fp8_quantize: too large");
@@ -366,10 +376,33 @@ std::vector<torch::Tensor> fp8_quantize(torch::Tensor x, bool square, bool plain
       if (wide) fp8::quant_tile_kernel<T, false, true><<<grid, 256, 0, stream>>>(a);
       else fp8::quant_tile_kernel<T, false, false><<<grid, 256, 0, stream>>>(a);
     } else {
-      if (wide) fp8::quant_rows_kernel<T, true><<<items, 256, 0, stream>>>(a);
-      else fp8::quant_rows_kernel<T, false><<<items, 256, 0, stream>>>(a);
+      const unsigned n = items + (unsigned)((job.count + 1) / 2);
+      if (wide) fp8::quant_rows_kernel<T, true><<<n, 256, 0, stream>>>(a, (int)items, job);
+      else fp8::quant_rows_kernel<T, false><<<n, 256, 0, stream>>>(a, (int)items, job);
     }
   });
   DTB_LAUNCH_CHECK();
   return {q, s, t, qt, st, tt};
+}
+
+std::vector<torch::Tensor> fp8_quantize(torch::Tensor x, bool square, bool plain, bool transposed) {
+  return quantize(x, square, plain, transposed, fp8::TileJob{});
+}
+
+// fp8_quantize of x's rows, and in the same launch (under 128 rows) the scale tiles of `rows` rows of codes with
+// the plain scales s: {codes, scales, tiles of x, tiles of s}.
+torch::Tensor fp8_scale_tiles(torch::Tensor s, int64_t gran, int64_t rows);
+std::vector<torch::Tensor> fp8_quantize_with_tiles(torch::Tensor x, torch::Tensor s, int64_t rows) {
+  const long mt = (rows + 127) / 128;
+  const int64_t gran = s.dim() == 2 && s.size(0) == mt ? 128 : 1;
+  if (x.dim() != 2 || x.size(0) == 0 || x.size(0) >= 128 || x.size(1) == 0 || rows == 0) {
+    auto q = quantize(x, false, true, false, fp8::TileJob{});
+    return {q[0], q[1], q[2], fp8_scale_tiles(s, gran, rows)};
+  }
+  const long kb = (x.size(1) + 127) / 128, kq = (kb + fp8::SF_STEP - 1) / fp8::SF_STEP;
+  DTB_CHECK(s.device() == x.device() && s.scalar_type() == at::kFloat8_e8m0fnu && s.dim() == 2 && s.size(0) == (rows + gran - 1) / gran && s.size(1) == kb && mt * kq < (1L << 31), "fp8: scales must be e8m0 [%ld or %ld, %ld] on x's device", (long)rows, mt, kb);
+  auto t = torch::empty({mt, kq, 512}, x.options().dtype(at::kByte));
+  auto q = quantize(x, false, true, false, fp8::TileJob{reinterpret_cast<const uint8_t*>(s.data_ptr()), s.stride(0), s.stride(1), (int)gran,
+                                                        (int)rows, (int)kb, (int)kq, reinterpret_cast<uint32_t*>(t.data_ptr()), (int)(mt * kq)});
+  return {q[0], q[1], q[2], t};
 }

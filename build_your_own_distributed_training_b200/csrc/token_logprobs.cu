@@ -29,6 +29,7 @@
 #include <torch/extension.h>
 
 #include <algorithm>
+#include <type_traits>
 
 #include "common.cuh"
 #include "vecio.cuh"
@@ -94,6 +95,61 @@ __device__ __forceinline__ unsigned long long warp_merge(unsigned long long k, u
 #pragma unroll
   for (int j = 16; j > 0; j >>= 1) k = exchange(k, j, (lane & j) == 0);
   return k;
+}
+
+// Two fp32 at a time (sm_100 add / mul / fma on register pairs): the forward's exponent and sums are bound by
+// instructions for 16-bit logits, where a vector brings 8 of them.
+typedef unsigned long long f2;
+__device__ __forceinline__ f2 pair(float a, float b) {
+  f2 r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ void unpair(f2 v, float& a, float& b) { asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(v)); }
+__device__ __forceinline__ f2 add2(f2 a, f2 b) {
+  f2 r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ f2 mul2(f2 a, f2 b) {
+  f2 r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ f2 fma2(f2 a, f2 b, f2 c) {
+  f2 r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+// (x0 - m) c and (x1 - m) c, at least kMinExp
+__device__ __forceinline__ f2 exponents(float x0, float x1, f2 neg_m, f2 c) {
+  float a, b;
+  unpair(mul2(add2(pair(x0, x1), neg_m), c), a, b);
+  return pair(fmaxf(a, kMinExp), fmaxf(b, kMinExp));
+}
+
+// largest element of a vector, NaN if one is
+template <typename T>
+__device__ __forceinline__ float vec_max(const Pack<T, 16 / sizeof(T)>& p) {
+  if constexpr (sizeof(T) == 4) {
+    return max_nan(max_nan(p.at(0), p.at(1)), max_nan(p.at(2), p.at(3)));
+  } else {
+    const uint4& w = p.w[0];
+    uint32_t a, b;
+    if constexpr (std::is_same<T, __nv_bfloat16>::value) {
+      asm("max.NaN.bf16x2 %0, %1, %2;" : "=r"(a) : "r"(w.x), "r"(w.y));
+      asm("max.NaN.bf16x2 %0, %1, %2;" : "=r"(b) : "r"(w.z), "r"(w.w));
+      asm("max.NaN.bf16x2 %0, %0, %1;" : "+r"(a) : "r"(b));
+    } else {
+      asm("max.NaN.f16x2 %0, %1, %2;" : "=r"(a) : "r"(w.x), "r"(w.y));
+      asm("max.NaN.f16x2 %0, %1, %2;" : "=r"(b) : "r"(w.z), "r"(w.w));
+      asm("max.NaN.f16x2 %0, %0, %1;" : "+r"(a) : "r"(b));
+    }
+    Pack<T, 2> q;
+    q.e[0] = reinterpret_cast<const T*>(&a)[0];
+    q.e[1] = reinterpret_cast<const T*>(&a)[1];
+    return max_nan(q.at(0), q.at(1));
+  }
 }
 
 struct FwdArgs {
@@ -172,7 +228,9 @@ __global__ void __launch_bounds__(NT) logprob_fwd_kernel(const FwdArgs a, int cs
   const int G = csize * NT, g = rank * NT + tid;
   const float c = a.invT * kLog2e;
 
-  Acc acc{-INFINITY, 0.f, 0.f};
+  float m = -INFINITY;
+  f2 s2 = pair(0.f, 0.f), a2 = s2;
+  const f2 c2 = pair(c, c);
   float best = -INFINITY;
   int best_i = -1;
   for (int j = g; j < nvec; j += U * G) {
@@ -186,11 +244,9 @@ __global__ void __launch_bounds__(NT) logprob_fwd_kernel(const FwdArgs a, int cs
         for (int e = 0; e < VEC; ++e) p[u].set(e, -INFINITY);
       }
     }
-    float cm = -INFINITY;
+    float cm = vec_max<T>(p[0]);
 #pragma unroll
-    for (int u = 0; u < U; ++u)
-#pragma unroll
-      for (int e = 0; e < VEC; ++e) cm = max_nan(cm, p[u].at(e));
+    for (int u = 1; u < U; ++u) cm = max_nan(cm, vec_max<T>(p[u]));
     if (TOP && (cm > best || best_i < 0)) {
       best = cm;
 #pragma unroll
@@ -201,21 +257,35 @@ __global__ void __launch_bounds__(NT) logprob_fwd_kernel(const FwdArgs a, int cs
           if (p[u].at(e) == cm && idx >= 0 && idx < a.V) best_i = idx;
         }
     }
-    const float mn = max_nan(acc.m, cm);
-    if (mn != acc.m) {
-      const float d = fmaxf((acc.m - mn) * c, kMinExp), f = ex2_approx(d);
-      acc.a = f * fmaf(d, acc.s, acc.a);
-      acc.s *= f;
-      acc.m = mn;
+    const float mn = max_nan(m, cm);
+    if (mn != m) {
+      const float d = fmaxf((m - mn) * c, kMinExp), f = ex2_approx(d);
+      const f2 f2v = pair(f, f);
+      a2 = mul2(f2v, fma2(pair(d, d), s2, a2));
+      s2 = mul2(f2v, s2);
+      m = mn;
     }
+    const f2 neg_m = pair(-mn, -mn);
 #pragma unroll
     for (int u = 0; u < U; ++u)
 #pragma unroll
-      for (int e = 0; e < VEC; ++e) {
-        const float t = fmaxf((p[u].at(e) - mn) * c, kMinExp), w = ex2_approx(t);
-        acc.s += w;
-        acc.a = fmaf(w, t, acc.a);
+      for (int e = 0; e < VEC; e += 2) {
+        const f2 t = exponents(p[u].at(e), p[u].at(e + 1), neg_m, c2);
+        float t0, t1;
+        unpair(t, t0, t1);
+        const f2 w = pair(ex2_approx(t0), ex2_approx(t1));
+        s2 = add2(s2, w);
+        a2 = fma2(w, t, a2);
       }
+  }
+  Acc acc;
+  acc.m = m;
+  {
+    float x0, x1;
+    unpair(s2, x0, x1);
+    acc.s = x0 + x1;
+    unpair(a2, x0, x1);
+    acc.a = x0 + x1;
   }
   // threads -> warp -> block -> cluster, in a fixed order
 #pragma unroll
@@ -337,7 +407,7 @@ struct BwdArgs {
 // WIDE: the row of x and the row of dx sit alike within their vectors
 template <typename T, typename TO, bool WIDE>
 __global__ void __launch_bounds__(256) logprob_bwd_kernel(const BwdArgs a) {
-  constexpr int VEC = WIDE ? 16 / sizeof(T) : 1;
+  constexpr int VEC = WIDE ? 16 / sizeof(T) : 1, U = 4;
   const long row = blockIdx.x / a.split;
   const int part = (int)(blockIdx.x % a.split);
   const T* x = reinterpret_cast<const T*>(a.x) + row * a.ld;
@@ -349,32 +419,49 @@ __global__ void __launch_bounds__(256) logprob_bwd_kernel(const BwdArgs a) {
   const float gl = a.g_lp ? a.g_lp[row] * a.invT : 0.f, ge = a.g_ent ? a.g_ent[row] * a.invT : 0.f;
   const float c = a.invT * kLog2e, m = st.x, l2s = st.y, ent = st.z;
   const long tok = a.tokens[row];
+  // d = p (g0 + g1 log2 p) + [i = tok] gl
+  const float g0 = -fmaf(ge, ent, gl), g1 = -ge / kLog2e;
   const int first = part * 256 + threadIdx.x, step = a.split * 256;
-  for (int j = first; j < nvec; j += step) {
-    const int e0 = j * VEC - shift;
-    Pack<T, VEC> p;
-    Pack<TO, VEC> o;
-    const bool whole = e0 >= 0 && e0 + VEC <= a.V;
-    if (kind == ROW_OK) {
-      if constexpr (WIDE) load_vec<T>(p, x, j, shift, a.V);
-      else p.load(x + e0);
-    }
+  for (int j0 = first; j0 < nvec; j0 += U * step) {
+    Pack<T, VEC> p[U];
 #pragma unroll
-    for (int e = 0; e < VEC; ++e) {
-      float d = kind == ROW_ZERO ? 0.f : __int_as_float(0x7fc00000);
-      if (kind == ROW_OK) {
-        const float t = fmaxf((p.at(e) - m) * c, kMinExp) - l2s;  // log2 p
-        const float pr = ex2_approx(t);
-        d = -pr * (gl + ge * fmaf(t, 1.f / kLog2e, ent)) + (e0 + e == tok ? gl : 0.f);
+    for (int u = 0; u < U; ++u) {
+      const int j = j0 + u * step;
+      if (kind == ROW_OK && j < nvec) {
+        if constexpr (WIDE) load_vec<T>(p[u], x, j, shift, a.V);
+        else p[u].load(x + j);
       }
-      o.set(e, d);
     }
-    if (whole) {
-      o.store(dx + e0);
-    } else {
 #pragma unroll
-      for (int e = 0; e < VEC; ++e)
-        if (e0 + e >= 0 && e0 + e < a.V) dx[e0 + e] = o.e[e];
+    for (int u = 0; u < U; ++u) {
+      const int j = j0 + u * step, e0 = j * VEC - shift;
+      if (j >= nvec) break;
+      Pack<TO, VEC> o;
+      if (kind == ROW_OK) {
+        float d[VEC];
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) {
+          const float t = fmaxf((p[u].at(e) - m) * c, kMinExp) - l2s;  // log2 p
+          d[e] = ex2_approx(t) * fmaf(g1, t, g0);
+        }
+        if (tok >= e0 && tok < e0 + VEC) {
+#pragma unroll
+          for (int e = 0; e < VEC; ++e)
+            if (e0 + e == tok) d[e] += gl;
+        }
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) o.set(e, d[e]);
+      } else {
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) o.set(e, kind == ROW_ZERO ? 0.f : __int_as_float(0x7fc00000));
+      }
+      if (e0 >= 0 && e0 + VEC <= a.V) {
+        o.store(dx + e0);
+      } else {
+#pragma unroll
+        for (int e = 0; e < VEC; ++e)
+          if (e0 + e >= 0 && e0 + e < a.V) dx[e0 + e] = o.e[e];
+      }
     }
   }
 }
