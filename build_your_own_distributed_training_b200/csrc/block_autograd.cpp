@@ -21,6 +21,8 @@ void token_logprobs_bwd(Tensor x, Tensor tokens, Tensor state, c10::optional<Ten
                         double temperature, Tensor dx);
 std::vector<Tensor> fp8_quantize_with_tiles(Tensor x, Tensor s, int64_t rows);
 std::vector<Tensor> fp8_quantize(Tensor x, bool square, bool plain, bool transposed);
+std::vector<Tensor> fp8_quantize_tiles(Tensor x, bool square, bool plain, bool transposed);
+void fp8_gemm(Tensor A, Tensor tA, Tensor B, Tensor tB, Tensor D, c10::optional<Tensor> R, bool accumulate);
 void fp8_product(Tensor A, Tensor sA, c10::optional<Tensor> tA, Tensor B, Tensor sB, c10::optional<Tensor> tB, Tensor D,
                  c10::optional<Tensor> R, bool accumulate);
 
@@ -95,11 +97,11 @@ struct TokenLogProbs : public Function<TokenLogProbs> {
 struct LinearFp8 : public Function<LinearFp8> {
   static Tensor forward(AutogradContext* ctx, const Tensor& x, const Tensor& w, const c10::optional<Tensor>& residual) {
     const bool need_x = x.requires_grad(), need_w = w.requires_grad();
-    auto xq = fp8_quantize(x, false, true, need_w);  // codes, scales, tiles; of the transpose: 3, 4, 5
-    auto wq = fp8_quantize(w, true, true, need_x);
+    auto xq = fp8_quantize_tiles(x, false, true, need_w);  // codes, scale tiles; of the transpose: 2, 3
+    auto wq = fp8_quantize_tiles(w, true, true, need_x);
     Tensor y = torch::empty({x.size(0), w.size(0)}, x.options());
-    fp8_product(xq[0], xq[1], xq[2], wq[0], wq[1], wq[2], y, residual, false);
-    ctx->save_for_backward({xq[3], xq[4], xq[5], wq[3], wq[4], wq[5]});
+    fp8_gemm(xq[0], xq[1], wq[0], wq[1], y, residual, false);
+    ctx->save_for_backward({xq[2], xq[3], wq[2], wq[3]});
     ctx->saved_data["t"] = w.scalar_type();
     ctx->saved_data["r"] = residual.has_value();
     return y;
@@ -110,15 +112,15 @@ struct LinearFp8 : public Function<LinearFp8> {
     Tensor dx, dw;
     if (need_x || need_w) {
       Tensor g = grads[0].contiguous();
-      auto gq = fp8_quantize(g, false, need_x, need_w);
+      auto gq = fp8_quantize_tiles(g, false, need_x, need_w);
       if (need_x) {
-        dx = torch::empty({g.size(0), s[3].size(0)}, g.options());
-        fp8_product(gq[0], gq[1], gq[2], s[3], s[4], s[5], dx, c10::nullopt, false);
+        dx = torch::empty({g.size(0), s[2].size(0)}, g.options());
+        fp8_gemm(gq[0], gq[1], s[2], s[3], dx, c10::nullopt, false);
       }
       if (need_w) {
         const auto t = ctx->saved_data["t"].toScalarType();
         dw = torch::empty({g.size(1), s[0].size(0)}, g.options().dtype(t == at::kHalf ? at::kFloat : t));
-        fp8_product(gq[3], gq[4], gq[5], s[0], s[1], s[2], dw, c10::nullopt, false);
+        fp8_gemm(gq[2], gq[3], s[0], s[1], dw, c10::nullopt, false);
         dw = dw.to(t);
       }
     }

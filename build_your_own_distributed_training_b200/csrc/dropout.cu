@@ -46,37 +46,50 @@ __device__ __forceinline__ uint32_t field(const uint4& r, int i) {
   return (i & 1) ? w >> 16 : w & 0xffffu;
 }
 
-// Group `first + t` of 8 consecutive element numbers per thread; element number minus `start` indexes
-// the tensors.  WIDE: start % 8 == 0 and 16-byte aligned bases, so full groups move as vectors.
-template <typename T, bool RES, bool WIDE>
+// Groups of 8 consecutive element numbers, U per thread (their loads go out together); an element's number
+// minus `start` indexes the tensors.  WIDE: start % 8 == 0 and 16-byte aligned bases, so whole groups move as
+// vectors.
+template <typename T, bool RES, bool WIDE, int U>
 __global__ void __launch_bounds__(NT) dropout_kernel(const T* __restrict__ x, const T* __restrict__ r,
                                                      T* __restrict__ y, uint64_t n, uint64_t start, uint64_t groups,
                                                      uint32_t k0, uint32_t k1, uint32_t cut, float scale) {
-  const uint64_t t = (uint64_t)blockIdx.x * NT + threadIdx.x;
-  if (t >= groups) return;
-  const uint64_t grp = (start >> 3) + t;
-  const int64_t base = (int64_t)(grp * 8 - start);  // may be negative in the first group
-  const bool whole = base >= 0 && (uint64_t)base + 8 <= n;
-  if (WIDE && whole) {
-    Pack<T, 8> px, pr;
-    px.load(x + base);
-    if (RES) pr.load(r + base);
-    const uint4 bits = philox(grp, k0, k1);
+  const uint64_t first = (uint64_t)blockIdx.x * (NT * U) + threadIdx.x;
+  Pack<T, 8> px[U], pr[U];
+  bool whole[U];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const float v = field(bits, i) >= cut ? px.at(i) * scale : 0.f;
-      px.set(i, RES ? pr.at(i) + v : v);
+  for (int u = 0; u < U; ++u) {
+    const uint64_t t = first + u * NT, grp = (start >> 3) + t;
+    const int64_t base = (int64_t)(grp * 8 - start);  // may be negative in the first group
+    whole[u] = WIDE && t < groups && base >= 0 && (uint64_t)base + 8 <= n;
+    if (whole[u]) {
+      px[u].load(x + base);
+      if (RES) pr[u].load(r + base);
     }
-    px.store(y + base);
-    return;
   }
-  const uint4 bits = philox(grp, k0, k1);
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    const int64_t e = base + i;
-    if (e < 0 || (uint64_t)e >= n) continue;
-    const float v = field(bits, i) >= cut ? as_float<T>(x[e]) * scale : 0.f;
-    y[e] = from_float<T>(RES ? as_float<T>(r[e]) + v : v);
+  for (int u = 0; u < U; ++u) {
+    const uint64_t t = first + u * NT, grp = (start >> 3) + t;
+    if (t >= groups) return;
+    const int64_t base = (int64_t)(grp * 8 - start);
+    const uint4 bits = philox(grp, k0, k1);
+    if (whole[u]) {
+      float f[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const float v = field(bits, i) >= cut ? px[u].at(i) * scale : 0.f;
+        f[i] = RES ? pr[u].at(i) + v : v;
+      }
+      px[u].set_all(f);
+      px[u].store(y + base);
+    } else {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const int64_t e = base + i;
+        if (e < 0 || (uint64_t)e >= n) continue;
+        const float v = field(bits, i) >= cut ? as_float<T>(x[e]) * scale : 0.f;
+        y[e] = from_float<T>(RES ? as_float<T>(r[e]) + v : v);
+      }
+    }
   }
 }
 
@@ -97,8 +110,6 @@ torch::Tensor dropout_add(torch::Tensor x, c10::optional<torch::Tensor> residual
   const uint64_t n = (uint64_t)x.numel(), s = (uint64_t)start;
   if (n == 0) return y;
   const uint64_t groups = (s + n + 7) / 8 - s / 8;
-  const uint64_t blocks = (groups + drop::NT - 1) / drop::NT;
-  DTB_CHECK(blocks < (1ull << 31), "dropout_add: too many elements");
   const float scale = cut < 65536 ? (float)(65536.0 / (double)(65536 - cut)) : 0.f;
   const uint32_t k0 = (uint32_t)(uint64_t)seed, k1 = (uint32_t)((uint64_t)seed >> 32);
   uintptr_t bases = reinterpret_cast<uintptr_t>(x.data_ptr()) | reinterpret_cast<uintptr_t>(y.data_ptr());
@@ -109,12 +120,18 @@ torch::Tensor dropout_add(torch::Tensor x, c10::optional<torch::Tensor> residual
     const T* xp = reinterpret_cast<const T*>(x.data_ptr());
     const T* rp = residual.has_value() ? reinterpret_cast<const T*>(residual->data_ptr()) : nullptr;
     T* yp = reinterpret_cast<T*>(y.data_ptr());
-    const unsigned nb = (unsigned)blocks;
     const uint32_t c = (uint32_t)cut;
-    if (rp && wide) drop::dropout_kernel<T, true, true><<<nb, drop::NT, 0, st>>>(xp, rp, yp, n, s, groups, k0, k1, c, scale);
-    else if (rp) drop::dropout_kernel<T, true, false><<<nb, drop::NT, 0, st>>>(xp, rp, yp, n, s, groups, k0, k1, c, scale);
-    else if (wide) drop::dropout_kernel<T, false, true><<<nb, drop::NT, 0, st>>>(xp, rp, yp, n, s, groups, k0, k1, c, scale);
-    else drop::dropout_kernel<T, false, false><<<nb, drop::NT, 0, st>>>(xp, rp, yp, n, s, groups, k0, k1, c, scale);
+    auto go = [&](auto kernel, int per) {
+      const uint64_t blocks = (groups + drop::NT * per - 1) / (drop::NT * per);
+      DTB_CHECK(blocks < (1ull << 31), "dropout_add: too many elements");
+      kernel<<<(unsigned)blocks, drop::NT, 0, st>>>(xp, rp, yp, n, s, groups, k0, k1, c, scale);
+    };
+    // two groups a thread once that still gives every SM its blocks
+    const bool deep = groups >= (uint64_t)device_sm_count() * drop::NT * 16;
+    if (rp && wide) deep ? go(drop::dropout_kernel<T, true, true, 2>, 2) : go(drop::dropout_kernel<T, true, true, 1>, 1);
+    else if (rp) go(drop::dropout_kernel<T, true, false, 1>, 1);
+    else if (wide) deep ? go(drop::dropout_kernel<T, false, true, 2>, 2) : go(drop::dropout_kernel<T, false, true, 1>, 1);
+    else go(drop::dropout_kernel<T, false, false, 1>, 1);
   });
   DTB_LAUNCH_CHECK();
   return y;

@@ -57,10 +57,10 @@ struct QuantArgs {
   int R, C;
   uint8_t* q;         // [R, q_ld] codes as they lie, or null
   long q_ld;
-  uint8_t* s;         // 1 x 128: [C / 128][R]; 128 x 128: [R / 128][C / 128]
+  uint8_t* s;         // 1 x 128: [C / 128][R]; 128 x 128: [R / 128][C / 128]; or null (tiles alone)
   uint8_t* qt;        // [C, qt_ld] transposed codes, or null
   long qt_ld;
-  uint8_t* st;        // 1 x 128 of the transpose: [R / 128][C]
+  uint8_t* st;        // 1 x 128 of the transpose: [R / 128][C], or null
   uint8_t* t;         // scale tiles of the codes as they lie: [R / 128][C / 512][512]
   uint8_t* tt;        // and of the transpose: [C / 128][R / 512][512]
 };
@@ -187,7 +187,7 @@ __global__ void __launch_bounds__(256, sizeof(T) == 2 ? 3 : 2) quant_tile_kernel
 #pragma unroll
     for (int w = 0; w < 8; ++w) m = max(m, colmax[0][w]);
     const uint8_t b = (uint8_t)scale_byte(m);
-    if (tid == 0) a.s[(long)blockIdx.y * gridDim.x + blockIdx.x] = b;
+    if (tid == 0 && a.s != nullptr) a.s[(long)blockIdx.y * gridDim.x + blockIdx.x] = b;
     if (tid < 128 && a.t != nullptr) a.t[blockIdx.y * tq * 512 + tile_byte(tid, blockIdx.x)] = b;
     if (tid >= 128 && a.tt != nullptr) a.tt[blockIdx.x * ttq * 512 + tile_byte(tid - 128, blockIdx.y)] = b;
     const float f = inv_scale(b);
@@ -217,7 +217,7 @@ __global__ void __launch_bounds__(256, sizeof(T) == 2 ? 3 : 2) quant_tile_kernel
       for (int i = 0; i < 8; ++i) {
         const uint32_t b = scale_byte(rmax[i]);
         if (cg == i) {
-          if (r0 + i < a.R) a.s[(long)blockIdx.x * a.R + r0 + i] = (uint8_t)b;
+          if (r0 + i < a.R && a.s != nullptr) a.s[(long)blockIdx.x * a.R + r0 + i] = (uint8_t)b;
           a.t[blockIdx.y * tq * 512 + tile_byte(rg * 8 + i, blockIdx.x)] = (uint8_t)b;
         }
         if (r0 + i < a.R && c0 < a.q_ld)
@@ -241,7 +241,7 @@ __global__ void __launch_bounds__(256, sizeof(T) == 2 ? 3 : 2) quant_tile_kernel
       for (int w = 0; w < 8; ++w) m = max(m, colmax[w][tid]);
       const uint32_t b = scale_byte(m);
       const int col = blockIdx.x * 128 + tid;
-      if (col < a.C) a.st[(long)blockIdx.y * a.C + col] = (uint8_t)b;
+      if (col < a.C && a.st != nullptr) a.st[(long)blockIdx.y * a.C + col] = (uint8_t)b;
       a.tt[blockIdx.x * ttq * 512 + tile_byte(tid, blockIdx.y)] = (uint8_t)b;
       colmax[0][tid] = __float_as_uint(inv_scale(b));
     }
@@ -303,7 +303,7 @@ __global__ void __launch_bounds__(256) quant_rows_kernel(const QuantArgs a, int 
   if (!live) return;
   const uint32_t b = scale_byte(m);
   if (cg == 0) {
-    a.s[(long)blk * a.R + row] = (uint8_t)b;
+    if (a.s != nullptr) a.s[(long)blk * a.R + row] = (uint8_t)b;
     a.t[tile_byte(row, blk)] = (uint8_t)b;  // fewer than 128 rows: one row block
   }
   if (c0 < a.q_ld) *reinterpret_cast<uint2*>(a.q + row * a.q_ld + c0) = codes8(v, inv_scale(b));
@@ -318,7 +318,8 @@ using namespace dtb;
 // square: 128 x 128 blocks, scales [R/128, C/128] and their transpose; else 1 x 128 along the last axis of
 // each output, scales [R, C/128] and [C, R/128] (block-major in memory).  Codes lie in rows padded to 16
 // bytes.  `plain` / `transposed` select which of the two are made (undefined tensors stand for the other).
-static std::vector<torch::Tensor> quantize(torch::Tensor x, bool square, bool plain, bool transposed, fp8::TileJob job) {
+static std::vector<torch::Tensor> quantize(torch::Tensor x, bool square, bool plain, bool transposed, fp8::TileJob job,
+                                           bool scales = true) {
   DTB_CHECK(x.is_cuda() && x.dim() == 2 && is_float_type(x.scalar_type()) && (x.numel() == 0 || x.size(1) == 1 || x.stride(1) == 1), "fp8_quantize: x must be a 2-D CUDA tensor of fp32, bf16 or fp16 with contiguous columns");
   DTB_CHECK(plain || transposed, "fp8_quantize: nothing asked for");
   DTB_CHECK(x.size(0) < (1L << 31) - 256 && x.size(1) < (1L << 31) - 256, "fp8_quantize: too large");
@@ -335,10 +336,10 @@ static std::vector<torch::Tensor> quantize(torch::Tensor x, bool square, bool pl
   if (transposed) tt = tiles(CB, RB);
   if (plain) q = codes(R, C);
   if (transposed) qt = codes(C, R);
-  if (square) {
+  if (square && scales) {
     s = torch::empty({RB, CB}, opts);
     st = s.t();
-  } else {
+  } else if (scales) {
     if (plain) s = torch::empty({CB, R}, opts).t();
     if (transposed) st = torch::empty({RB, C}, opts).t();
   }
@@ -354,11 +355,11 @@ static std::vector<torch::Tensor> quantize(torch::Tensor x, bool square, bool pl
   }
   if (plain) a.t = t.data_ptr<uint8_t>();
   if (transposed) a.tt = tt.data_ptr<uint8_t>();
-  if (square || plain) a.s = reinterpret_cast<uint8_t*>(s.data_ptr());
+  if (scales && (square || plain)) a.s = reinterpret_cast<uint8_t*>(s.data_ptr());
   if (transposed) {
     a.qt = reinterpret_cast<uint8_t*>(qt.data_ptr());
     a.qt_ld = (R + 15) / 16 * 16;
-    if (!square) a.st = reinterpret_cast<uint8_t*>(st.data_ptr());
+    if (scales && !square) a.st = reinterpret_cast<uint8_t*>(st.data_ptr());
   }
   const bool wide = (reinterpret_cast<uintptr_t>(a.x) & 15) == 0 && (a.ld * (long)x.element_size()) % 16 == 0;
   auto stream = at::cuda::getCurrentCUDAStream();
@@ -405,4 +406,10 @@ std::vector<torch::Tensor> fp8_quantize_with_tiles(torch::Tensor x, torch::Tenso
   auto q = quantize(x, false, true, false, fp8::TileJob{reinterpret_cast<const uint8_t*>(s.data_ptr()), s.stride(0), s.stride(1), (int)gran,
                                                         (int)rows, (int)kb, (int)kq, reinterpret_cast<uint32_t*>(t.data_ptr()), (int)(mt * kq)});
   return {q[0], q[1], q[2], t};
+}
+
+// fp8_quantize without the plain scales: {codes, tiles, transposed codes, their tiles}.
+std::vector<torch::Tensor> fp8_quantize_tiles(torch::Tensor x, bool square, bool plain, bool transposed) {
+  auto q = quantize(x, square, plain, transposed, fp8::TileJob{}, false);
+  return {q[0], q[2], q[3], q[5]};
 }

@@ -184,13 +184,17 @@ __device__ __forceinline__ void fwd_run(const Args& a, const T* x, T* y, const L
           }
         const float r = rsqrtf(group_sum(ss, a.lanes) * inv_hd + a.eps);
 #pragma unroll
-        for (int i = 0; i < NP; ++i)
+        for (int i = 0; i < NP; ++i) {
+          float yl[VEC], yh[VEC];
 #pragma unroll
           for (int v = 0; v < VEC; ++v) {
             const float ul = lo[u][i].at(v) * r * wl[i][v], uh = hi[u][i].at(v) * r * wh[i][v];
-            lo[u][i].set(v, ul * c[i][v] - uh * s[i][v]);
-            hi[u][i].set(v, uh * c[i][v] + ul * s[i][v]);
+            yl[v] = ul * c[i][v] - uh * s[i][v];
+            yh[v] = uh * c[i][v] + ul * s[i][v];
           }
+          lo[u][i].set_all(yl);
+          hi[u][i].set_all(yh);
+        }
       }
       store_head(lo[u], hi[u], y + (long)h * a.hd, half, ln, h < end);
     }
@@ -251,16 +255,20 @@ __device__ __forceinline__ void bwd_run(const Args& a, const T* x, const T* g, T
         dot = group_sum(dot, a.lanes);
         const float r = rsqrtf(ss * inv_hd + a.eps), m = r * dot * inv_hd;  // m = mean(gu w n)
 #pragma unroll
-        for (int i = 0; i < NP; ++i)
+        for (int i = 0; i < NP; ++i) {
+          float al[VEC], ah[VEC];
 #pragma unroll
           for (int v = 0; v < VEC; ++v) {
             const float nl = xl[u][i].at(v) * r, nh = xh[u][i].at(v) * r;
-            gl[u][i].set(v, r * (ul[i][v] * wl[i][v] - nl * m));
-            gh[u][i].set(v, r * (uh[i][v] * wh[i][v] - nh * m));
+            al[v] = r * (ul[i][v] * wl[i][v] - nl * m);
+            ah[v] = r * (uh[i][v] * wh[i][v] - nh * m);
             // (heads past the run were loaded as zeros and add nothing)
             dl[i][v] = fmaf(ul[i][v], nl, dl[i][v]);
             dh[i][v] = fmaf(uh[i][v], nh, dh[i][v]);
           }
+          gl[u][i].set_all(al);
+          gh[u][i].set_all(ah);
+        }
       }
       store_head(gl[u], gh[u], dx + (long)h * a.hd, half, ln, h < end);
     }

@@ -449,8 +449,7 @@ __global__ void __launch_bounds__(256) logprob_bwd_kernel(const BwdArgs a) {
           for (int e = 0; e < VEC; ++e)
             if (e0 + e == tok) d[e] += gl;
         }
-#pragma unroll
-        for (int e = 0; e < VEC; ++e) o.set(e, d[e]);
+        o.set_all(d);
       } else {
 #pragma unroll
         for (int e = 0; e < VEC; ++e) o.set(e, kind == ROW_ZERO ? 0.f : __int_as_float(0x7fc00000));

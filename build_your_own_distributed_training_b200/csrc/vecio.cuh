@@ -5,6 +5,8 @@
 #include <cuda_fp16.h>
 #include <stdint.h>
 
+#include <type_traits>
+
 namespace dtb {
 
 template <typename T>
@@ -62,6 +64,31 @@ struct Pack {
   }
   __device__ __forceinline__ float at(int i) const { return as_float<T>(e[i]); }
   __device__ __forceinline__ void set(int i, float v) { e[i] = from_float<T>(v); }
+  // elements i and i + 1 (i even): one conversion instruction for a pair of 16-bit elements
+  __device__ __forceinline__ void set2(int i, float a, float b) {
+    if constexpr (std::is_same<T, __nv_bfloat16>::value) {
+      const __nv_bfloat162 v = __floats2bfloat162_rn(a, b);
+      e[i] = v.x;
+      e[i + 1] = v.y;
+    } else if constexpr (std::is_same<T, __half>::value) {
+      const __half2 v = __floats2half2_rn(a, b);
+      e[i] = v.x;
+      e[i + 1] = v.y;
+    } else {
+      e[i] = a;
+      e[i + 1] = b;
+    }
+  }
+  // all elements of f
+  __device__ __forceinline__ void set_all(const float (&f)[VEC]) {
+    if constexpr (VEC % 2 == 0) {
+#pragma unroll
+      for (int i = 0; i < VEC; i += 2) set2(i, f[i], f[i + 1]);
+    } else {
+#pragma unroll
+      for (int i = 0; i < VEC; ++i) set(i, f[i]);
+    }
+  }
 };
 
 // storage type of an operand whose type is chosen at run time
