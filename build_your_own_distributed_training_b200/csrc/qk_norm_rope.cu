@@ -155,14 +155,46 @@ __device__ __forceinline__ void store_head(const Pack<T, VEC> (&lo)[NP], const P
     }
 }
 
+// elements i and i + 1 of a lane's row as a pair (0 past its end)
+template <int VEC>
+__device__ __forceinline__ f2 two(const float (&v)[VEC], int i) { return pair(v[i], i + 1 < VEC ? v[i + 1] : 0.f); }
+template <int VEC>
+__device__ __forceinline__ void put(float (&v)[VEC], int i, f2 p) {
+  float a, b;
+  unpair(p, a, b);
+  v[i] = a;
+  if (i + 1 < VEC) v[i + 1] = b;
+}
+__device__ __forceinline__ float sum2(f2 p) {
+  float a, b;
+  unpair(p, a, b);
+  return a + b;
+}
+
+// With the weight taken into the rotation's factors, y_lo = r (x_lo wl c - x_hi wh s) and
+// y_hi = r (x_hi wh c + x_lo wl s).
 template <int KIND, typename T, int VEC, int NP, int U>
 __device__ __forceinline__ void fwd_run(const Args& a, const T* x, T* y, const Lane<VEC, NP>& ln, int grp, int part,
                                         const float (&c)[NP][VEC], const float (&s)[NP][VEC]) {
   const int half = a.hd >> 1, per = 32 / a.lanes, stride = per * a.split;
   const int first = KIND == Q ? 0 : KIND == K ? a.nq : a.nq + a.nkv, end = first + (KIND == Q ? a.nq : a.nkv);
   const float inv_hd = 1.f / (float)a.hd;
-  float wl[NP][VEC], wh[NP][VEC];
-  if constexpr (KIND != V) load_weight(KIND == Q ? a.wq : a.wk, a.wdt, ln, half, wl, wh);
+  constexpr int PAIRS = (VEC + 1) / 2;
+  f2 lc[NP][PAIRS], ls[NP][PAIRS], hc[NP][PAIRS], hs[NP][PAIRS];  // wl c, wl s, wh c, -wh s
+  if constexpr (KIND != V) {
+    float wl[NP][VEC], wh[NP][VEC];
+    load_weight(KIND == Q ? a.wq : a.wk, a.wdt, ln, half, wl, wh);
+#pragma unroll
+    for (int i = 0; i < NP; ++i)
+#pragma unroll
+      for (int v = 0; v < VEC; v += 2) {
+        const f2 cc = two(c[i], v), ss = two(s[i], v), l = two(wl[i], v), h = two(wh[i], v);
+        lc[i][v / 2] = mul2(l, cc);
+        ls[i][v / 2] = mul2(l, ss);
+        hc[i][v / 2] = mul2(h, cc);
+        hs[i][v / 2] = mul2(mul2(h, ss), pair(-1.f, -1.f));
+      }
+  }
   for (int h0 = first + part * per; h0 < end; h0 += U * stride) {
     Pack<T, VEC> lo[U][NP], hi[U][NP];
 #pragma unroll
@@ -174,23 +206,24 @@ __device__ __forceinline__ void fwd_run(const Args& a, const T* x, T* y, const L
     for (int u = 0; u < U; ++u) {
       const int h = h0 + u * stride + grp;
       if constexpr (KIND != V) {
-        float ss = 0.f;
+        f2 ss = pair(0.f, 0.f);
 #pragma unroll
         for (int i = 0; i < NP; ++i)
 #pragma unroll
-          for (int v = 0; v < VEC; ++v) {
-            const float p = lo[u][i].at(v), q = hi[u][i].at(v);
-            ss = fmaf(p, p, fmaf(q, q, ss));
+          for (int v = 0; v < VEC; v += 2) {
+            const f2 p = lo[u][i].at2(v), q = hi[u][i].at2(v);
+            ss = fma2(p, p, fma2(q, q, ss));
           }
-        const float r = rsqrtf(group_sum(ss, a.lanes) * inv_hd + a.eps);
+        const float r = rsqrtf(group_sum(sum2(ss), a.lanes) * inv_hd + a.eps);
+        const f2 rr = pair(r, r);
 #pragma unroll
         for (int i = 0; i < NP; ++i) {
           float yl[VEC], yh[VEC];
 #pragma unroll
-          for (int v = 0; v < VEC; ++v) {
-            const float ul = lo[u][i].at(v) * r * wl[i][v], uh = hi[u][i].at(v) * r * wh[i][v];
-            yl[v] = ul * c[i][v] - uh * s[i][v];
-            yh[v] = uh * c[i][v] + ul * s[i][v];
+          for (int v = 0; v < VEC; v += 2) {
+            const f2 p = mul2(lo[u][i].at2(v), rr), q = mul2(hi[u][i].at2(v), rr);
+            put(yl, v, fma2(q, hs[i][v / 2], mul2(p, lc[i][v / 2])));
+            put(yh, v, fma2(p, ls[i][v / 2], mul2(q, hc[i][v / 2])));
           }
           lo[u][i].set_all(yl);
           hi[u][i].set_all(yh);
@@ -240,31 +273,33 @@ __device__ __forceinline__ void bwd_run(const Args& a, const T* x, const T* g, T
       const int h = h0 + u * stride + grp;
       if constexpr (KIND != V) {
         // gu = R^T g; with n = x r, mean(gu w n) = r mean(gu w x), so both sums go over the lanes together
-        float ul[NP][VEC], uh[NP][VEC], ss = 0.f, dot = 0.f;
+        constexpr int PAIRS = (VEC + 1) / 2;
+        f2 ul[NP][PAIRS], uh[NP][PAIRS], ss = pair(0.f, 0.f), dot = ss;
 #pragma unroll
         for (int i = 0; i < NP; ++i)
 #pragma unroll
-          for (int v = 0; v < VEC; ++v) {
-            const float p = xl[u][i].at(v), q = xh[u][i].at(v), e = gl[u][i].at(v), f = gh[u][i].at(v);
-            ul[i][v] = e * c[i][v] + f * s[i][v];
-            uh[i][v] = f * c[i][v] - e * s[i][v];
-            ss = fmaf(p, p, fmaf(q, q, ss));
-            dot = fmaf(ul[i][v] * wl[i][v], p, fmaf(uh[i][v] * wh[i][v], q, dot));
+          for (int v = 0; v < VEC; v += 2) {
+            const f2 p = xl[u][i].at2(v), q = xh[u][i].at2(v), e = gl[u][i].at2(v), f = gh[u][i].at2(v);
+            const f2 cc = two(c[i], v), sn = two(s[i], v);
+            ul[i][v / 2] = fma2(f, sn, mul2(e, cc));
+            uh[i][v / 2] = fma2(mul2(e, sn), pair(-1.f, -1.f), mul2(f, cc));
+            ss = fma2(p, p, fma2(q, q, ss));
+            dot = fma2(mul2(ul[i][v / 2], two(wl[i], v)), p, fma2(mul2(uh[i][v / 2], two(wh[i], v)), q, dot));
           }
-        ss = group_sum(ss, a.lanes);
-        dot = group_sum(dot, a.lanes);
-        const float r = rsqrtf(ss * inv_hd + a.eps), m = r * dot * inv_hd;  // m = mean(gu w n)
+        const float sq = group_sum(sum2(ss), a.lanes), dt = group_sum(sum2(dot), a.lanes);
+        const float r = rsqrtf(sq * inv_hd + a.eps), m = r * dt * inv_hd;  // m = mean(gu w n)
+        const f2 rr = pair(r, r), mm = pair(-m, -m);
 #pragma unroll
         for (int i = 0; i < NP; ++i) {
           float al[VEC], ah[VEC];
 #pragma unroll
-          for (int v = 0; v < VEC; ++v) {
-            const float nl = xl[u][i].at(v) * r, nh = xh[u][i].at(v) * r;
-            al[v] = r * (ul[i][v] * wl[i][v] - nl * m);
-            ah[v] = r * (uh[i][v] * wh[i][v] - nh * m);
+          for (int v = 0; v < VEC; v += 2) {
+            const f2 nl = mul2(xl[u][i].at2(v), rr), nh = mul2(xh[u][i].at2(v), rr);
+            put(al, v, mul2(rr, fma2(nl, mm, mul2(ul[i][v / 2], two(wl[i], v)))));
+            put(ah, v, mul2(rr, fma2(nh, mm, mul2(uh[i][v / 2], two(wh[i], v)))));
             // (heads past the run were loaded as zeros and add nothing)
-            dl[i][v] = fmaf(ul[i][v], nl, dl[i][v]);
-            dh[i][v] = fmaf(uh[i][v], nh, dh[i][v]);
+            put(dl[i], v, fma2(ul[i][v / 2], nl, two(dl[i], v)));
+            put(dh[i], v, fma2(uh[i][v / 2], nh, two(dh[i], v)));
           }
           gl[u][i].set_all(al);
           gh[u][i].set_all(ah);

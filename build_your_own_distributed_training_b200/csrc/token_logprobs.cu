@@ -97,30 +97,6 @@ __device__ __forceinline__ unsigned long long warp_merge(unsigned long long k, u
   return k;
 }
 
-// Two fp32 at a time (sm_100 add / mul / fma on register pairs): the forward's exponent and sums are bound by
-// instructions for 16-bit logits, where a vector brings 8 of them.
-typedef unsigned long long f2;
-__device__ __forceinline__ f2 pair(float a, float b) {
-  f2 r;
-  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
-  return r;
-}
-__device__ __forceinline__ void unpair(f2 v, float& a, float& b) { asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(v)); }
-__device__ __forceinline__ f2 add2(f2 a, f2 b) {
-  f2 r;
-  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
-  return r;
-}
-__device__ __forceinline__ f2 mul2(f2 a, f2 b) {
-  f2 r;
-  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
-  return r;
-}
-__device__ __forceinline__ f2 fma2(f2 a, f2 b, f2 c) {
-  f2 r;
-  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
-  return r;
-}
 // (x0 - m) c and (x1 - m) c, at least kMinExp
 __device__ __forceinline__ f2 exponents(float x0, float x1, f2 neg_m, f2 c) {
   float a, b;
