@@ -29,8 +29,11 @@ __device__ __forceinline__ void make_tile_word(const TileJob& a, int t, int r) {
 }
 
 // The product's kernels are launched so that they may start while the kernel before them in the stream still
-// runs (their set-up then costs no time of its own): they wait here before they touch memory.  A kernel
-// lets its successor start early with the other call; without it the successor starts at its end.
+// runs (their set-up then costs no time of its own): they wait here before they touch memory.  A kernel lets
+// its successor start early with the other call; without it the successor starts at its end.  The product
+// and the small kernels before it make that call (48 x 4096 x 11008: 17.8 -> 16.0 us); the tile quantisation
+// does not, as early blocks of the product would take the shared memory that its own still need (8192 x
+// 11008 x 4096 with its quantisation 290 -> 317 us).
 __device__ __forceinline__ void wait_for_predecessor() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 __device__ __forceinline__ void let_successor_start() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
 

@@ -23,9 +23,12 @@
 // blocks] tensor in this kernel was measured and left: two warps per CTA could not keep up (their loads'
 // latency came back once per stage), 1230 TFLOP/s at 8192 x 11008 x 4096 where the rest ran at 2290.
 //
+// 8192 x 11008 x 4096: bf16 result 264 us (2.80 PFLOP/s), fp32 288 us.
+//
 // What bounds it: a 128 x 256 x 128 step takes the tensor cores 512 cycles, in which one CTA alone would
 // move 48 KB into shared memory and read 48 KB from it, 192 bytes a cycle against the 128 there are.  A pair
-// halves B's share: 64 KB per CTA and step, 128 bytes a cycle.
+// halves B's share: 64 KB per CTA and step, 128 bytes a cycle.  At about 1.5 GHz under the power limit a step
+// takes some 700 cycles.
 //
 // Tensor memory: the accumulator takes 256 columns (one 256-column tile, or two 128-column tiles in turn),
 // the scales 16 columns for each of eight 512-deep steps in turn.  The accumulator is read into registers
@@ -636,7 +639,8 @@ void fp8_gemm(torch::Tensor A, torch::Tensor tA, torch::Tensor B, torch::Tensor 
   // single CTA (128 x 128 tile) and 700 on a pair (256 x 256) when nothing else holds it up; a unit of work
   // costs two stages more for its start and end, and parts of K, whose fp32 sums a second kernel adds in
   // order, about 11 stages more and their bytes (100 cycles for 275 kB).  Parts fill the SMs where tiles are few (a few tokens against the weights).
-  // 48 x 4096 x 11008: one part 28 us, six 16; 1 x 22016 x 4096: pairs 30 us, single CTAs in four parts 19.
+  // 48 x 4096 x 11008: one part 28 us, several and their join 16; 1 x 22016 x 4096: pairs 30 us, single CTAs
+  // in four parts 20 and the join 3.
   const int sms = device_sm_count();
   const long tiles = ((M + 127) / 128) * ((N + 127) / 128), tiles2 = ((M + 255) / 256) * ((N + 255) / 256);
   auto cost = [&](long splits, long k_per) { return (tiles * splits + sms - 1) / sms * (k_per + 2) * 5 + (splits > 1 ? 55 + splits * M * N * 8 / 275000 : 0); };

@@ -13,7 +13,9 @@
 // first half and their partners of the second, so the rotation needs no exchange and the only cross-lane
 // step is the L-lane sum.  (8 + 8 elements a lane filled the register file in the backward: 121 us for 8192
 // tokens of 48 heads of 128.)  A warp stays on one token: its cos/sin row is read once and lives in
-// registers while the token's heads stream through, several heads per lane group in flight.  Statistics, rotation and
+// registers while the token's heads stream through, several heads per lane group in flight; arithmetic goes
+// two fp32 at a time.  8192 tokens of 32 + 8 + 8 heads of 128, bf16: forward 44 us (4.6 TB/s), backward
+// 75 us (3.8 TB/s): between the memory's rate and the instructions of 8 elements a lane and head.  Statistics, rotation and
 // weight gradients are fp32; y and dx are rounded once, to the storage type.
 //
 // dw: every warp adds up the heads of its tokens in registers, the block's warps are added in order

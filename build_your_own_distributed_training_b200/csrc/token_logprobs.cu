@@ -15,6 +15,10 @@
 // type's lowest value cannot overflow, and exponents are held at -256 or above, where 2^t is zero:
 // an excluded logit (-inf) then adds exactly nothing to S and A.
 //
+// 4096 x 32000 fp32 without alternatives: forward 86 us (6.1 TB/s, memory), backward 144 us.  777 x 32003 bf16
+// with 5 alternatives: 35 and 21 us, bound by instructions (a 16-byte vector holds 8 exponentials) and, per
+// row, by the sorts.  One row of 128256 fp32 with 20 alternatives: 11 us in a cluster of 8, all latency.
+//
 // Top k (k <= 32) without sorting the row: the k largest thread maxima name the k threads that can
 // own one of the k largest elements, and the k-th of these maxima is a lower bound for all of them;
 // the warps read those threads' vectors again (a few per owner, from L2) and keep sorted lists of 32

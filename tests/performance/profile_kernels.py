@@ -23,6 +23,7 @@ import sys
 sys.path.insert(0, os.path.dirname(os.path.dirname(os.path.dirname(os.path.abspath(__file__)))))
 import torch  # noqa: E402
 
+from build_your_own_distributed_training_b200 import ops  # noqa: E402
 from build_your_own_distributed_training_b200.ops import gemm  # noqa: E402
 from build_your_own_distributed_training_b200.ops._ext import native  # noqa: E402
 from build_your_own_distributed_training_b200.ops.rope import precompute_rope_cache  # noqa: E402
@@ -303,6 +304,53 @@ def case_adamw():
 def case_sumsq():
     x = torch.randn(256 << 20, device=DEV)
     return lambda: native().sumsq(x), 0, x.numel() * 4
+
+
+def case_fp8_matmul():
+    # 8-bit product on CTA pairs, 8192 x 11008 x 4096, bf16 result
+    a, b = ops.quantize_fp8(_bf(T, D)), ops.quantize_fp8(_bf(FFN, D), square=True)
+    out = torch.empty(T, FFN, device=DEV, dtype=BF)
+    return lambda: ops.fp8_matmul(a, b, out=out), 2 * T * FFN * D, 0
+
+
+def case_fp8_matmul_48():
+    # 48 tokens against 4096 x 11008: K in parts, joined by a second kernel
+    a, b = ops.quantize_fp8(_bf(48, FFN)), ops.quantize_fp8(_bf(D, FFN), square=True)
+    return lambda: ops.fp8_matmul(a, b), 0, D * FFN
+
+
+def case_fp8_quantize():
+    x = _bf(T, FFN)
+    return lambda: native().fp8_quantize(x, False, True, True), 0, 4 * T * FFN
+
+
+def case_qk_norm_rope():
+    W = (HEADS + 16) * HD
+    x, dy, w = _bf(T, W), _bf(T, W), torch.ones(HD, device=DEV, dtype=BF)
+    cos, sin = precompute_rope_cache(HD, T, 10000.0, device=DEV)
+    dw = torch.empty(2, HD, device=DEV)
+
+    def run():
+        native().qk_norm_rope_fwd(x, w, w, cos, sin, None, HEADS, 8, HD, T, 1e-5)
+        native().qk_norm_rope_bwd(dy, x, w, w, cos, sin, None, HEADS, 8, HD, T, 1e-5, dw[0], dw[1], False)
+    return run, 0, (4 * W + (HEADS + 8) * HD) * T * 2
+
+
+def case_dropout_add():
+    x, r = _bf(T, D), _bf(T, D)
+    return lambda: ops.dropout_add(x, r, 0.1, 7), 0, 3 * T * D * 2
+
+
+def case_token_log_probs():
+    x = torch.randn(T // 2, V, device=DEV)
+    tok = torch.randint(0, V, (T // 2,), device=DEV)
+    g = torch.ones(T // 2, device=DEV)
+    dx = torch.empty_like(x)
+
+    def run():
+        state = native().token_logprobs_fwd(x, tok, 1.0, 0, -100, True)[-1]
+        native().token_logprobs_bwd(x, tok, state, g, g, 1.0, dx)
+    return run, 0, 3 * x.numel() * 4
 
 
 CASES = {k[5:]: v for k, v in globals().items() if k.startswith("case_")}
