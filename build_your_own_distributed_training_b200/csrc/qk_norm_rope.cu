@@ -14,8 +14,10 @@
 // step is the L-lane sum.  (8 + 8 elements a lane filled the register file in the backward: 121 us for 8192
 // tokens of 48 heads of 128.)  A warp stays on one token: its cos/sin row is read once and lives in
 // registers while the token's heads stream through, several heads per lane group in flight; arithmetic goes
-// two fp32 at a time.  8192 tokens of 32 + 8 + 8 heads of 128, bf16: forward 44 us (4.6 TB/s), backward
-// 75 us (3.8 TB/s): between the memory's rate and the instructions of 8 elements a lane and head.  Statistics, rotation and
+// two fp32 at a time.  8192 tokens of 32 + 8 + 8 heads of 128, bf16: forward 39 us (5.1 TB/s), backward
+// 75 us (3.8 TB/s).  Both wait on latency: half the issue slots are used, and the registers of the heads in
+// flight allow four blocks an SM forward (three took 44 us) and two backward (three with half the heads in
+// flight spilled and took 105 us).  Statistics, rotation and
 // weight gradients are fp32; y and dx are rounded once, to the storage type.
 //
 // dw: every warp adds up the heads of its tokens in registers, the block's warps are added in order
@@ -237,7 +239,7 @@ __device__ __forceinline__ void fwd_run(const Args& a, const T* x, T* y, const L
 }
 
 template <typename T, int VEC, int NP, int U>
-__global__ void __launch_bounds__(NT) qk_fwd_kernel(const Args a) {
+__global__ void __launch_bounds__(NT, VEC > 1 ? 4 : 1) qk_fwd_kernel(const Args a) {
   const int lane = threadIdx.x & 31;
   const long item = (long)blockIdx.x * (NT / 32) + (threadIdx.x >> 5);
   if (item >= a.tokens * a.split) return;
@@ -468,7 +470,7 @@ torch::Tensor qk_norm_rope_fwd(torch::Tensor x, torch::Tensor wq, torch::Tensor 
   DTB_CHECK(blocks < (1L << 31), "qk_norm_rope: too many tokens");
   auto st = at::cuda::getCurrentCUDAStream();
   DTB_FLOAT_TYPES(x.scalar_type(), {
-    if (vec) qk::qk_fwd_kernel<T, 4, 1, 4><<<(unsigned)blocks, qk::NT, 0, st>>>(a);
+    if (vec) qk::qk_fwd_kernel<T, 4, 1, sizeof(T) == 4 ? 2 : 4><<<(unsigned)blocks, qk::NT, 0, st>>>(a);
     else qk::qk_fwd_kernel<T, 1, 8, 1><<<(unsigned)blocks, qk::NT, 0, st>>>(a);
   });
   DTB_LAUNCH_CHECK();
