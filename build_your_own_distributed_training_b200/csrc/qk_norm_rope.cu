@@ -291,7 +291,8 @@ __device__ __forceinline__ void bwd_run(const Args& a, const T* x, const T* g, T
             dot = fma2(mul2(ul[i][v / 2], two(wl[i], v)), p, fma2(mul2(uh[i][v / 2], two(wh[i], v)), q, dot));
           }
         const float sq = group_sum(sum2(ss), a.lanes), dt = group_sum(sum2(dot), a.lanes);
-        const float r = rsqrtf(sq * inv_hd + a.eps), m = r * dt * inv_hd;  // m = mean(gu w n)
+        // heads past the run were loaded as zeros: with r = 0 they add nothing, at eps = 0 neither
+        const float r = h < end ? rsqrtf(sq * inv_hd + a.eps) : 0.f, m = r * dt * inv_hd;  // m = mean(gu w n)
         const f2 rr = pair(r, r), mm = pair(-m, -m);
 #pragma unroll
         for (int i = 0; i < NP; ++i) {
@@ -301,7 +302,6 @@ __device__ __forceinline__ void bwd_run(const Args& a, const T* x, const T* g, T
             const f2 nl = mul2(xl[u][i].at2(v), rr), nh = mul2(xh[u][i].at2(v), rr);
             put(al, v, mul2(rr, fma2(nl, mm, mul2(ul[i][v / 2], two(wl[i], v)))));
             put(ah, v, mul2(rr, fma2(nh, mm, mul2(uh[i][v / 2], two(wh[i], v)))));
-            // (heads past the run were loaded as zeros and add nothing)
             put(dl[i], v, fma2(ul[i][v / 2], nl, two(dl[i], v)));
             put(dh[i], v, fma2(uh[i][v / 2], nh, two(dh[i], v)));
           }
