@@ -16,6 +16,7 @@ import os
 from typing import NamedTuple
 
 import torch
+import torch.nn.functional as F
 
 from . import gemm, grad_state
 from ._ext import native
@@ -140,12 +141,19 @@ def _row_blocks(rows: int, vocab: int) -> list[tuple[int, int]]:
     return [(r, min(rows, r + step)) for r in range(0, rows, step)]
 
 
+def _whole_rows(w: torch.Tensor) -> torch.Tensor:
+    """The head's weight with rows of zeros up to a multiple of 8, which the products' 16-byte rows of
+    logits need; the log probabilities read the vocabulary's columns alone."""
+    return F.pad(w, (0, 0, 0, -w.shape[0] % 8)) if w.shape[0] % 8 else w
+
+
 class _HeadLogProbsFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, h, w, tokens, temperature, top_k, ignore, main_grad):  # type: ignore[override]
         outs = []
-        for r0, r1 in _row_blocks(h.shape[0], w.shape[0]):
-            logits = gemm.mm_nt(h[r0:r1], w, out_dtype=torch.float32)
+        V, wp = w.shape[0], _whole_rows(w)
+        for r0, r1 in _row_blocks(h.shape[0], V):
+            logits = gemm.mm_nt(h[r0:r1], wp, out_dtype=torch.float32)[:, :V]
             outs.append(native().token_logprobs_fwd(logits, tokens[r0:r1], temperature, top_k, ignore, True))
         lp, ent, *top, state = (torch.cat(t) if len(outs) > 1 else t[0] for t in zip(*outs))
         top_v, top_i = top or (None, None)
@@ -162,32 +170,50 @@ class _HeadLogProbsFn(torch.autograd.Function):
         g_lp, g_ent, mg = _row_grad(g_lp), _row_grad(g_ent), ctx.main_grad
         need_w = mg is not None or w.requires_grad
         dh = torch.empty_like(h)
-        store = grad_state.take_fresh(mg) if mg is not None else True
-        acc = mg.view(w.shape) if mg is not None else (
-            torch.empty(w.shape, device=w.device, dtype=torch.float32) if need_w else None)
-        for r0, r1 in _row_blocks(h.shape[0], w.shape[0]):
+        V, wp = w.shape[0], _whole_rows(w)
+        direct = mg is not None and wp is w  # products straight into the engine's gradient
+        store = grad_state.take_fresh(mg) if direct else True
+        acc = mg.view(w.shape) if direct else (
+            torch.empty(wp.shape, device=w.device, dtype=torch.float32) if need_w else None)
+        for r0, r1 in _row_blocks(h.shape[0], V):
             hb = h[r0:r1]
-            logits = gemm.mm_nt(hb, w, out_dtype=torch.float32)
-            dl = torch.empty(r1 - r0, w.shape[0], device=h.device, dtype=h.dtype)
+            logits = gemm.mm_nt(hb, wp, out_dtype=torch.float32)[:, :V]
+            dl = torch.empty(r1 - r0, wp.shape[0], device=h.device, dtype=h.dtype)
+            if wp is not w:
+                dl[:, V:] = 0
             native().token_logprobs_bwd(logits, tokens[r0:r1], state[r0:r1], None if g_lp is None else g_lp[r0:r1],
-                                        None if g_ent is None else g_ent[r0:r1], ctx.temperature, dl)
-            gemm.mm_nn(dl, w, out=dh[r0:r1])
+                                        None if g_ent is None else g_ent[r0:r1], ctx.temperature, dl[:, :V])
+            gemm.mm_nn(dl, wp, out=dh[r0:r1])
             if acc is not None:
                 gemm.mm_tn_acc(dl, hb, acc, store=store)
                 store = False
-        dw = acc.to(w.dtype) if mg is None and need_w else None
+        if mg is not None and not direct:
+            grad_state.zero_if_fresh(mg)
+            mg.view(w.shape).add_(acc[:V])
+        dw = acc[:V].to(w.dtype) if mg is None and need_w else None
         return dh, dw, None, None, None, None, None
 
 
 def lm_head_token_log_probs(h: torch.Tensor, weight: torch.Tensor, tokens: torch.Tensor, *, temperature: float = 1.0,
                             top_k: int = 0, ignore_index: int = IGNORE,
                             main_grad: torch.Tensor | None = None) -> TokenLogProbs:
-    """:func:`token_log_probs` of ``h @ weight^T`` for ``h: [M, d]``, ``tokens: [M]``."""
+    """:func:`token_log_probs` of ``h @ weight^T`` for ``h: [M, d]``, ``tokens: [M]``.
+
+    On CUDA ``h`` and ``weight`` are bf16 and ``d`` a multiple of 8; the logits are fp32.  A vocabulary that is
+    no multiple of 8 costs a padded copy of the weight in each direction.
+    """
     _check(tokens, h.shape[:1], weight.shape[0], temperature, top_k)
-    if not h.is_cuda or h.dtype != torch.bfloat16 or weight.shape[0] % 8 or h.shape[1] % 8 or h.shape[0] == 0:
+    if not h.is_cuda:
         from .linear import linear
         return token_log_probs(linear(h, weight, main_grad=main_grad), tokens, temperature=temperature, top_k=top_k,
                                ignore_index=ignore_index)
+    if h.dtype != torch.bfloat16 or weight.dtype != torch.bfloat16:
+        raise ValueError(f"the scoring head takes bf16 on CUDA, got {h.dtype} and {weight.dtype}")
+    if h.shape[1] % 8:
+        raise ValueError(f"the scoring head needs a hidden size that is a multiple of 8 on CUDA, got {h.shape[1]}")
+    if h.shape[0] == 0:  # no rows: nothing for the products, zero gradients
+        logits = F.linear(h, weight.detach() if main_grad is not None else weight).float()
+        return token_log_probs(logits, tokens, temperature=temperature, top_k=top_k, ignore_index=ignore_index)
     lp, ent, top_v, top_i = _HeadLogProbsFn.apply(h.contiguous(), weight, tokens.contiguous(), float(temperature),
                                                   int(top_k), int(ignore_index), main_grad)
     return _shaped(lp, ent, top_v, top_i, tokens.shape, top_k)

@@ -48,3 +48,65 @@ def test_qk_norm_rope_without_eps(nq, nkv, hd, dt):
     unit = 0.0 if dt == F32 else UNIT[dt]
     assert rel(y, ref) < 2.0 ** -18 + unit and rel(x.grad, xd.grad) < 2.0 ** -18 + unit
     assert rel(wq.grad, qd.grad) < 2.0 ** -14 + unit and rel(wk.grad, kd.grad) < 2.0 ** -14 + unit
+
+
+@pytest.mark.parametrize("V", [5, 2001, 32003])
+@pytest.mark.parametrize("main", [False, True])
+def test_scoring_head_takes_any_vocabulary(V, main, monkeypatch):
+    from build_your_own_distributed_training_b200.ops import logprobs as mod
+    monkeypatch.setattr(mod, "HEAD_BYTES", 128 * 4 * V)  # blocks of 128 rows
+    M, d, k = 150, 256, min(V, 3)
+    h = _randn(M, d, seed=1, dt=BF).requires_grad_(True)
+    w = (_randn(V, d, seed=2) * 0.1).to(BF).requires_grad_(not main)
+    tok = torch.randint(0, V, (M,), device=DEV, generator=torch.Generator(device=DEV).manual_seed(3))
+    tok[::7] = -100
+    mg = torch.ones(V, d, device=DEV) if main else None
+    r = ops.lm_head_token_log_probs(h, w, tok, top_k=k, main_grad=mg)
+    hd, wd = h.detach().double().requires_grad_(True), w.detach().double().requires_grad_(True)
+    lp, ent = plain.logprobs(hd @ wd.t(), tok)
+    # fp32 logits: no rounding to bf16 before the log probabilities
+    assert float((r.logprob.double() - lp).abs().max()) < 2.0 ** -16 and float((r.entropy.double() - ent).abs().max()) < 2.0 ** -16
+    live = tok != -100
+    assert (r.top_tokens[live] >= 0).all() and (r.top_tokens[live] < V).all() and (r.top_tokens[~live] == -1).all()
+    (r.logprob.sum() - 0.1 * r.entropy.sum()).backward()
+    (lp.sum() - 0.1 * ent.sum()).backward()
+    # the logit gradient is rounded to bf16 between the two products, the results once more
+    assert rel(h.grad, hd.grad) < 2 * UNIT[BF] and rel(mg - 1 if main else w.grad, wd.grad) < 2 * UNIT[BF]
+
+
+def test_scoring_head_refusals_and_no_rows():
+    w, tok = _randn(64, 32, dt=BF), torch.zeros(4, device=DEV, dtype=torch.int64)
+    with pytest.raises(ValueError, match="bf16"):
+        ops.lm_head_token_log_probs(_randn(4, 32), w, tok)
+    with pytest.raises(ValueError, match="bf16"):
+        ops.lm_head_token_log_probs(_randn(4, 32, dt=BF), w.float(), tok)
+    with pytest.raises(ValueError, match="multiple of 8"):
+        ops.lm_head_token_log_probs(_randn(4, 30, dt=BF), w[:, :30].contiguous(), tok)
+    h, wg = _randn(0, 32, dt=BF).requires_grad_(True), w.clone().requires_grad_(True)
+    for V in (64, 61):
+        h.grad = wg.grad = None
+        r = ops.lm_head_token_log_probs(h, wg[:V], tok[:0], top_k=2)
+        assert r.logprob.shape == (0,) and r.logprob.dtype == F32 and r.top_tokens.shape == (0, 2)
+        (r.logprob.sum() + r.entropy.sum()).backward()
+        assert h.grad.shape == (0, 32) and (wg.grad == 0).all()
+
+
+def test_model_with_an_odd_vocabulary_scores():
+    from build_your_own_distributed_training_b200.config import ModelConfig, ParallelConfig
+    from build_your_own_distributed_training_b200.models import TransformerBlock, build_model
+    from build_your_own_distributed_training_b200.parallel.fsdp import FullyShardedModel
+    torch.manual_seed(0)
+    mc = ModelConfig(vocab_size=509, d_model=128, n_layers=1, n_heads=2, n_kv_heads=1, ffn_hidden_size=256,
+                     max_seq_len=64, tie_embeddings=False)
+    ref, model = build_model(mc), build_model(mc)
+    model.load_state_dict(ref.state_dict())
+    eng = FullyShardedModel(model, None, ParallelConfig(), {TransformerBlock}, device=DEV)
+    model.rope_cos, model.rope_sin = model.rope_cos.to(DEV), model.rope_sin.to(DEV)
+    x, y = torch.randint(0, 509, (2, 2, 50), generator=torch.Generator().manual_seed(1))
+    r, c = eng(x.to(DEV), targets=y.to(DEV), top_k=2), ref(x, targets=y, top_k=2)
+    # bf16 activations through one block; the logits' spread is about 0.3
+    assert float((r.logprob.cpu() - c.logprob).abs().max()) < 0.1
+    (-r.logprob.sum() / 100 - 0.1 * r.entropy.sum() / 100).backward()
+    (-c.logprob.sum() / 100 - 0.1 * c.entropy.sum() / 100).backward()
+    for (n, p), (_, q) in zip(eng.module.named_parameters(), ref.named_parameters()):
+        assert rel(p.main_grad, q.grad) < 0.06, n  # some dozens of bf16 roundings
