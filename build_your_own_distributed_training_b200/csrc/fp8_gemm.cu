@@ -594,7 +594,7 @@ using namespace dtb;
 void fp8_gemm(torch::Tensor A, torch::Tensor tA, torch::Tensor B, torch::Tensor tB, torch::Tensor D,
               c10::optional<torch::Tensor> R, bool accumulate) {
   for (const torch::Tensor* t : {&A, &B})
-    DTB_CHECK(t->is_cuda() && t->device() == A.device() && t->scalar_type() == at::kFloat8_e4m3fn && t->dim() == 2 && (t->numel() == 0 || ((t->size(1) == 1 || t->stride(1) == 1) && t->stride(0) % 16 == 0 && (reinterpret_cast<uintptr_t>(t->data_ptr()) & 15) == 0)), "fp8_gemm: operands must be 2-D e4m3 on one GPU, rows contiguous and starting on 16-byte boundaries");
+    DTB_CHECK(t->is_cuda() && t->device() == A.device() && t->scalar_type() == at::kFloat8_e4m3fn && t->dim() == 2 && (t->numel() == 0 || ((t->size(1) == 1 || t->stride(1) == 1) && (t->size(0) == 1 || t->stride(0) % 16 == 0) && (reinterpret_cast<uintptr_t>(t->data_ptr()) & 15) == 0)), "fp8_gemm: operands must be 2-D e4m3 on one GPU, rows contiguous and starting on 16-byte boundaries");
   const long M = A.size(0), N = B.size(0), K = A.size(1);
   DTB_CHECK(B.size(1) == K && D.dim() == 2 && D.size(0) == M && D.size(1) == N && D.device() == A.device() && (N == 1 || M == 0 || D.stride(1) == 1), "fp8_gemm: shapes do not match");
   DTB_CHECK(D.scalar_type() == at::kBFloat16 || D.scalar_type() == at::kFloat, "fp8_gemm: the result is bf16 or fp32");

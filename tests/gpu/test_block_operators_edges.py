@@ -110,3 +110,17 @@ def test_model_with_an_odd_vocabulary_scores():
     (-c.logprob.sum() / 100 - 0.1 * c.entropy.sum() / 100).backward()
     for (n, p), (_, q) in zip(eng.module.named_parameters(), ref.named_parameters()):
         assert rel(p.main_grad, q.grad) < 0.06, n  # some dozens of bf16 roundings
+
+
+@pytest.mark.parametrize("K", [1, 15, 130, 300])
+def test_single_rows_of_codes_with_any_row_length(K):
+    tight = lambda b: ops.Fp8Blocks(torch.empty(b.values.shape, device=DEV, dtype=b.values.dtype).copy_(b.values),  # noqa: E731
+                                    b.scales)
+    one, many = ops.quantize_fp8(_randn(1, K, seed=1, dt=BF)), ops.quantize_fp8(_randn(40, K, seed=2, dt=BF))
+    for a, b in ((one, many), (many, one), (one, one)):
+        want = ops.fp8_matmul(a, b, out_dtype=F32)
+        assert tight(one).values.stride(0) == K
+        for x, y in ((tight(a), tight(b)), (tight(a), b), (a, tight(b))):
+            assert torch.equal(ops.fp8_matmul(x, y, out_dtype=F32), want)
+    x, w = _randn(5, K, seed=3, dt=BF), ops.quantize_fp8(_randn(1, K, seed=4), square=True)
+    assert torch.equal(ops.linear_fp8(x, tight(w)), ops.linear_fp8(x, w))
