@@ -4,6 +4,8 @@
 // (gradients that go into its fp32 buffers) and for the CPU path; both call the same kernels.
 #include <torch/extension.h>
 
+#include <cstdio>
+
 using torch::Tensor;
 using torch::autograd::AutogradContext;
 using torch::autograd::Function;
@@ -155,9 +157,22 @@ Tensor linear_fp8_autograd(Tensor x, Tensor w, c10::optional<Tensor> residual) {
   return LinearFp8::apply(x, w, residual);
 }
 
+// ValueError unless q is e4m3 [rows, cols] and s its e8m0 scales in 1 x 128 or 128 x 128 blocks.
+void fp8_check_blocks(const Tensor& q, const Tensor& s) {
+  TORCH_CHECK_VALUE(q.dim() == 2 && q.scalar_type() == at::kFloat8_e4m3fn && s.scalar_type() == at::kFloat8_e8m0fnu,
+                    "8-bit blocks are e4m3 [rows, cols] codes with e8m0 scales, got ", q.scalar_type(), " and ", s.scalar_type());
+  const long rows = q.size(0), cols = q.size(1), blocks = (rows + 127) / 128;
+  const long sr = s.dim() > 0 ? s.size(0) : 0, sc = s.dim() > 1 ? s.size(1) : 0;
+  if (s.dim() == 2 && (sr == blocks || sr == rows) && sc == (cols + 127) / 128) return;
+  char msg[160];
+  std::snprintf(msg, sizeof(msg), "scales [%ld, %ld] fit neither 1 x 128 nor 128 x 128 blocks of %ld x %ld", sr, sc, rows, cols);
+  TORCH_CHECK_VALUE(false, msg);
+}
+
 // x [T, K] bf16 with weights kept in 8 bits: values [N, K] e4m3, scales e8m0, their tiles or none
 Tensor linear_fp8_kept(Tensor x, Tensor values, Tensor scales, c10::optional<Tensor> tiles,
                        c10::optional<Tensor> residual) {
+  fp8_check_blocks(values, scales);
   auto xq = tiles.has_value() ? fp8_quantize(x, false, true, false) : fp8_quantize_with_tiles(x, scales, values.size(0));
   Tensor y = torch::empty({x.size(0), values.size(0)}, x.options());
   fp8_product(xq[0], xq[1], xq[2], values, scales, tiles.has_value() ? tiles : xq[3], y, residual, false);

@@ -718,11 +718,15 @@ static torch::Tensor fp8_aligned(torch::Tensor q) {
   return pad.narrow(1, 0, K);
 }
 
+void fp8_check_blocks(const torch::Tensor& q, const torch::Tensor& s);
+
 // fp8_gemm for operands as a user holds them: codes in rows of any alignment, plain scales, scale tiles or none.
 void fp8_product(torch::Tensor A, torch::Tensor sA, c10::optional<torch::Tensor> tA, torch::Tensor B, torch::Tensor sB,
                  c10::optional<torch::Tensor> tB, torch::Tensor D, c10::optional<torch::Tensor> R, bool accumulate) {
   for (const torch::Tensor* t : {&A, &B})
     DTB_CHECK(t->is_cuda() && t->scalar_type() == at::kFloat8_e4m3fn && t->dim() == 2, "fp8_product: operands must be 2-D e4m3 on the GPU");
+  fp8_check_blocks(A, sA);
+  fp8_check_blocks(B, sB);
   const c10::cuda::CUDAGuard guard(A.device());
   auto tiles = [](const torch::Tensor& q, const torch::Tensor& s, const c10::optional<torch::Tensor>& t) {
     return t.has_value() ? *t : fp8_scale_tiles(s, s.size(0) == (q.size(0) + 127) / 128 ? 128 : 1, q.size(0));

@@ -396,14 +396,14 @@ std::vector<torch::Tensor> fp8_quantize(torch::Tensor x, bool square, bool plain
 // the plain scales s: {codes, scales, tiles of x, tiles of s}.
 torch::Tensor fp8_scale_tiles(torch::Tensor s, int64_t gran, int64_t rows);
 std::vector<torch::Tensor> fp8_quantize_with_tiles(torch::Tensor x, torch::Tensor s, int64_t rows) {
-  const long mt = (rows + 127) / 128;
+  DTB_CHECK(x.dim() == 2, "fp8: a matrix of rows");
+  const long mt = (rows + 127) / 128, kb = (x.size(1) + 127) / 128, kq = (kb + fp8::SF_STEP - 1) / fp8::SF_STEP;
   const int64_t gran = s.dim() == 2 && s.size(0) == mt ? 128 : 1;
-  if (x.dim() != 2 || x.size(0) == 0 || x.size(0) >= 128 || x.size(1) == 0 || rows == 0) {
+  DTB_CHECK(s.device() == x.device() && s.scalar_type() == at::kFloat8_e8m0fnu && s.dim() == 2 && s.size(0) == (rows + gran - 1) / gran && s.size(1) == kb && mt * kq < (1L << 31), "fp8: scales must be e8m0 [%ld or %ld, %ld] on x's device", (long)rows, mt, kb);
+  if (x.size(0) == 0 || x.size(0) >= 128 || x.size(1) == 0 || rows == 0) {
     auto q = quantize(x, false, true, false, fp8::TileJob{});
     return {q[0], q[1], q[2], fp8_scale_tiles(s, gran, rows)};
   }
-  const long kb = (x.size(1) + 127) / 128, kq = (kb + fp8::SF_STEP - 1) / fp8::SF_STEP;
-  DTB_CHECK(s.device() == x.device() && s.scalar_type() == at::kFloat8_e8m0fnu && s.dim() == 2 && s.size(0) == (rows + gran - 1) / gran && s.size(1) == kb && mt * kq < (1L << 31), "fp8: scales must be e8m0 [%ld or %ld, %ld] on x's device", (long)rows, mt, kb);
   auto t = torch::empty({mt, kq, 512}, x.options().dtype(at::kByte));
   auto q = quantize(x, false, true, false, fp8::TileJob{reinterpret_cast<const uint8_t*>(s.data_ptr()), s.stride(0), s.stride(1), (int)gran,
                                                         (int)rows, (int)kb, (int)kq, reinterpret_cast<uint32_t*>(t.data_ptr()), (int)(mt * kq)});

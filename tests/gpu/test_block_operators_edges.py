@@ -124,3 +124,39 @@ def test_single_rows_of_codes_with_any_row_length(K):
             assert torch.equal(ops.fp8_matmul(x, y, out_dtype=F32), want)
     x, w = _randn(5, K, seed=3, dt=BF), ops.quantize_fp8(_randn(1, K, seed=4), square=True)
     assert torch.equal(ops.linear_fp8(x, tight(w)), ops.linear_fp8(x, w))
+
+
+@pytest.mark.parametrize("T", [5, 200])
+@pytest.mark.parametrize("square", [False, True])
+def test_kept_weights_with_wrong_scales_are_refused(T, square):
+    N, K = 200, 1000
+    x, b = _randn(T, K, dt=BF), ops.quantize_fp8(_randn(N, K, seed=1), square=square)
+    s = b.scales
+    wide = torch.cat((s.view(torch.uint8), s.view(torch.uint8)[:, :1]), 1).view(s.dtype)
+    a = ops.quantize_fp8(x)
+    wrong = [s[:, :5], s[:, :7], wide, s[:1], s[:, 0]]
+    for bad in wrong:
+        for tiles in (None, b.tiles):
+            with pytest.raises(ValueError, match="scales"):
+                ops.linear_fp8(x, ops.Fp8Blocks(b.values, bad, tiles))
+        with pytest.raises(ValueError, match="scales"):
+            native().linear_fp8_kept(x, b.values, bad, None, None)
+        with pytest.raises(ValueError, match="scales"):
+            native().fp8_product(a.values, a.scales, None, b.values, bad, None, torch.empty(T, N, device=DEV), None, False)
+    with pytest.raises(ValueError, match="e4m3"):
+        ops.linear_fp8(x, ops.Fp8Blocks(b.values.float(), s))
+
+
+@pytest.mark.parametrize("T", [1, 5, 64, 127, 128, 300])
+@pytest.mark.parametrize("N,K", [(22016, 512), (100, 4096), (515, 640), (64, 130)])
+@pytest.mark.parametrize("square", [False, True])
+def test_kept_weights_without_tiles(T, N, K, square):
+    """Weights given as codes and scales alone: the tiles are made in the call."""
+    x, b = _randn(T, K, seed=T, dt=BF), ops.quantize_fp8(_randn(N, K, seed=9), square=square)
+    want = ops.linear_fp8(x, b)
+    assert torch.equal(ops.linear_fp8(x, ops.Fp8Blocks(b.values, b.scales)), want)
+    # codes in tight rows, scales stored the other way round
+    turned = b.scales.view(torch.uint8).t().contiguous().t().view(b.scales.dtype)
+    assert torch.equal(ops.linear_fp8(x, ops.Fp8Blocks(b.values.contiguous(), turned)), want)
+    r = _randn(T, N, seed=5, dt=BF)
+    assert torch.equal(ops.linear_fp8(x, ops.Fp8Blocks(b.values, b.scales), residual=r), ops.linear_fp8(x, b, residual=r))
