@@ -35,7 +35,7 @@ class TokenLogProbs(NamedTuple):
 
 
 def _reference(x: torch.Tensor, tokens: torch.Tensor, temperature: float, top_k: int, ignore: int):
-    """``x: [M, V]`` -> (logprob, entropy, top log probabilities, top tokens, (m, S, entropy, ok))."""
+    """``x: [M, V]`` -> (logprob, entropy, top log probabilities, top tokens, (m, kind))."""
     x = x.float()
     V = x.shape[1]
     m = x.amax(-1)
@@ -61,21 +61,27 @@ def _reference(x: torch.Tensor, tokens: torch.Tensor, temperature: float, top_k:
     top_i = top_i.masked_fill((bad | skip)[:, None], -1)
     # rows that are skipped or empty have no gradient, bad ones a NaN gradient
     kind = torch.where(skip | (empty & ~bad), 1, torch.where(bad, 2, 0))
-    return finish(lp, ninf, 0.0), finish(ent, 0.0, 0.0), top_v, top_i, (m, s, ent, kind)
+    return finish(lp, ninf, 0.0), finish(ent, 0.0, 0.0), top_v, top_i, (m, kind)
 
 
 def _reference_grad(x, tokens, state, g_lp, g_ent, temperature):
-    m, s, ent, kind = state
+    """The logits' gradient as a function of ``x`` alone (``m`` only shifts), so that it can be differentiated again;
+    excluded tokens (-inf, or so far below ``m`` that the difference is) stay out of every product."""
+    m, kind = state
     ok = kind == 0
-    z = torch.where(ok[:, None], (x.float() - m[:, None]) / temperature, 0.0)
-    p = z.exp() / s[:, None]
-    plogp = torch.where(p > 0, p * (z - s.log()[:, None]), 0.0)
+    x = x.float()
+    live = ok[:, None] & ((x.detach() - m[:, None]) / temperature > float("-inf"))
+    z = torch.where(live, (torch.where(live, x, 0.0) - torch.where(ok, m, 0.0)[:, None]) / temperature, 0.0)
+    e = torch.where(live, z.exp(), 0.0)
+    s = torch.where(ok, e.sum(-1), 1.0)
+    p = e / s[:, None]
     d = torch.zeros_like(z)
     if g_lp is not None:
-        d -= p * g_lp[:, None]
-        d.scatter_add_(1, torch.where(ok, tokens, 0)[:, None], g_lp[:, None])
+        d = d - p * g_lp[:, None]
+        d = d.scatter_add(1, torch.where(ok, tokens, 0)[:, None], g_lp[:, None])
     if g_ent is not None:
-        d -= g_ent[:, None] * (plogp + p * ent[:, None])
+        ent = s.log() - (e * z).sum(-1) / s
+        d = d - g_ent[:, None] * (p * (z - s.log()[:, None]) + p * ent[:, None])
     d = d / temperature
     d[kind == 1], d[kind == 2] = 0.0, float("nan")
     return d
