@@ -90,6 +90,7 @@ torch::Tensor dropout_add_autograd(torch::Tensor x, c10::optional<torch::Tensor>
                                    int64_t start);
 std::vector<torch::Tensor> token_logprobs_autograd(torch::Tensor x, torch::Tensor tokens, double temperature,
                                                    int64_t top_k, int64_t ignore);
+torch::Tensor first_order(torch::Tensor g, const std::string& op, const std::vector<torch::Tensor>& dys);
 torch::Tensor linear_fp8_autograd(torch::Tensor x, torch::Tensor w, c10::optional<torch::Tensor> residual);
 
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
@@ -154,5 +155,6 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("qk_norm_rope", &qk_norm_rope_autograd, "qk_norm_rope_fwd as an autograd node");
   m.def("dropout_add", &dropout_add_autograd, "residual + dropout(x), mask from Philox4x32-10 by element number; an autograd node");
   m.def("token_logprobs", &token_logprobs_autograd, "token_logprobs_fwd as an autograd node");
+  m.def("first_order", &first_order, "a gradient of the running autograd node that must not be differentiated again");
   m.def("linear_fp8", &linear_fp8_autograd, "8-bit linear layer with its backward as an autograd node");
 }

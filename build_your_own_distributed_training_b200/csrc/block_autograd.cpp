@@ -3,6 +3,8 @@
 // to a forward and backward.  The Python layer keeps its own nodes for what belongs to the sharding engine
 // (gradients that go into its fp32 buffers) and for the CPU path; both call the same kernels.
 #include <torch/extension.h>
+#include <torch/csrc/autograd/functions/basic_ops.h>
+#include <torch/csrc/autograd/functions/utils.h>
 
 #include <cstdio>
 
@@ -28,6 +30,24 @@ void fp8_gemm(Tensor A, Tensor tA, Tensor B, Tensor tB, Tensor D, c10::optional<
 void fp8_product(Tensor A, Tensor sA, c10::optional<Tensor> tA, Tensor B, Tensor sB, c10::optional<Tensor> tB, Tensor D,
                  c10::optional<Tensor> R, bool accumulate);
 
+Tensor dropout_add_autograd(Tensor x, c10::optional<Tensor> residual, int64_t cut, int64_t seed, int64_t start);
+
+// A kernel's result has no graph: under create_graph a term through it would count as constant and be missing
+// from the second derivative without a word.  This lets the gradient g of the running node through and makes a
+// differentiation of it raise, for all that the node (or the gradients dys it was given) depends on.
+Tensor first_order(Tensor g, const std::string& op, const std::vector<Tensor>& dys) {
+  if (!g.defined() || !at::GradMode::is_enabled()) return g;
+  torch::autograd::edge_list edges;
+  if (const auto node = torch::autograd::get_current_node())
+    for (const auto& e : node->next_edges())
+      if (e.is_valid()) edges.push_back(e);
+  for (const Tensor& dy : dys)
+    if (dy.defined() && dy.requires_grad()) edges.push_back(torch::autograd::impl::gradient_edge(dy));
+  g = g.detach();
+  torch::autograd::set_history(g, std::make_shared<torch::autograd::Error>(op + " has no second derivative", std::move(edges)));
+  return g;
+}
+
 namespace {
 
 struct QkNormRope : public Function<QkNormRope> {
@@ -48,7 +68,8 @@ struct QkNormRope : public Function<QkNormRope> {
     Tensor dx = qk_norm_rope_bwd(g, s[0], s[1], s[2], s[3], s[4],
                                  s[5].defined() ? c10::optional<Tensor>(s[5]) : c10::nullopt, c[0], c[1], c[2], c[3],
                                  ctx->saved_data["eps"].toDouble(), dwq, dwk, false);
-    return {dx, dwq, dwk, {}, {}, {}, {}, {}, {}, {}, {}};
+    const char* op = "qk_norm_rope";
+    return {first_order(dx, op, grads), first_order(dwq, op, grads), first_order(dwk, op, grads), {}, {}, {}, {}, {}, {}, {}, {}};
   }
 };
 
@@ -61,7 +82,8 @@ struct DropoutAdd : public Function<DropoutAdd> {
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
     const auto c = ctx->saved_data["c"].toIntVector();
     Tensor dx;
-    if (ctx->needs_input_grad(0)) dx = dropout_add(grads[0].contiguous(), c10::nullopt, c[0], c[1], c[2]);
+    // (linear in the gradient: the same node again where the gradient is to be differentiated)
+    if (ctx->needs_input_grad(0)) dx = dropout_add_autograd(grads[0].contiguous(), c10::nullopt, c[0], c[1], c[2]);
     // an input that was not given takes no gradient
     return {dx, c[3] ? grads[0] : Tensor(), {}, {}, {}};
   }
@@ -92,7 +114,7 @@ struct TokenLogProbs : public Function<TokenLogProbs> {
     const Tensor gl = row_grad(grads[0]), ge = row_grad(grads[1]);  // (of the tokens' shape)
     token_logprobs_bwd(x, s[1], s[2], gl.defined() ? c10::optional<Tensor>(gl) : c10::nullopt,
                        ge.defined() ? c10::optional<Tensor>(ge) : c10::nullopt, ctx->saved_data["t"].toDouble(), dx);
-    return {dx, {}, {}, {}, {}};
+    return {first_order(dx, "token_log_probs", grads), {}, {}, {}, {}};
   }
 };
 
@@ -126,7 +148,7 @@ struct LinearFp8 : public Function<LinearFp8> {
         dw = dw.to(t);
       }
     }
-    return {dx, dw, ctx->saved_data["r"].toBool() ? grads[0] : Tensor()};
+    return {first_order(dx, "linear_fp8", grads), first_order(dw, "linear_fp8", grads), ctx->saved_data["r"].toBool() ? grads[0] : Tensor()};
   }
 };
 

@@ -24,6 +24,7 @@ import torch
 
 from . import grad_state
 from ._ext import native
+from .first_order import first_order
 
 BLOCK = 128
 E4M3, E8M0 = torch.float8_e4m3fn, torch.float8_e8m0fnu
@@ -129,21 +130,29 @@ class _LinearFp8Fn(torch.autograd.Function):
         xq, xt = _quantize(x2, False, True, need_w)
         wq, wt = _quantize(weight, True, True, need_x)
         y = fp8_matmul(xq, wq, residual=residual, out_dtype=x2.dtype)
-        ctx.save_for_backward(*(xt or (None,) * 3), *(wt or (None,) * 3))
+        inputs = () if x2.is_cuda else (x2, weight)  # what the gradients would depend on, see first_order
+        ctx.save_for_backward(*(xt or (None,) * 3), *(wt or (None,) * 3), *inputs)
         ctx.main_grad, ctx.need = main_grad, (need_x, need_w, residual is not None)
         ctx.wshape, ctx.wdtype = weight.shape, weight.dtype
         return y
 
     @staticmethod
     def backward(ctx, dy):  # type: ignore[override]
+        with torch.no_grad():
+            dx, dw = _LinearFp8Fn._gradients(ctx, dy)
+        dx, dw = (first_order("linear_fp8", t, (dy,), *ctx.saved_tensors[6:]) for t in (dx, dw))
+        return dx, dw, (dy if ctx.need[2] else None), None
+
+    @staticmethod
+    def _gradients(ctx, dy):
         saved = ctx.saved_tensors
-        need_x, need_w, has_res = ctx.need
+        need_x, need_w, _ = ctx.need
         dy2 = dy.contiguous()
         dx = dw = None
         if need_x or need_w:
             g, gt = _quantize(dy2, False, need_x, need_w)
         if need_x:
-            dx = fp8_matmul(g, Fp8Blocks(*saved[3:]), out_dtype=dy.dtype)
+            dx = fp8_matmul(g, Fp8Blocks(*saved[3:6]), out_dtype=dy.dtype)
         if need_w:
             mg, xt = ctx.main_grad, Fp8Blocks(*saved[:3])
             if mg is not None:
@@ -153,7 +162,7 @@ class _LinearFp8Fn(torch.autograd.Function):
                 wide = ctx.wdtype not in (torch.bfloat16, torch.float32)
                 dw = fp8_matmul(gt, xt, out_dtype=torch.float32 if wide else ctx.wdtype)
                 dw = dw.to(ctx.wdtype) if wide else dw
-        return dx, dw, (dy if has_res else None), None
+        return dx, dw
 
 
 def linear_fp8(x: torch.Tensor, weight: torch.Tensor | Fp8Blocks, *, residual: torch.Tensor | None = None,

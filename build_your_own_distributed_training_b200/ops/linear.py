@@ -21,6 +21,7 @@ import torch
 import torch.nn.functional as F
 
 from . import gemm
+from .first_order import first_order
 from .rope import rope_backward_, rope_forward
 
 
@@ -223,7 +224,11 @@ class _SwiGLUPackedFn(torch.autograd.Function):
     @staticmethod
     def backward(ctx, dact):  # type: ignore[override]
         (gu,) = ctx.saved_tensors
-        return swiglu_backward(dact, gu, ctx.ffn), None
+        if not gu.is_cuda:
+            return swiglu_backward(dact, gu, ctx.ffn), None
+        with torch.no_grad():
+            dgu = swiglu_backward(dact, gu, ctx.ffn)
+        return first_order("swiglu_packed", dgu, (dact,)), None
 
 
 def swiglu_packed(gu: torch.Tensor, ffn: int) -> torch.Tensor:

@@ -20,6 +20,7 @@ import torch.nn.functional as F
 
 from . import gemm, grad_state
 from ._ext import native
+from .first_order import first_order
 from .loss import IGNORE
 
 MAX_TOP_K = 32
@@ -172,6 +173,13 @@ class _HeadLogProbsFn(torch.autograd.Function):
 
     @staticmethod
     def backward(ctx, g_lp, g_ent, _v, _i):  # type: ignore[override]
+        with torch.no_grad():
+            dh, dw = _HeadLogProbsFn._gradients(ctx, g_lp, g_ent)
+        dh, dw = (first_order("lm_head_token_log_probs", t, (g_lp, g_ent)) for t in (dh, dw))
+        return dh, dw, None, None, None, None, None
+
+    @staticmethod
+    def _gradients(ctx, g_lp, g_ent):
         h, w, tokens, state = ctx.saved_tensors
         g_lp, g_ent, mg = _row_grad(g_lp), _row_grad(g_ent), ctx.main_grad
         need_w = mg is not None or w.requires_grad
@@ -197,7 +205,7 @@ class _HeadLogProbsFn(torch.autograd.Function):
             grad_state.zero_if_fresh(mg)
             mg.view(w.shape).add_(acc[:V])
         dw = acc[:V].to(w.dtype) if mg is None and need_w else None
-        return dh, dw, None, None, None, None, None
+        return dh, dw
 
 
 def lm_head_token_log_probs(h: torch.Tensor, weight: torch.Tensor, tokens: torch.Tensor, *, temperature: float = 1.0,

@@ -20,6 +20,7 @@ import torch
 
 from . import grad_state
 from ._ext import native
+from .first_order import first_order
 
 
 def _rotate(u: torch.Tensor, c: torch.Tensor, s: torch.Tensor) -> torch.Tensor:
@@ -76,6 +77,14 @@ class _QKNormRopeFn(torch.autograd.Function):
 
     @staticmethod
     def backward(ctx, g):  # type: ignore[override]
+        if not g.is_cuda and ctx.main_grads is None and ctx.reduce is None:
+            return _QKNormRopeFn._gradients(ctx, g) + (None,) * 10  # plain differentiable operations
+        with torch.no_grad():
+            grads = _QKNormRopeFn._gradients(ctx, g)
+        return tuple(first_order("qk_norm_rope", t, (g,), *ctx.saved_tensors[:3]) for t in grads) + (None,) * 10
+
+    @staticmethod
+    def _gradients(ctx, g):
         qkv, wq, wk, cos, sin, positions = ctx.saved_tensors
         nq, nkv, hd, seqlen, eps = ctx.cfg
         mgs = ctx.main_grads
@@ -107,7 +116,7 @@ class _QKNormRopeFn(torch.autograd.Function):
             dwq = dwk = None
         else:
             dwq, dwk = dwq.to(wq.dtype), dwk.to(wk.dtype)
-        return (dx, dwq, dwk) + (None,) * 10
+        return dx, dwq, dwk
 
 
 def qk_norm_rope(qkv: torch.Tensor, q_weight: torch.Tensor, k_weight: torch.Tensor, cos: torch.Tensor,

@@ -81,6 +81,8 @@ class _RopePackedFn(torch.autograd.Function):
     @staticmethod
     def backward(ctx, d):  # type: ignore[override]
         cos, sin = ctx.saved_tensors
+        if torch.is_grad_enabled():  # to be differentiated again: the transposed rotation as a call of its own
+            return _RopePackedFn.apply(d, cos, -sin, *ctx.cfg), None, None, None, None, None
         back = d.contiguous().clone()
         rope_backward_(back, cos, sin, *ctx.cfg)
         return back, None, None, None, None, None

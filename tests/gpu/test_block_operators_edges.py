@@ -160,3 +160,66 @@ def test_kept_weights_without_tiles(T, N, K, square):
     assert torch.equal(ops.linear_fp8(x, ops.Fp8Blocks(b.values.contiguous(), turned)), want)
     r = _randn(T, N, seed=5, dt=BF)
     assert torch.equal(ops.linear_fp8(x, ops.Fp8Blocks(b.values, b.scales), residual=r), ops.linear_fp8(x, b, residual=r))
+
+
+def _cases():
+    """(name, call, differentiated inputs): each operator as a program calls it."""
+    from build_your_own_distributed_training_b200.ops.linear import swiglu_packed
+    cos, sin = (t.to(DEV) for t in ops.precompute_rope_cache(16, 8, 10000.0))
+    x, w = _randn(8, 64, seed=1, dt=BF), _randn(24, 64, seed=2, dt=BF)
+    nw, tok = _randn(16, seed=3, dt=BF), torch.arange(8, device=DEV)
+    grads = lambda *n: [torch.zeros(m, device=DEV) for m in n]  # noqa: E731
+    qk = lambda **kw: lambda x, w: ops.qk_norm_rope(x, w, w, cos, sin, 2, 1, 16, 8, **kw)  # noqa: E731
+    lp = lambda r: r.logprob * 2 + r.entropy  # noqa: E731
+    return {
+        "qk_norm_rope": (qk(), (x, nw)),
+        "qk_norm_rope main_grads": (qk(main_grads=grads(16, 16)), (x, nw)),
+        "token_log_probs": (lambda x: lp(ops.token_log_probs(x, tok)), (x,)),
+        "lm_head_token_log_probs": (lambda x, w: lp(ops.lm_head_token_log_probs(x, w, tok)), (x, w)),
+        "linear_fp8": (lambda x, w: ops.linear_fp8(x, w), (x, w)),
+        "linear_fp8 main_grad": (lambda x, w: ops.linear_fp8(x, w, main_grad=grads(24 * 64)[0]), (x, w)),
+        "swiglu_packed": (lambda x: swiglu_packed(x, 32), (x,)),
+    }
+
+
+@pytest.mark.parametrize("name", ["qk_norm_rope", "qk_norm_rope main_grads", "token_log_probs", "lm_head_token_log_probs",
+                                  "linear_fp8", "linear_fp8 main_grad", "swiglu_packed"])
+def test_second_derivatives_are_refused(name):
+    f, args = _cases()[name]
+    args = [a.clone().requires_grad_(True) for a in args]
+    first = torch.autograd.grad(f(*args).float().sum(), args, allow_unused=True)
+    again = torch.autograd.grad(f(*args).float().sum(), args, create_graph=True, allow_unused=True)
+    for a, b in zip(first, again):
+        assert (a is None) == (b is None)
+        if a is not None:
+            assert torch.equal(a, b.detach())
+            # a term that is added to others must not vanish
+            with pytest.raises(RuntimeError, match="second derivative"):
+                torch.autograd.grad((b.float().sum() + args[0].float().pow(2).sum()), args[0], retain_graph=True)
+
+
+def test_second_derivatives_of_linear_operators():
+    from build_your_own_distributed_training_b200.ops.rope import rope_packed
+    x = _randn(6, 64, seed=1).requires_grad_(True)
+    m = ops.dropout_add(torch.ones_like(x), None, 0.3, 5)
+    xd = x.detach().double().requires_grad_(True)
+    for f, g, z in ((lambda t: ops.dropout_add(t, t * 2, 0.3, 5), lambda t: t * 2 + t * m.double(), x),):
+        a, = torch.autograd.grad(f(z).pow(3).sum(), z, create_graph=True)
+        b, = torch.autograd.grad(g(xd).pow(3).sum(), xd, create_graph=True)
+        v = _randn(6, 64, seed=2)
+        assert rel(torch.autograd.grad((a * v).sum(), z)[0], torch.autograd.grad((b * v.double()).sum(), xd)[0]) < 2.0 ** -20
+    cos, sin = (t.to(DEV) for t in ops.precompute_rope_cache(16, 3, 10000.0))
+    z, v = x.detach().to(BF).requires_grad_(True), _randn(6, 64, seed=2, dt=BF)
+    zd = z.detach().double().requires_grad_(True)
+
+    def turn(t):
+        u = t.view(2, 3, 4, 16)
+        c, s = cos.double()[None, :, None, :8], sin.double()[None, :, None, :8]
+        lo, hi = u[:, :, :3, :8], u[:, :, :3, 8:]
+        return torch.cat((torch.cat((lo * c - hi * s, hi * c + lo * s), -1), u[:, :, 3:]), 2).reshape(6, 64)
+    a, = torch.autograd.grad(rope_packed(z, cos, sin, 48, 16, 3).float().pow(3).sum(), z, create_graph=True)
+    b, = torch.autograd.grad(turn(zd).pow(3).sum(), zd, create_graph=True)
+    got, = torch.autograd.grad((a.float() * v.float()).sum(), z)
+    want, = torch.autograd.grad((b * v.double()).sum(), zd)
+    # four bf16 roundings on the way, one of a factor that the cube's derivative doubles
+    assert rel(got, want) < 6 * UNIT[BF]

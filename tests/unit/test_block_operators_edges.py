@@ -69,3 +69,46 @@ def test_log_prob_gradients_beside_the_lowest_value():
     row = torch.stack((-p[0] - p[0] * (p[0].log() + ent), 1 - p[1] - p[1] * (p[1].log() + ent))) / 0.5
     assert rel(g[1, [0, 2]], row) < F32 and (g[1, [1, 3]] == 0).all()
     assert torch.autograd.grad(g.sum(), x)[0].isfinite().all()
+
+
+def test_second_derivatives_of_the_other_operators():
+    from build_your_own_distributed_training_b200.ops.linear import swiglu_packed
+    from build_your_own_distributed_training_b200.ops.rope import rope_packed
+    g = torch.Generator().manual_seed(2)
+    x, v = torch.randn(6, 64, generator=g), torch.randn(6, 64, generator=g)
+    wq, wk = torch.randn(16, generator=g), torch.randn(16, generator=g)
+    cos, sin = ops.precompute_rope_cache(16, 3, 10000.0)
+    mask = ops.dropout_add(torch.ones_like(x), None, 0.3, 5).double()
+    pos = [0, 1, 2, 0, 1, 2]
+    turn = lambda t: plain.qk_norm_rope(t, 1.0, 1.0, cos, sin, 2, 1, 16, pos, 0.0)  # noqa: E731
+
+    def rotated(t):  # a head of unit rms is only rotated
+        u = t.view(6, 4, 16)
+        r = u.square().mean(-1, keepdim=True).sqrt()
+        return (turn(t).view(6, 4, 16) * torch.cat((r[:, :3], torch.ones_like(r[:, 3:])), 1)).reshape(6, 64)
+    for f, ref in ((lambda t: ops.qk_norm_rope(t, wq, wk, cos, sin, 2, 1, 16, 3),
+                    lambda t: plain.qk_norm_rope(t, wq.double(), wk.double(), cos, sin, 2, 1, 16, pos, 1e-5)),
+                   (lambda t: ops.dropout_add(t, None, 0.3, 5), lambda t: t * mask),
+                   (lambda t: swiglu_packed(t, 32), lambda t: torch.nn.functional.silu(t[:, :32]) * t[:, 32:]),
+                   (lambda t: rope_packed(t, cos, sin, 48, 16, 3), rotated)):
+        got = _hessian_product(lambda t: f(t).pow(3).sum(), x.clone().requires_grad_(True), v)
+        want = _hessian_product(lambda t: ref(t).pow(3).sum(), x.double().requires_grad_(True), v.double())
+        assert rel(got, want) < 4 * F32
+
+
+@pytest.mark.parametrize("name", ["linear_fp8", "linear_fp8 main_grad", "qk_norm_rope main_grads"])
+def test_second_derivatives_that_do_not_exist_are_refused(name):
+    """Rounded operands, and gradients that went into the engine's buffers."""
+    g = torch.Generator().manual_seed(3)
+    x, w, nw = (torch.randn(*s, generator=g).requires_grad_(True) for s in ((8, 64), (24, 64), (16,)))
+    cos, sin = ops.precompute_rope_cache(16, 8, 10000.0)
+    f, args = {"linear_fp8": (lambda: ops.linear_fp8(x, w), (x, w)),
+               "linear_fp8 main_grad": (lambda: ops.linear_fp8(x, w, main_grad=torch.zeros(24 * 64)), (x,)),
+               "qk_norm_rope main_grads": (lambda: ops.qk_norm_rope(x, nw, nw, cos, sin, 2, 1, 16, 8, main_grads=(
+                   torch.zeros(16), torch.zeros(16))), (x,))}[name]
+    first = torch.autograd.grad(f().sum(), args)
+    again = torch.autograd.grad(f().sum(), args, create_graph=True)
+    for a, b in zip(first, again):
+        assert torch.equal(a, b.detach())
+        with pytest.raises(RuntimeError, match="second derivative"):
+            torch.autograd.grad(b.sum() + x.pow(2).sum(), x, retain_graph=True)
