@@ -154,8 +154,10 @@ struct LinearFp8 : public Function<LinearFp8> {
 
 }  // namespace
 
-// (a call that nothing will differentiate skips the node)
-static bool tracked(const Tensor& t) { return t.requires_grad() && at::GradMode::is_enabled(); }
+// A call that nothing will differentiate skips the node.  A tangent (forward mode, which works without grad mode)
+// goes to the node, which refuses it.
+static bool has_tangent(const Tensor& t) { return t._fw_grad(/*level=*/0).defined(); }
+static bool tracked(const Tensor& t) { return (t.requires_grad() && at::GradMode::is_enabled()) || has_tangent(t); }
 
 Tensor qk_norm_rope_autograd(Tensor x, Tensor wq, Tensor wk, Tensor cos_t, Tensor sin_t, c10::optional<Tensor> pos,
                              int64_t nq, int64_t nkv, int64_t hd, int64_t seqlen, double eps) {
@@ -195,6 +197,8 @@ void fp8_check_blocks(const Tensor& q, const Tensor& s) {
 Tensor linear_fp8_kept(Tensor x, Tensor values, Tensor scales, c10::optional<Tensor> tiles,
                        c10::optional<Tensor> residual) {
   fp8_check_blocks(values, scales);
+  TORCH_CHECK(!has_tangent(x) && !(residual.has_value() && has_tangent(*residual)),
+              "weights kept in 8 bits have no derivative: call linear_fp8 with the weight tensor");
   auto xq = tiles.has_value() ? fp8_quantize(x, false, true, false) : fp8_quantize_with_tiles(x, scales, values.size(0));
   Tensor y = torch::empty({x.size(0), values.size(0)}, x.options());
   fp8_product(xq[0], xq[1], xq[2], values, scales, tiles.has_value() ? tiles : xq[3], y, residual, false);

@@ -21,6 +21,7 @@ from __future__ import annotations
 from typing import NamedTuple
 
 import torch
+import torch.autograd.forward_ad as fwd
 
 from . import grad_state
 from ._ext import native
@@ -190,7 +191,9 @@ def linear_fp8(x: torch.Tensor, weight: torch.Tensor | Fp8Blocks, *, residual: t
             raise ValueError("weights kept in 8 bits have no backward: call linear_fp8 with the weight tensor")
         if x.is_cuda:
             y = native().linear_fp8_kept(x2, *weight, r2)
-        else:
+        else:  # (tangents: the native call above looks for them itself)
+            if any(t is not None and fwd.unpack_dual(t).tangent is not None for t in (x, residual)):
+                raise ValueError("weights kept in 8 bits have no derivative: call linear_fp8 with the weight tensor")
             y = fp8_matmul(_quantize(x2, False, True, False)[0], weight, residual=r2, out_dtype=x.dtype)
     else:
         w = weight if weight.is_contiguous() else weight.contiguous()

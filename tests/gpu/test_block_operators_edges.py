@@ -223,3 +223,24 @@ def test_second_derivatives_of_linear_operators():
     want, = torch.autograd.grad((b * v.double()).sum(), zd)
     # four bf16 roundings on the way, one of a factor that the cube's derivative doubles
     assert rel(got, want) < 6 * UNIT[BF]
+
+
+@pytest.mark.parametrize("name", ["qk_norm_rope", "qk_norm_rope main_grads", "token_log_probs", "lm_head_token_log_probs",
+                                  "linear_fp8", "linear_fp8 main_grad", "swiglu_packed", "dropout_add", "residual", "kept weights",
+                                  "kept weights residual"])
+@pytest.mark.parametrize("grad", [False, True])
+def test_tangents_are_refused(name, grad):
+    """Forward-mode differentiation has no kernels here; a tangent must not get lost on the way."""
+    import torch.autograd.forward_ad as fwd
+    x, w, r = _randn(8, 64, seed=1, dt=BF), ops.quantize_fp8(_randn(24, 64, seed=2), square=True), _randn(8, 24, dt=BF)
+    cases = dict(_cases(), **{"dropout_add": (lambda x: ops.dropout_add(x, None, 0.3, 5), (x,)),
+                              "residual": (lambda x: ops.dropout_add(x.detach(), x, 0.3, 5), (x,)),
+                              "kept weights": (lambda x: ops.linear_fp8(x, w), (x,)),
+                              "kept weights residual": (lambda r: ops.linear_fp8(x, w, residual=r), (r,))})
+    f, args = cases[name]
+    with fwd.dual_level(), torch.set_grad_enabled(grad):
+        duals = [fwd.make_dual(a, torch.ones_like(a)) for a in args]
+        with pytest.raises((RuntimeError, ValueError)):
+            f(*duals)
+        plain_call = f(*args)  # without tangents the same call goes through
+        assert plain_call.shape[0] == 8

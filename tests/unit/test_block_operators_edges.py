@@ -112,3 +112,22 @@ def test_second_derivatives_that_do_not_exist_are_refused(name):
         assert torch.equal(a, b.detach())
         with pytest.raises(RuntimeError, match="second derivative"):
             torch.autograd.grad(b.sum() + x.pow(2).sum(), x, retain_graph=True)
+
+
+@pytest.mark.parametrize("name", ["qk_norm_rope", "dropout_add", "token_log_probs", "linear_fp8", "kept weights",
+                                  "kept weights residual"])
+def test_tangents_are_refused(name):
+    import torch.autograd.forward_ad as fwd
+    x, w, nw, r = torch.randn(8, 64), torch.randn(24, 64), torch.ones(16), torch.zeros(8, 24)
+    cos, sin = ops.precompute_rope_cache(16, 8, 10000.0)
+    kept = ops.quantize_fp8(w, square=True)
+    f, t = {"qk_norm_rope": (lambda x: ops.qk_norm_rope(x, nw, nw, cos, sin, 2, 1, 16, 8), x),
+            "dropout_add": (lambda x: ops.dropout_add(x, None, 0.3, 5), x),
+            "token_log_probs": (lambda x: ops.token_log_probs(x, torch.arange(8)).logprob, x),
+            "linear_fp8": (lambda x: ops.linear_fp8(x, w), x),
+            "kept weights": (lambda x: ops.linear_fp8(x, kept), x),
+            "kept weights residual": (lambda r: ops.linear_fp8(x, kept, residual=r), r)}[name]
+    with fwd.dual_level():
+        with pytest.raises((RuntimeError, ValueError)):
+            f(fwd.make_dual(t, torch.ones_like(t)))
+        assert f(t).shape[0] == 8
