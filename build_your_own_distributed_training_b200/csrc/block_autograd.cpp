@@ -178,6 +178,13 @@ std::vector<Tensor> token_logprobs_autograd(Tensor x, Tensor tokens, double temp
 }
 // x [T, K] bf16, w [N, K], residual [T, N] bf16 or none
 Tensor linear_fp8_autograd(Tensor x, Tensor w, c10::optional<Tensor> residual) {
+  if (!tracked(x) && !tracked(w) && !(residual.has_value() && tracked(*residual))) {
+    // no backward: codes as they lie alone (8192 x 4096: 24 us instead of 34)
+    auto xq = fp8_quantize_tiles(x, false, true, false), wq = fp8_quantize_tiles(w, true, true, false);
+    Tensor y = torch::empty({x.size(0), w.size(0)}, x.options());
+    fp8_gemm(xq[0], xq[1], wq[0], wq[1], y, residual, false);
+    return y;
+  }
   return LinearFp8::apply(x, w, residual);
 }
 

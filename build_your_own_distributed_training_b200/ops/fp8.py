@@ -126,8 +126,9 @@ def fp8_matmul(a: Fp8Blocks, b: Fp8Blocks, *, residual: torch.Tensor | None = No
 
 class _LinearFp8Fn(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, x2, weight, residual, main_grad):  # type: ignore[override]
-        need_x, need_w = ctx.needs_input_grad[0], ctx.needs_input_grad[1] or main_grad is not None
+    def forward(ctx, x2, weight, residual, main_grad, grad):  # type: ignore[override]
+        # transposed codes are for the backward: none without gradients, whatever the tensors ask for
+        need_x, need_w = grad and ctx.needs_input_grad[0], grad and (ctx.needs_input_grad[1] or main_grad is not None)
         xq, xt = _quantize(x2, False, True, need_w)
         wq, wt = _quantize(weight, True, True, need_x)
         y = fp8_matmul(xq, wq, residual=residual, out_dtype=x2.dtype)
@@ -142,7 +143,7 @@ class _LinearFp8Fn(torch.autograd.Function):
         with torch.no_grad():
             dx, dw = _LinearFp8Fn._gradients(ctx, dy)
         dx, dw = (first_order("linear_fp8", t, (dy,), *ctx.saved_tensors[6:]) for t in (dx, dw))
-        return dx, dw, (dy if ctx.need[2] else None), None
+        return dx, dw, (dy if ctx.need[2] else None), None, None
 
     @staticmethod
     def _gradients(ctx, dy):
@@ -197,5 +198,8 @@ def linear_fp8(x: torch.Tensor, weight: torch.Tensor | Fp8Blocks, *, residual: t
             y = fp8_matmul(_quantize(x2, False, True, False)[0], weight, residual=r2, out_dtype=x.dtype)
     else:
         w = weight if weight.is_contiguous() else weight.contiguous()
-        y = native().linear_fp8(x2, w, r2) if x.is_cuda and main_grad is None else _LinearFp8Fn.apply(x2, w, r2, main_grad)
+        if x.is_cuda and main_grad is None:
+            y = native().linear_fp8(x2, w, r2)
+        else:
+            y = _LinearFp8Fn.apply(x2, w, r2, main_grad, torch.is_grad_enabled())
     return y.view(*x.shape[:-1], N)

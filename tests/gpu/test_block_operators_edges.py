@@ -244,3 +244,21 @@ def test_tangents_are_refused(name, grad):
             f(*duals)
         plain_call = f(*args)  # without tangents the same call goes through
         assert plain_call.shape[0] == 8
+
+
+@pytest.mark.parametrize("route", ["plain", "main_grad"])
+def test_a_call_without_gradients_makes_one_set_of_codes(route):
+    """The transposed codes serve the backward only."""
+    T, N, K = 2048, 512, 4096
+    x, w = _randn(T, K, seed=1, dt=BF).requires_grad_(True), _randn(N, K, seed=2, dt=BF).requires_grad_(True)
+    kw = {"main_grad": torch.zeros(N, K, device=DEV)} if route == "main_grad" else {}
+    want = ops.linear_fp8(x, w, **kw).detach()
+    torch.cuda.synchronize()
+    before = torch.cuda.memory_allocated()
+    torch.cuda.reset_peak_memory_stats()
+    with torch.no_grad():
+        y = ops.linear_fp8(x, w, **kw)
+    peak = torch.cuda.max_memory_allocated() - before
+    assert torch.equal(y, want) and not y.requires_grad
+    # the codes once, the result, the scales (a 128th of the codes, up to twice as tiles), allocations in 2 MB steps at most
+    assert peak < T * K + N * K + 2 * T * N + (T + N) * K // 32 + (2 << 20)

@@ -131,3 +131,16 @@ def test_tangents_are_refused(name):
         with pytest.raises((RuntimeError, ValueError)):
             f(fwd.make_dual(t, torch.ones_like(t)))
         assert f(t).shape[0] == 8
+
+
+@pytest.mark.parametrize("grad,x_grad,w_grad,main,sets", [
+    (True, True, True, False, 4), (True, False, True, False, 3), (True, True, False, False, 3), (True, True, False, True, 4),
+    (False, True, True, False, 2), (False, True, False, True, 2), (True, False, False, False, 2)])
+def test_transposed_codes_are_made_for_a_backward_alone(grad, x_grad, w_grad, main, sets, monkeypatch):
+    from build_your_own_distributed_training_b200.ops import fp8
+    made, inner = [], fp8._quantize
+    monkeypatch.setattr(fp8, "_quantize", lambda x, square, plain, t: made.append(plain + t) or inner(x, square, plain, t))
+    x, w = torch.randn(8, 64).requires_grad_(x_grad), torch.randn(24, 64).requires_grad_(w_grad)
+    with torch.set_grad_enabled(grad):
+        ops.linear_fp8(x, w, main_grad=torch.zeros(24, 64) if main else None)
+    assert sum(made) == sets
