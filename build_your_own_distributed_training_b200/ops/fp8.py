@@ -130,10 +130,14 @@ class _LinearFp8Fn(torch.autograd.Function):
         # transposed codes are for the backward: none without gradients, whatever the tensors ask for
         need_x, need_w = grad and ctx.needs_input_grad[0], grad and (ctx.needs_input_grad[1] or main_grad is not None)
         xq, xt = _quantize(x2, False, True, need_w)
-        wq, wt = _quantize(weight, True, True, need_x)
+        # the engine's weight is a view that it fills again for the backward: keeping that costs no memory, keeping
+        # codes would hold a byte of every layer's weight on every rank, so the backward makes them again
+        again = need_x and main_grad is not None
+        wq, wt = _quantize(weight, True, True, need_x and not again)
         y = fp8_matmul(xq, wq, residual=residual, out_dtype=x2.dtype)
-        inputs = () if x2.is_cuda else (x2, weight)  # what the gradients would depend on, see first_order
-        ctx.save_for_backward(*(xt or (None,) * 3), *(wt or (None,) * 3), *inputs)
+        on_cpu = not x2.is_cuda  # there first_order wants what the gradients would depend on
+        ctx.save_for_backward(*(xt or (None,) * 3), *(wt or (None,) * 3), weight if again or on_cpu else None,
+                              x2 if on_cpu else None)
         ctx.main_grad, ctx.need = main_grad, (need_x, need_w, residual is not None)
         ctx.wshape, ctx.wdtype = weight.shape, weight.dtype
         return y
@@ -142,7 +146,7 @@ class _LinearFp8Fn(torch.autograd.Function):
     def backward(ctx, dy):  # type: ignore[override]
         with torch.no_grad():
             dx, dw = _LinearFp8Fn._gradients(ctx, dy)
-        dx, dw = (first_order("linear_fp8", t, (dy,), *ctx.saved_tensors[6:]) for t in (dx, dw))
+        dx, dw = (first_order("linear_fp8", t, (dy,), *(s for s in ctx.saved_tensors[6:] if s is not None)) for t in (dx, dw))
         return dx, dw, (dy if ctx.need[2] else None), None, None
 
     @staticmethod
@@ -154,7 +158,8 @@ class _LinearFp8Fn(torch.autograd.Function):
         if need_x or need_w:
             g, gt = _quantize(dy2, False, need_x, need_w)
         if need_x:
-            dx = fp8_matmul(g, Fp8Blocks(*saved[3:6]), out_dtype=dy.dtype)
+            wt = Fp8Blocks(*saved[3:6]) if saved[3] is not None else _quantize(saved[6], True, False, True)[1]
+            dx = fp8_matmul(g, wt, out_dtype=dy.dtype)
         if need_w:
             mg, xt = ctx.main_grad, Fp8Blocks(*saved[:3])
             if mg is not None:

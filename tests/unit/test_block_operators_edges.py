@@ -134,7 +134,7 @@ def test_tangents_are_refused(name):
 
 
 @pytest.mark.parametrize("grad,x_grad,w_grad,main,sets", [
-    (True, True, True, False, 4), (True, False, True, False, 3), (True, True, False, False, 3), (True, True, False, True, 4),
+    (True, True, True, False, 4), (True, False, True, False, 3), (True, True, False, False, 3), (True, True, False, True, 3),
     (False, True, True, False, 2), (False, True, False, True, 2), (True, False, False, False, 2)])
 def test_transposed_codes_are_made_for_a_backward_alone(grad, x_grad, w_grad, main, sets, monkeypatch):
     from build_your_own_distributed_training_b200.ops import fp8
@@ -144,3 +144,16 @@ def test_transposed_codes_are_made_for_a_backward_alone(grad, x_grad, w_grad, ma
     with torch.set_grad_enabled(grad):
         ops.linear_fp8(x, w, main_grad=torch.zeros(24, 64) if main else None)
     assert sum(made) == sets
+
+
+@pytest.mark.parametrize("main", [True, False])
+def test_the_engine_route_keeps_no_copy_of_the_weight(main):
+    """The sharding engine frees gathered weights between forward and backward; codes of them would stay."""
+    x, w = torch.randn(8, 256).requires_grad_(True), torch.randn(384, 256).requires_grad_(not main)
+    kept = []
+    with torch.autograd.graph.saved_tensors_hooks(lambda t: kept.append(t) or t, lambda t: t):
+        y = ops.linear_fp8(x, w, main_grad=torch.zeros(384, 256) if main else None)
+    extra = sum(t.numel() * t.element_size() for t in kept if t.data_ptr() not in (x.data_ptr(), w.data_ptr()))
+    codes = w.numel()
+    assert extra < codes if main else extra >= codes
+    y.sum().backward()
