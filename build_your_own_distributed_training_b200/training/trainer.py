@@ -37,7 +37,7 @@ from ..observability.profiler import build_profiler
 from ..parallel.fsdp import apply_activation_checkpointing, wrap_model_with_fsdp
 from ..parallel.process_groups import ProcessContext, build_process_context
 from ..parallel.tensor_parallel import apply_tensor_parallelism
-from ..utils.seed import seed_everything
+from ..utils.seed import get_rng_state, seed_everything, set_rng_state
 from .loop import eval_step, train_step
 from .optimizer import build_optimizer
 from .scheduler import build_scheduler
@@ -141,10 +141,14 @@ class Trainer:
             self._epoch += 1
 
     def _fast_forward_data(self, step: int) -> None:
+        # starting the loader draws from the generators that the checkpoint restored (residual dropout takes its
+        # seeds from one of them): put their state back
+        state = get_rng_state()
         self._epoch = 0
         self._train_iter = self._batch_iterator()
         for _ in range(step * self.config.grad_accum_steps):
             next(self._train_iter)
+        set_rng_state(state)
 
     def _next_window(self) -> tuple[list[Any], float]:
         if self._train_iter is None:
