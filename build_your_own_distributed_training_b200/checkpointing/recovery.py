@@ -15,7 +15,7 @@ from typing import Any
 from .checkpoint import META_FILE, SUCCESS_MARKER, safe_load
 
 MODEL_CONFIG_KEYS = ("vocab_size", "d_model", "n_layers", "n_heads", "n_kv_heads",
-                     "ffn_hidden_size", "max_seq_len")
+                     "ffn_hidden_size", "max_seq_len", "qk_norm")
 
 
 class CheckpointValidationError(Exception):
