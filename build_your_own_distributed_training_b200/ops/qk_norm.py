@@ -31,8 +31,13 @@ def _rotate(u: torch.Tensor, c: torch.Tensor, s: torch.Tensor) -> torch.Tensor:
 
 def _tables(cos: torch.Tensor, sin: torch.Tensor, positions: torch.Tensor | None, tokens: int, seqlen: int,
             hd: int) -> tuple[torch.Tensor, torch.Tensor]:
-    pos = torch.arange(tokens, device=cos.device) % seqlen if positions is None else positions.long()
-    return cos[pos, None, : hd // 2].float(), sin[pos, None, : hd // 2].float()
+    if positions is None:
+        pos = torch.arange(tokens, device=cos.device) % seqlen
+        return cos[pos, None, : hd // 2].float(), sin[pos, None, : hd // 2].float()
+    out = ((positions < 0) | (positions >= cos.shape[0]))[:, None, None]  # no such position: NaN heads
+    pos = positions.long().clamp(0, cos.shape[0] - 1)
+    c, s = (t[pos, None, : hd // 2].float().masked_fill(out, float("nan")) for t in (cos, sin))
+    return c, s
 
 
 def qk_norm_rope_reference(qkv: torch.Tensor, q_weight: torch.Tensor, k_weight: torch.Tensor, cos: torch.Tensor,

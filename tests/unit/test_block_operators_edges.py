@@ -157,3 +157,17 @@ def test_the_engine_route_keeps_no_copy_of_the_weight(main):
     codes = w.numel()
     assert extra < codes if main else extra >= codes
     y.sum().backward()
+
+
+@pytest.mark.parametrize("dt", [torch.int64, torch.int32])
+def test_positions_outside_the_tables_give_nan(dt):
+    cos, sin = ops.precompute_rope_cache(16, 8, 10000.0)
+    x, w = torch.randn(5, 64).requires_grad_(True), torch.ones(16)
+    pos = torch.tensor([-1, 0, 8, 7, -9], dtype=dt)
+    y = ops.qk_norm_rope(x, w, w, cos, sin, 2, 1, 16, 1, positions=pos)
+    bad = torch.tensor([True, False, True, False, True])
+    assert y[bad][:, :48].isnan().all() and torch.equal(y[bad][:, 48:], x[bad][:, 48:]) and y[~bad].isfinite().all()
+    good = ops.qk_norm_rope(x[~bad], w, w, cos, sin, 2, 1, 16, 1, positions=pos[~bad])
+    assert torch.equal(y[~bad], good)
+    g, = torch.autograd.grad(y.nan_to_num(0.0).sum(), x)
+    assert g[~bad].isfinite().all()
