@@ -92,20 +92,28 @@ def quantize_fp8(x: torch.Tensor, *, square: bool = False) -> Fp8Blocks:
         raise ValueError(f"quantize_fp8 takes a matrix, got {tuple(x.shape)}")
     if not x.is_floating_point() or x.dtype.itemsize not in (2, 4):
         raise ValueError(f"quantize_fp8 takes fp32, bf16 or fp16, got {x.dtype}")
+    x = x.detach()  # codes have no derivative
     if x.shape[1] > 1 and x.stride(1) != 1:
         x = x.contiguous()
     return _quantize(x, square, True, False)[0]
 
 
+def _wants_grad(t: torch.Tensor) -> bool:
+    return t.requires_grad and torch.is_grad_enabled()
+
+
 def fp8_matmul(a: Fp8Blocks, b: Fp8Blocks, *, residual: torch.Tensor | None = None, out: torch.Tensor | None = None,
                out_dtype: torch.dtype = torch.bfloat16, accumulate: bool = False) -> torch.Tensor:
-    """``a [M, K] @ b [N, K]^T (+ residual)`` in bf16 or fp32; ``accumulate`` adds to the fp32 ``out``."""
+    """``a [M, K] @ b [N, K]^T (+ residual)`` in bf16 or fp32; ``accumulate`` adds to the fp32 ``out``.
+    Has no backward (:func:`linear_fp8` has)."""
     if a.values.shape[1] != b.values.shape[1]:
         raise ValueError(f"summed axes differ: {tuple(a.values.shape)} and {tuple(b.values.shape)}")
     for t in (a, b):
         if t.values.dtype != E4M3 or t.scales.dtype != E8M0:
             raise ValueError(f"fp8_matmul takes e4m3 codes with e8m0 scales, got {t.values.dtype} and {t.scales.dtype}")
         t.rows_per_scale  # noqa: B018 - raises when the scales do not fit
+    if any(t is not None and (_wants_grad(t) or fwd.unpack_dual(t).tangent is not None) for t in (residual, out)):
+        raise ValueError("fp8_matmul has no backward: call linear_fp8 for the gradient of a residual")
     shape = (a.values.shape[0], b.values.shape[0])
     if out is None:
         if accumulate:
@@ -193,7 +201,7 @@ def linear_fp8(x: torch.Tensor, weight: torch.Tensor | Fp8Blocks, *, residual: t
         x2 = x2.contiguous()
     r2 = None if residual is None else residual.reshape(-1, N).contiguous()
     if isinstance(weight, Fp8Blocks):
-        if torch.is_grad_enabled() and (x.requires_grad or (residual is not None and residual.requires_grad)):
+        if _wants_grad(x) or (residual is not None and _wants_grad(residual)):
             raise ValueError("weights kept in 8 bits have no backward: call linear_fp8 with the weight tensor")
         if x.is_cuda:
             y = native().linear_fp8_kept(x2, *weight, r2)

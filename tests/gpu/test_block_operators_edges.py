@@ -262,3 +262,22 @@ def test_a_call_without_gradients_makes_one_set_of_codes(route):
     assert torch.equal(y, want) and not y.requires_grad
     # the codes once, the result, the scales (a 128th of the codes, up to twice as tiles), allocations in 2 MB steps at most
     assert peak < T * K + N * K + 2 * T * N + (T + N) * K // 32 + (2 << 20)
+
+
+def test_products_and_codes_do_not_drop_gradients():
+    """fp8_matmul and quantize_fp8 are no autograd operations: a residual that wants its gradient is refused."""
+    import torch.autograd.forward_ad as fwd
+    w = torch.randn(24, 64, device=DEV, requires_grad=True)
+    a, b = ops.quantize_fp8(torch.randn(8, 64, device=DEV)), ops.quantize_fp8(w, square=True)
+    assert not b.values.requires_grad and not b.scales.requires_grad and not b.dequantize().requires_grad
+    r = torch.zeros(8, 24, device=DEV, dtype=torch.bfloat16, requires_grad=True)
+    with pytest.raises(ValueError, match="linear_fp8"):
+        ops.fp8_matmul(a, b, residual=r)
+    with pytest.raises(ValueError, match="linear_fp8"):
+        ops.fp8_matmul(a, b, out=r * 1.0)
+    with fwd.dual_level(), pytest.raises(ValueError, match="linear_fp8"):
+        ops.fp8_matmul(a, b, residual=fwd.make_dual(r.detach(), torch.ones_like(r)))
+    want = ops.fp8_matmul(a, b)
+    assert not want.requires_grad
+    with torch.no_grad():
+        assert torch.equal(ops.fp8_matmul(a, b, residual=r), want)

@@ -171,3 +171,22 @@ def test_positions_outside_the_tables_give_nan(dt):
     assert torch.equal(y[~bad], good)
     g, = torch.autograd.grad(y.nan_to_num(0.0).sum(), x)
     assert g[~bad].isfinite().all()
+
+
+def test_products_and_codes_do_not_drop_gradients():
+    """fp8_matmul and quantize_fp8 are no autograd operations: a residual that wants its gradient is refused."""
+    import torch.autograd.forward_ad as fwd
+    w = torch.randn(24, 64, requires_grad=True)
+    a, b = ops.quantize_fp8(torch.randn(8, 64)), ops.quantize_fp8(w, square=True)
+    assert not b.values.requires_grad and not b.scales.requires_grad and not b.dequantize().requires_grad
+    r = torch.zeros(8, 24, dtype=torch.bfloat16, requires_grad=True)
+    with pytest.raises(ValueError, match="linear_fp8"):
+        ops.fp8_matmul(a, b, residual=r)
+    with pytest.raises(ValueError, match="linear_fp8"):
+        ops.fp8_matmul(a, b, out=r * 1.0)
+    with fwd.dual_level(), pytest.raises(ValueError, match="linear_fp8"):
+        ops.fp8_matmul(a, b, residual=fwd.make_dual(r.detach(), torch.ones_like(r)))
+    want = ops.fp8_matmul(a, b)
+    assert not want.requires_grad
+    with torch.no_grad():
+        assert torch.equal(ops.fp8_matmul(a, b, residual=r), want)
