@@ -470,7 +470,7 @@ using namespace dtb;
 static void lp_check_logits(const char* op, const torch::Tensor& x, const torch::Tensor& tokens, double temperature) {
   DTB_CHECK(x.is_cuda() && x.dim() == 2 && is_float_type(x.scalar_type()) && x.size(1) > 0 && x.size(1) < (1L << 30) && (x.numel() == 0 || x.size(1) == 1 || x.stride(1) == 1), "%s: logits must be a 2-D CUDA tensor of fp32, bf16 or fp16 with contiguous columns", op);
   DTB_CHECK(tokens.device() == x.device() && tokens.scalar_type() == at::kLong && tokens.is_contiguous() && tokens.numel() == x.size(0), "%s: tokens must be contiguous int64, one per row, on the logits' device", op);
-  DTB_CHECK(temperature > 0, "%s: temperature must be positive", op);
+  DTB_CHECK(temperature >= 0x1p-126 && temperature <= 0x1p126, "%s: temperature must lie in [2^-126, 2^126]", op);
 }
 
 // x [M, V], tokens of any shape with M entries -> {logprob, entropy} of the tokens' shape, then {top log

@@ -113,8 +113,8 @@ def _check(tokens: torch.Tensor, rows: torch.Size, vocab: int, temperature: floa
         raise ValueError(f"tokens {tuple(tokens.shape)} do not match the logits' rows {tuple(rows)}")
     if tokens.dtype != torch.int64:
         raise ValueError(f"tokens must be int64, got {tokens.dtype}")
-    if not temperature > 0:
-        raise ValueError(f"temperature must be positive, got {temperature}")
+    if not 2.0 ** -126 <= temperature <= 2.0 ** 126:  # fp32 holds the reciprocal
+        raise ValueError(f"temperature must be positive, in [2^-126, 2^126], got {temperature}")
     if not 0 <= top_k <= min(MAX_TOP_K, vocab):
         raise ValueError(f"top_k={top_k} is outside [0, {min(MAX_TOP_K, vocab)}]")
 

@@ -190,3 +190,15 @@ def test_products_and_codes_do_not_drop_gradients():
     assert not want.requires_grad
     with torch.no_grad():
         assert torch.equal(ops.fp8_matmul(a, b, residual=r), want)
+
+
+@pytest.mark.parametrize("temperature", [1e-46, 1e-40, 2.0 ** -127, 2.0 ** 127, 1e39, float("inf")])
+def test_temperatures_whose_reciprocal_fp32_cannot_hold_are_refused(temperature):
+    x, tok = torch.randn(3, 40), torch.zeros(3, dtype=torch.int64)
+    with pytest.raises(ValueError, match="temperature"):
+        ops.token_log_probs(x, tok, temperature=temperature)
+    for t in (2.0 ** -126, 2.0 ** 126):  # the ends: all on the maximum, and uniform
+        x[:, 5] = -float("inf")
+        r = ops.token_log_probs(x, tok, temperature=t)
+        n = 1 if t < 1 else 39
+        assert float((r.entropy - torch.log(torch.tensor(float(n)))).abs().max()) < 2.0 ** -18 and not r.logprob.isnan().any()
