@@ -389,6 +389,19 @@ __global__ void swiglu_bwd_kernel(const __nv_bfloat16* __restrict__ da, const __
   }
 }
 
+// Same arithmetic, one element at a time: odd F, or tensors that do not start on 4 bytes.
+__global__ void swiglu_bwd_one_kernel(const __nv_bfloat16* __restrict__ da, const __nv_bfloat16* __restrict__ gu,
+                                      __nv_bfloat16* __restrict__ dgu, int M, int F) {
+  const long total = (long)M * F;
+  for (long i = blockIdx.x * (long)blockDim.x + threadIdx.x; i < total; i += (long)gridDim.x * blockDim.x) {
+    const long g_at = i / F * 2L * F + i % F;
+    const float a = __bfloat162float(da[i]), g = __bfloat162float(gu[g_at]), u = __bfloat162float(gu[g_at + F]);
+    const float sg = 1.f / (1.f + expf(-g));
+    dgu[g_at] = __float2bfloat16_rn(a * u * sg * (1.f + g * (1.f - sg)));
+    dgu[g_at + F] = __float2bfloat16_rn(a * (g * sg));
+  }
+}
+
 // Same arithmetic, eight elements per thread with 16-byte accesses (F % 8 == 0).
 __global__ void swiglu_bwd_vec8_kernel(const __nv_bfloat16* __restrict__ da, const __nv_bfloat16* __restrict__ gu,
                                        __nv_bfloat16* __restrict__ dgu, int M, int F) {
@@ -806,11 +819,22 @@ void rope_fwd(torch::Tensor d, torch::Tensor c, torch::Tensor s, int64_t rc, int
 void swiglu_bwd(torch::Tensor da, torch::Tensor gu, torch::Tensor dgu) {
   const c10::cuda::CUDAGuard g(da.device());
   const int M = (int)da.size(0), F = (int)da.size(1);
-  TORCH_CHECK(F % 2 == 0 && gu.size(1) == 2 * F && da.is_contiguous() && gu.is_contiguous(), "swiglu_bwd shapes");
+  for (const torch::Tensor* t : {&da, &gu, &dgu})
+    TORCH_CHECK(t->device() == da.device() && t->is_cuda() && t->scalar_type() == at::kBFloat16 && t->dim() == 2 &&
+                    t->is_contiguous() && t->size(0) == M && t->size(1) == (t == &da ? F : 2L * F),
+                "swiglu_bwd: contiguous bf16 [tokens, F] and [tokens, 2 F] on one GPU");
   const long total = (long)M * F / 2;
-  if (total == 0) return;
-  if (F % 8 == 0 && (reinterpret_cast<uintptr_t>(da.data_ptr()) & 15) == 0 &&
-      (reinterpret_cast<uintptr_t>(gu.data_ptr()) & 15) == 0 && (reinterpret_cast<uintptr_t>(dgu.data_ptr()) & 15) == 0) {
+  if (M == 0 || F == 0) return;
+  const uintptr_t bases = reinterpret_cast<uintptr_t>(da.data_ptr()) | reinterpret_cast<uintptr_t>(gu.data_ptr()) |
+                          reinterpret_cast<uintptr_t>(dgu.data_ptr());
+  if (F % 2 != 0 || (bases & 3) != 0) {
+    swiglu_bwd_one_kernel<<<grid_for((long)M * F, 256), 256, 0, cur_stream()>>>(
+        reinterpret_cast<const __nv_bfloat16*>(da.data_ptr()), reinterpret_cast<const __nv_bfloat16*>(gu.data_ptr()),
+        reinterpret_cast<__nv_bfloat16*>(dgu.data_ptr()), M, F);
+    DTB_LAUNCH_CHECK();
+    return;
+  }
+  if (F % 8 == 0 && (bases & 15) == 0) {
     swiglu_bwd_vec8_kernel<<<grid_for(total / 4, 256), 256, 0, cur_stream()>>>(
         reinterpret_cast<const __nv_bfloat16*>(da.data_ptr()), reinterpret_cast<const __nv_bfloat16*>(gu.data_ptr()),
         reinterpret_cast<__nv_bfloat16*>(dgu.data_ptr()), M, F);

@@ -300,3 +300,52 @@ def test_native_log_probs_refuse_such_temperatures():
     for t in (0.0, 1e-40, float("inf"), float("nan")):
         with pytest.raises(RuntimeError, match="temperature"):
             native().token_logprobs(x, tok, t, 0, -100)
+
+
+@pytest.mark.parametrize("T,ffn", [(1, 1), (30, 37), (129, 1001)])
+def test_packed_swiglu_of_an_odd_width(T, ffn):
+    from build_your_own_distributed_training_b200.ops.linear import swiglu_packed
+    gu = (_randn(T, 2 * ffn, seed=1) * 2).to(BF).requires_grad_(True)
+    da = _randn(T, ffn, seed=2, dt=BF)
+    act = swiglu_packed(gu, ffn)
+    act.backward(da)
+    gd = gu.detach().double().requires_grad_(True)
+    ref = torch.nn.functional.silu(gd[:, :ffn]) * gd[:, ffn:]
+    ref.backward(da.double())
+    # fp32 arithmetic and one rounding
+    assert rel(act, ref) < UNIT[BF] + 2.0 ** -18 and rel(gu.grad, gd.grad) < UNIT[BF] + 2.0 ** -18
+
+
+@pytest.mark.parametrize("ffn", [64, 38, 37])
+@pytest.mark.parametrize("off", [1, 2, 8])
+def test_packed_swiglu_of_tensors_off_the_vector_grid(ffn, off):
+    from build_your_own_distributed_training_b200.ops.linear import swiglu_backward, swiglu_packed
+    T = 21
+    shifted = lambda t: torch.empty(t.numel() + off, device=DEV, dtype=BF)[off:].view(t.shape).copy_(t)  # noqa: E731
+    gu, da = (_randn(T, 2 * ffn, seed=1) * 2).to(BF), _randn(T, ffn, seed=2, dt=BF)
+    want = swiglu_backward(da, gu, ffn)
+    assert torch.equal(swiglu_packed(shifted(gu), ffn), swiglu_packed(gu, ffn))
+    for a, b in ((shifted(da), gu), (da, shifted(gu)), (shifted(da), shifted(gu))):
+        assert torch.equal(swiglu_backward(a, b, ffn), want)
+
+
+def test_8_bit_model_of_an_odd_width_trains():
+    from build_your_own_distributed_training_b200.config import ModelConfig, ParallelConfig
+    from build_your_own_distributed_training_b200.models import TransformerBlock, build_model, set_fp8_linear
+    from build_your_own_distributed_training_b200.parallel.fsdp import FullyShardedModel
+    torch.manual_seed(0)
+    mc = ModelConfig(vocab_size=512, d_model=128, n_layers=1, n_heads=2, n_kv_heads=1, ffn_hidden_size=301,
+                     max_seq_len=64, tie_embeddings=False)
+    ref, model = set_fp8_linear(build_model(mc)), set_fp8_linear(build_model(mc))
+    model.load_state_dict(ref.state_dict())
+    eng = FullyShardedModel(model, None, ParallelConfig(), {TransformerBlock}, device=DEV)
+    model.rope_cos, model.rope_sin = model.rope_cos.to(DEV), model.rope_sin.to(DEV)
+    model.return_logits = False
+    x, y = torch.randint(0, 512, (2, 3, 50), generator=torch.Generator().manual_seed(1))
+    _, a = eng(x.to(DEV), labels=y.to(DEV))
+    a.backward()
+    _, b = ref(x, labels=y)
+    b.backward()
+    assert abs(float(a.detach()) - float(b.detach())) < 0.01
+    for (n, p), (_, q) in zip(eng.module.named_parameters(), ref.named_parameters()):
+        assert rel(p.main_grad, q.grad) < 0.15, n  # roundings to 4 bits that fall differently
