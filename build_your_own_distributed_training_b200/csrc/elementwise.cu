@@ -787,7 +787,13 @@ torch::Tensor rmsnorm_bwd(torch::Tensor dy, torch::Tensor x, torch::Tensor w, to
 
 void rope_apply(torch::Tensor x, torch::Tensor cos_t, torch::Tensor sin_t, int64_t rope_cols, int64_t hd,
                 int64_t seqlen, double sign) {
-  TORCH_CHECK(x.scalar_type() == at::kBFloat16 && x.stride(1) == 1, "rope: bf16 rows");
+  TORCH_CHECK(x.is_cuda() && x.dim() == 2 && x.scalar_type() == at::kBFloat16 && x.stride(1) == 1, "rope: bf16 rows");
+  TORCH_CHECK(hd > 0 && hd % 2 == 0 && rope_cols % hd == 0 && rope_cols >= 0 && rope_cols <= x.size(1) && seqlen > 0,
+              "rope: whole heads of an even size within the rows");
+  for (const torch::Tensor* t : {&cos_t, &sin_t})
+    TORCH_CHECK(t->device() == x.device() && t->scalar_type() == at::kFloat && t->is_contiguous() && t->dim() == 2 &&
+                    t->size(1) == hd && t->size(0) >= std::min<int64_t>(seqlen, x.size(0)),
+                "rope: tables are contiguous fp32 [positions, head_dim] on the rows' device, one row per position");
   const c10::cuda::CUDAGuard g(x.device());
   const int M = (int)x.size(0);
   const long total = (long)M * rope_cols / 2;

@@ -349,3 +349,18 @@ def test_8_bit_model_of_an_odd_width_trains():
     assert abs(float(a.detach()) - float(b.detach())) < 0.01
     for (n, p), (_, q) in zip(eng.module.named_parameters(), ref.named_parameters()):
         assert rel(p.main_grad, q.grad) < 0.15, n  # roundings to 4 bits that fall differently
+
+
+def test_packed_rotation_refuses_tables_it_cannot_read():
+    from build_your_own_distributed_training_b200.ops.rope import rope_packed
+    cos, sin = ops.precompute_rope_cache(16, 8, 10000.0)
+    x, c, s = _randn(16, 64, dt=BF), cos.to(DEV), sin.to(DEV)
+    for args in ((cos, sin, 48, 16, 8),                   # tables on the host
+                 (c[:4], s[:4], 48, 16, 8),               # fewer rows than positions
+                 (c.double(), s.double(), 48, 16, 8),
+                 (c[:, :8].contiguous(), s[:, :8].contiguous(), 48, 16, 8),
+                 (c, s, 80, 16, 8), (c, s, 40, 16, 8)):   # columns past the rows, half a head
+        with pytest.raises(RuntimeError, match="rope"):
+            rope_packed(x, *args)
+    assert rope_packed(x, c, s, 48, 16, 8).isfinite().all()
+    assert rope_packed(x[:4], c[:4], s[:4], 48, 16, 8).isfinite().all()  # four tokens read four rows
