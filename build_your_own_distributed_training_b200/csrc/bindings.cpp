@@ -148,7 +148,7 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("token_logprobs_bwd", &token_logprobs_bwd);
   m.def("fp8_quantize", &fp8_quantize, "e4m3 codes with a power-of-two scale per block of 128, as they lie and / or transposed");
   m.def("fp8_scale_tiles", &fp8_scale_tiles, "scale tiles for fp8_gemm from plain e8m0 scales");
-  m.def("fp8_product", &fp8_product, "product of e4m3 operands by the kernel that fits their number of rows");
+  m.def("fp8_product", &fp8_product, "product of e4m3 operands as a user holds them: plain scales, rows of any alignment");
   m.def("linear_fp8_kept", &linear_fp8_kept, "8-bit linear layer with kept 8-bit weights");
   m.def("fp8_gemm", &fp8_gemm, "tcgen05 block-scaled product of e4m3 operands");
   m.def("swiglu_fwd", &swiglu_fwd, "silu(g) * u of packed [g | u]");

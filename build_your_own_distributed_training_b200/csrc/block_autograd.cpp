@@ -190,12 +190,15 @@ Tensor linear_fp8_autograd(Tensor x, Tensor w, c10::optional<Tensor> residual) {
 
 // ValueError unless q is e4m3 [rows, cols] and s its e8m0 scales in 1 x 128 or 128 x 128 blocks.
 void fp8_check_blocks(const Tensor& q, const Tensor& s) {
-  TORCH_CHECK_VALUE(q.dim() == 2 && q.scalar_type() == at::kFloat8_e4m3fn && s.scalar_type() == at::kFloat8_e8m0fnu,
-                    "8-bit blocks are e4m3 [rows, cols] codes with e8m0 scales, got ", q.scalar_type(), " and ", s.scalar_type());
+  char msg[160];
+  if (q.dim() != 2 || q.scalar_type() != at::kFloat8_e4m3fn || s.scalar_type() != at::kFloat8_e8m0fnu) {
+    std::snprintf(msg, sizeof(msg), "8-bit blocks are e4m3 [rows, cols] codes with e8m0 scales, got %s and %s",
+                  c10::toString(q.scalar_type()), c10::toString(s.scalar_type()));
+    TORCH_CHECK_VALUE(false, msg);
+  }
   const long rows = q.size(0), cols = q.size(1), blocks = (rows + 127) / 128;
   const long sr = s.dim() > 0 ? s.size(0) : 0, sc = s.dim() > 1 ? s.size(1) : 0;
   if (s.dim() == 2 && (sr == blocks || sr == rows) && sc == (cols + 127) / 128) return;
-  char msg[160];
   std::snprintf(msg, sizeof(msg), "scales [%ld, %ld] fit neither 1 x 128 nor 128 x 128 blocks of %ld x %ld", sr, sc, rows, cols);
   TORCH_CHECK_VALUE(false, msg);
 }

@@ -9,7 +9,7 @@
 // rows of A and 128 columns of B.  Small ones run on single CTAs with 128 x 128 tiles.
 //   warp 0       TMA: 128 x 128-byte tiles of A and B (128-byte swizzle) and their scale tiles into a 6-stage
 //                ring;
-//   warp 1       one thread issues, per stage, the tcgen05.cp of the stage's scales (shared memory -> tensor
+//   warp 1       an elected lane issues, per stage, the tcgen05.cp of the stage's scales (shared memory -> tensor
 //                memory) and four block-scaled MMAs (kind::mxf8f6f4, 32 deep);
 //   warps 2-9    epilogue: two warpgroups, each half of the tile's columns.
 // The hardware applies a scale to 32 elements, one byte of a row's 32-bit scale word; a block of 128 is four

@@ -12,8 +12,8 @@
 // thread), and writes the codes as they lie and transposed, so that both products get operands whose
 // summed axis is contiguous.  2 bytes in, 1 or 2 bytes out per element: 8192 x 4096 bf16 takes 24 us as it
 // lies, 34 us both ways (4.0 TB/s), 25 us both ways in 128 x 128 blocks, whose one scale lets the transposed
-// codes be byte permutes of the others.  The 1 x 128 form is bound by its instructions (two products and two
-// conversions an element); magnitudes go two elements at a time (71 us before).  The transposed
+// codes be byte permutes of the others.  The 1 x 128 form uses 67% of the issue slots: a product by the
+// scale and a conversion for each of an element's two codes.  Magnitudes go two elements at a time (71 us before).  The transposed
 // codes go through 16 KB of shared memory in 8-byte chunks (8 rows of one column) at chunk
 // rg ^ (column / 8), which is free of bank conflicts on the way in, and leave as 16-byte stores.
 //

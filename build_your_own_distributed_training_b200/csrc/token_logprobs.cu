@@ -16,8 +16,9 @@
 // an excluded logit (-inf) then adds exactly nothing to S and A.
 //
 // 4096 x 32000 fp32 without alternatives: forward 86 us (6.1 TB/s, memory), backward 144 us.  777 x 32003 bf16
-// with 5 alternatives: 35 and 21 us, bound by instructions (a 16-byte vector holds 8 exponentials) and, per
-// row, by the sorts.  One row of 128256 fp32 with 20 alternatives: 11 us in a cluster of 8, all latency.
+// with 5 alternatives: 35 and 21 us.  A thread of the 512 sees 8 vectors of such a row, so the forward's merges
+// weigh as much as the elements (53% of the issue slots, warps wait at barriers most); the backward uses 67%
+// of the slots, one element at a time.  One row of 128256 fp32 with 20 alternatives: 11 us in a cluster of 8, all latency.
 //
 // Top k (k <= 32) without sorting the row: the k largest thread maxima name the k threads that can
 // own one of the k largest elements, and the k-th of these maxima is a lower bound for all of them;

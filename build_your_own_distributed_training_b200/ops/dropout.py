@@ -66,7 +66,7 @@ def dropout_add(x: torch.Tensor, residual: torch.Tensor | None, p: float, seed: 
     ``seed``: 64 bits; draw a new one per call site and step (on the host, e.g. from torch's CPU
     generator, whose state activation checkpointing restores before it recomputes).  ``start``: the
     element number of ``x``'s first element within the whole activation.  A captured CUDA graph
-    replays the seed it was captured with.
+    replays the seed it was captured with.  Differentiable any number of times (the mask is a constant).
     """
     if not 0.0 <= p <= 1.0:
         raise ValueError(f"dropout probability {p} is outside [0, 1]")

@@ -187,6 +187,10 @@ def linear_fp8(x: torch.Tensor, weight: torch.Tensor | Fp8Blocks, *, residual: t
     A weight tensor is quantised in the call and gets its gradient (into ``main_grad`` when given);
     kept :class:`Fp8Blocks` are for inference.  On CUDA ``x`` and ``residual`` are bf16; keep the rows
     of ``Fp8Blocks.values`` on 16-byte boundaries (:func:`quantize_fp8` does), others are copied first.
+
+    The backward needs codes of ``x`` and of the weight along their other axes.  Those of ``x`` (a byte an
+    element) are kept from the forward, and so are the weight's, unless it comes with ``main_grad``: then the
+    weight itself is kept and quantised again.  The rounded product has no second derivative (refused).
     """
     K = weight.values.shape[1] if isinstance(weight, Fp8Blocks) else weight.shape[1]
     N = weight.values.shape[0] if isinstance(weight, Fp8Blocks) else weight.shape[0]

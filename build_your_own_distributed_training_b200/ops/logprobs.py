@@ -123,7 +123,8 @@ def token_log_probs(logits: torch.Tensor, tokens: torch.Tensor, *, temperature: 
                     ignore_index: int = IGNORE) -> TokenLogProbs:
     """``logits [..., V]`` (fp32, bf16, fp16), ``tokens [...]`` int64 -> :class:`TokenLogProbs`.
 
-    Differentiable in ``logprob`` and ``entropy``.  Forbidden tokens may be ``-inf`` or the type's
+    Differentiable in ``logprob`` and ``entropy`` (twice on the CPU alone; on CUDA second derivatives and
+    tangents are refused).  Forbidden tokens may be ``-inf`` or the type's
     lowest value.  Rows whose token is ``ignore_index`` give 0, 0, alternatives ``-1`` at ``-inf``, and
     no gradient; a row with every logit at ``-inf`` gives ``-inf``, entropy 0 and no gradient; NaN or
     +inf in a row, or a token outside the vocabulary (which also sets the device error word), gives NaN.

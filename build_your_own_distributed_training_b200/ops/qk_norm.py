@@ -135,7 +135,8 @@ def qk_norm_rope(qkv: torch.Tensor, q_weight: torch.Tensor, k_weight: torch.Tens
     sequences, decoding) of the fp32 tables ``cos``/``sin`` ``[positions, hd]``; a position outside
     the tables gives NaN and sets the device error word.  ``qkv`` is fp32, bf16 or fp16 with any row
     stride; the weights share one float type.  With ``main_grads`` (the engine's fp32 gradient views
-    of the two weights) the weight gradients are added there.
+    of the two weights) the weight gradients are added there.  On CUDA, and with ``main_grads``, second
+    derivatives and tangents are refused.
     """
     if qkv.dim() != 2 or qkv.shape[1] != (n_q_heads + 2 * n_kv_heads) * head_dim:
         raise ValueError(f"qkv must be [tokens, {(n_q_heads + 2 * n_kv_heads) * head_dim}], got {tuple(qkv.shape)}")

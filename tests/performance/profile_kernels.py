@@ -353,6 +353,19 @@ def case_token_log_probs():
     return run, 0, 3 * x.numel() * 4
 
 
+def case_token_log_probs_16():
+    # 16-bit rows of an odd vocabulary in a padded buffer, with alternatives (50 MB: stays in the L2)
+    x = (torch.randn(777, 32064, device=DEV) * 2.5).to(BF)[:, :32003]
+    tok = torch.randint(0, 32003, (777,), device=DEV)
+    g = torch.ones(777, device=DEV)
+    dx = torch.empty(777, 32064, device=DEV, dtype=BF)[:, :32003]
+
+    def run():
+        state = native().token_logprobs_fwd(x, tok, 0.7, 5, -100, True)[-1]
+        native().token_logprobs_bwd(x, tok, state, g, g, 0.7, dx)
+    return run, 0, 3 * x.numel() * 2
+
+
 CASES = {k[5:]: v for k, v in globals().items() if k.startswith("case_")}
 
 
