@@ -152,14 +152,15 @@ class _LinearFp8Fn(torch.autograd.Function):
 
     @staticmethod
     def backward(ctx, dy):  # type: ignore[override]
+        saved = ctx.saved_tensors  # once: recomputed under activation checkpointing
         with torch.no_grad():
-            dx, dw = _LinearFp8Fn._gradients(ctx, dy)
-        dx, dw = (first_order("linear_fp8", t, (dy,), *(s for s in ctx.saved_tensors[6:] if s is not None)) for t in (dx, dw))
+            grads = _LinearFp8Fn._gradients(ctx, saved, dy)
+        inputs = [t for t in saved[6:] if t is not None]
+        dx, dw = (first_order("linear_fp8", t, (dy,), *inputs) for t in grads)
         return dx, dw, (dy if ctx.need[2] else None), None, None
 
     @staticmethod
-    def _gradients(ctx, dy):
-        saved = ctx.saved_tensors
+    def _gradients(ctx, saved, dy):
         need_x, need_w, _ = ctx.need
         dy2 = dy.contiguous()
         dx = dw = None

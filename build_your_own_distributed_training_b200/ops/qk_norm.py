@@ -82,15 +82,16 @@ class _QKNormRopeFn(torch.autograd.Function):
 
     @staticmethod
     def backward(ctx, g):  # type: ignore[override]
+        saved = ctx.saved_tensors  # once: recomputed under activation checkpointing
         if not g.is_cuda and ctx.main_grads is None and ctx.reduce is None:
-            return _QKNormRopeFn._gradients(ctx, g) + (None,) * 10  # plain differentiable operations
+            return _QKNormRopeFn._gradients(ctx, saved, g) + (None,) * 10  # plain differentiable operations
         with torch.no_grad():
-            grads = _QKNormRopeFn._gradients(ctx, g)
-        return tuple(first_order("qk_norm_rope", t, (g,), *ctx.saved_tensors[:3]) for t in grads) + (None,) * 10
+            grads = _QKNormRopeFn._gradients(ctx, saved, g)
+        return tuple(first_order("qk_norm_rope", t, (g,), *saved[:3]) for t in grads) + (None,) * 10
 
     @staticmethod
-    def _gradients(ctx, g):
-        qkv, wq, wk, cos, sin, positions = ctx.saved_tensors
+    def _gradients(ctx, saved, g):
+        qkv, wq, wk, cos, sin, positions = saved
         nq, nkv, hd, seqlen, eps = ctx.cfg
         mgs = ctx.main_grads
         if mgs is not None:

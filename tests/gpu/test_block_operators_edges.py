@@ -364,3 +364,29 @@ def test_packed_rotation_refuses_tables_it_cannot_read():
             rope_packed(x, *args)
     assert rope_packed(x, c, s, 48, 16, 8).isfinite().all()
     assert rope_packed(x[:4], c[:4], s[:4], 48, 16, 8).isfinite().all()  # four tokens read four rows
+
+
+@pytest.mark.parametrize("score", [False, True])
+def test_recomputed_blocks_give_the_same_gradients(score):
+    """Activation checkpointing runs a block again in its backward: same kernels, inputs and seeds, same bits."""
+    from build_your_own_distributed_training_b200.config import ModelConfig, ParallelConfig
+    from build_your_own_distributed_training_b200.models import TransformerBlock, build_model, set_fp8_linear
+    from build_your_own_distributed_training_b200.parallel.fsdp import FullyShardedModel, apply_activation_checkpointing
+    x, y = torch.randint(0, 512, (2, 2, 64), generator=torch.Generator().manual_seed(1)).to(DEV)
+    seen = []
+    for ckpt in (False, True):
+        torch.manual_seed(0)
+        model = set_fp8_linear(build_model(ModelConfig(
+            vocab_size=512, d_model=256, n_layers=2, n_heads=4, n_kv_heads=2, ffn_hidden_size=512, max_seq_len=64,
+            tie_embeddings=False, qk_norm=True, resid_dropout=0.2)))
+        if ckpt:
+            apply_activation_checkpointing(model, {TransformerBlock})
+        eng = FullyShardedModel(model, None, ParallelConfig(), {TransformerBlock}, device=DEV)
+        model.rope_cos, model.rope_sin = model.rope_cos.to(DEV), model.rope_sin.to(DEV)
+        model.return_logits = False
+        eng.train()
+        torch.manual_seed(3)
+        loss = -eng(x, targets=y).logprob.mean() if score else eng(x, labels=y)[1]
+        loss.backward()
+        seen.append([loss.detach()] + [p.main_grad.clone() for p in model.parameters()])
+    assert all(torch.equal(a, b) for a, b in zip(*seen))

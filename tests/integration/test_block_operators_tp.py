@@ -47,3 +47,34 @@ def _worker(rank, world, sp, qk):
 @pytest.mark.parametrize("qk", [False, True])
 def test_fp8_gradients_under_tensor_parallelism(sp, qk):
     run_distributed(_worker, 2, sp, qk)
+
+
+def _sharded_worker(rank, world, ckpt):
+    cfg = tiny_config(model__d_model=256, model__n_layers=5, model__n_heads=4, model__n_kv_heads=4, model__ffn_hidden_size=512,
+                      model__qk_norm=True, kernels__fp8_linear=True, parallel__activation_checkpointing=ckpt,
+                      parallel__sharding_strategy="FULL_SHARD", parallel__limit_all_gathers=True)
+    ctx = build_process_context(1, backend="gloo", verbose=False)
+    eng = build_engine(cfg, ctx)
+    assert eng.shard_world == 2 and len({u.gathered.data_ptr() for u in eng.units}) < len(eng.units)  # slots are shared
+    torch.manual_seed(cfg.seed)
+    ref = set_fp8_linear(build_model(cfg.model))
+    t = torch.randint(0, cfg.model.vocab_size, (4, 65), generator=torch.Generator().manual_seed(1))
+    x, y = t[:, :-1], t[:, 1:]  # the same tokens on both ranks, so the mean gradient is either's
+    _, a = eng(x, labels=y)
+    a.backward()
+    _, b = ref(x, labels=y)
+    b.backward()
+    assert abs(float(a.detach()) - float(b.detach())) < 1e-5
+    grads = dict((n, p.grad) for n, p in ref.named_parameters())
+    for u in eng.units:
+        want = torch.zeros(u.numel)
+        for e in u.entries:
+            want[e.offset:e.offset + e.numel] = grads[e.fqn].reshape(-1)
+        lo, hi = u.shard_range(rank)
+        assert rel(u.grad_shard, want[lo:hi]) < 2.0 ** -18, u.name
+
+
+@pytest.mark.parametrize("ckpt", [False, True])
+def test_fp8_gradients_with_gathered_weights_freed_in_between(ckpt):
+    """Five blocks share two gather slots: the backward quantises weights that were gathered again."""
+    run_distributed(_sharded_worker, 2, ckpt)
